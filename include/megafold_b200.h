@@ -267,6 +267,97 @@ MF_API int mf_gate_bwd(const void* d, const void* o, const void* g, int64_t g_st
 MF_API int mf_bias_layout(void* rows, void* planes, int32_t L, int32_t np, int32_t H, int32_t swap, int32_t to_rows, int32_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Positions in attention.  (No counterpart among the reference's fused operators; they stand where it leaves torch to it: the
+ * relative position encoding of the pair representation and the windowed attention over atoms, attention.py:260-394.)
+ *
+ * Relative position bias:  bias[b,0,h,i,j] = weight[row, h],  row = bucket of d = k_pos[b,j] - q_pos[b,i], or rows - 1 where
+ * q_seg[b,i] != k_seg[b,j].  With m = the number of edges that are <= |d|:  row = base_pos + step_pos * m where d > 0, else
+ * base_neg + step_neg * m (kept within the table).  Differences of positions have to fit 64 bits.
+ *
+ * weight [rows, H] in w_dtype (fp32 or any other floating type), contiguous; rows <= MF_RELPOS_MAX_ROWS.
+ * edges: n_edges ascending positive distances in HOST memory, the last at most MF_RELPOS_MAX_DISTANCE.
+ * q_pos [B, Lq], k_pos [B, Lk]: pos_bytes (4 or 8) wide integers, elements adjacent, `*_stride` elements between batches (0: shared);
+ * both NULL: key j at j, query i at i + Lk - Lq.  q_seg, k_seg likewise (seg_bytes), both NULL: one segment.
+ * bias, d_bias: contiguous [B,1,H,Lq,Lk] in `dtype`.  d_weight [rows, H] in dw_dtype, fully overwritten, summed in a fixed
+ * order (bit-reproducible).  workspace (backward): mf_relpos_bwd_workspace_bytes() bytes, 256-byte aligned.
+ * ------------------------------------------------------------------------------------------ */
+#define MF_RELPOS_MAX_EDGES 512
+#define MF_RELPOS_MAX_ROWS 1024
+#define MF_RELPOS_MAX_DISTANCE 16384
+typedef struct mf_relpos_args {
+  int32_t B, H, Lq, Lk, rows;
+  int32_t dtype, w_dtype, dw_dtype;
+  int32_t n_edges, base_pos, step_pos, base_neg, step_neg;
+  int32_t pos_bytes, seg_bytes;
+  const int32_t* edges;
+  const void* q_pos; const void* k_pos; int64_t q_pos_stride, k_pos_stride;
+  const void* q_seg; const void* k_seg; int64_t q_seg_stride, k_seg_stride;
+  const void* weight; void* bias;
+  const void* d_bias; void* d_weight;
+  void* workspace; size_t workspace_bytes;
+} mf_relpos_args;
+
+MF_API int mf_relpos_fwd(const mf_relpos_args* args, void* stream);
+MF_API size_t mf_relpos_bwd_workspace_bytes(const mf_relpos_args* args);
+MF_API int mf_relpos_bwd(const mf_relpos_args* args, void* stream);
+
+/*
+ * RMS norm of every head of queries and keys and their rotation by position:
+ *   y = x * (mean_d x^2 + eps)^-1/2 * weight;  of y's first R elements, pair k (elements k and k + R/2, or 2k and 2k + 1 with
+ *   `interleaved`) is turned by the angle position * inv_freq[k], formed in 64 bits; the others stay.
+ * q [B,N,L,H,D] and k [B,N,L,Hk,D] with arbitrary element strides; D <= 256, R even, R <= D.
+ * q_weight, k_weight: [D], or with per_head [H,D] and [Hk,D], contiguous in w_dtype; both NULL: ones.  inv_freq: fp32 [R/2].
+ * positions: pos_bytes (4 or 8) wide integers with element strides (b, n, l); NULL: the index along L.
+ * q_out, k_out, dq_out, dk_out, dq, dk: contiguous, in `dtype`.  dq_weight, dk_weight: as the weights (NULL without), fully
+ * overwritten, summed in a fixed order.  workspace (backward): mf_qk_rotary_bwd_workspace_bytes() bytes, 256-byte aligned.
+ */
+typedef struct mf_qk_rotary_args {
+  int32_t B, N, L, H, Hk, D, R;
+  int32_t dtype, w_dtype, per_head, interleaved, pos_bytes;
+  float eps;
+  const void* q; const void* k; int64_t q_strides[5], k_strides[5];
+  const void* q_weight; const void* k_weight; const float* inv_freq;
+  const void* positions; int64_t pos_strides[3];
+  void* q_out; void* k_out;
+  const void* dq_out; const void* dk_out; void* dq; void* dk; void* dq_weight; void* dk_weight;
+  void* workspace; size_t workspace_bytes;
+} mf_qk_rotary_args;
+
+MF_API int mf_qk_rotary_fwd(const mf_qk_rotary_args* args, void* stream);
+MF_API size_t mf_qk_rotary_bwd_workspace_bytes(const mf_qk_rotary_args* args);
+MF_API int mf_qk_rotary_bwd(const mf_qk_rotary_args* args, void* stream);
+
+/*
+ * Attention with a sliding window and sinks: query i, at position p = i + Lk - Lq, sees key j iff j <= p + right and
+ * (j >= p - left or j < sinks) and its mask is set;  o = softmax(D^-1/2 q . k over the seen keys) v.  A query that sees no key
+ * gives 0 and a log-sum-exp of -inf, and passes no gradient.  Query head h reads key head h / (H / Hk).
+ *
+ * q [B,N,Lq,H,D], k and v [B,N,Lk,Hk,D] with arbitrary element strides; D <= 128, H a multiple of Hk, Lq and Lk <= 2^29.
+ * left, right, sinks >= 0 (INT32_MAX: no bound).  mask: MF_U8 keep-mask with element strides (b, n, l), NULL: every key is
+ * kept.  What masked keys hold (NaN, too) reaches nothing.
+ * o, d_o, dq [B,N,Lq,H,D], dk, dv [B,N,Lk,Hk,D]: contiguous in `dtype`; lse: fp32 [B,N,H,Lq], may be NULL on the forward.
+ * Every result is summed in a fixed order (bit-reproducible).  workspace: mf_window_fwd_workspace_bytes() /
+ * mf_window_bwd_workspace_bytes() bytes (0: none needed), 256-byte aligned.
+ */
+typedef struct mf_window_args {
+  int32_t B, N, Lq, Lk, H, Hk, D;
+  int32_t left, right, sinks;
+  int32_t dtype;
+  uint32_t flags;
+  const void* q; const void* k; const void* v;
+  int64_t q_strides[5], k_strides[5], v_strides[5];
+  const void* mask; int64_t mask_strides[3];
+  void* o; float* lse;
+  const void* d_o; void* dq; void* dk; void* dv;
+  void* workspace; size_t workspace_bytes;
+} mf_window_args;
+
+MF_API size_t mf_window_fwd_workspace_bytes(const mf_window_args* args);
+MF_API int mf_window_fwd(const mf_window_args* args, void* stream);
+MF_API size_t mf_window_bwd_workspace_bytes(const mf_window_args* args);
+MF_API int mf_window_bwd(const mf_window_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Type conversion of several contiguous arrays (fp32, bf16, fp16 in any combination) in one launch, for hosts that
  * hold their parameters in another type than the one they compute in.  n_items <= MF_CAST_MAX.
  * (No counterpart in the reference, which leaves these conversions to torch: fused_layernorm_linear.py:480.)

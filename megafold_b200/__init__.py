@@ -2,6 +2,7 @@
 
 Public names follow the reference: ``TritonEvoformer`` / ``EvoformerAttention``,
 ``LayernormLinear`` / ``LayernormLinearFunction``, ``FusedTransition`` / ``FusedSwiGLU``.
+Beside them stand operators for positions in attention: ``relative_position_bias``, ``qk_norm_rotary``, ``window_attention``.
 Everything runs in hand-written CUDA behind a C ABI (include/megafold_b200.h); there is no CPU
 or library fallback.
 """
@@ -12,11 +13,16 @@ from .fused_transition import (FusedSwiGLU, FusedSwiGLUFunction, FusedTransition
                                transition_backward, transition_forward)
 from .host_pipeline import evoformer_fwd_bwd_host
 from .pairformer_block import PairformerBlock
+from .qk_rotary import QKNormRotary, qk_norm_rotary
+from .relative_position import RelativePositionBias, relative_position_bias
 from .sharded import AllReduceGradient, row_shard, sharded_evoformer
+from .window_attention import window_attention, window_attention_backward, window_attention_forward
 
 __all__ = [
     "EvoformerAttention", "TritonEvoformer", "evo_attention_forward", "evo_attention_backward",
     "LayernormLinear", "LayernormLinearFunction", "FusedSwiGLU", "FusedSwiGLUFunction", "FusedTransition",
     "TransitionFunction", "layernorm_linear_forward", "layernorm_linear_backward", "transition_forward",
     "transition_backward", "AllReduceGradient", "row_shard", "sharded_evoformer", "evoformer_fwd_bwd_host", "PairformerBlock",
+    "relative_position_bias", "RelativePositionBias", "qk_norm_rotary", "QKNormRotary",
+    "window_attention", "window_attention_forward", "window_attention_backward",
 ]

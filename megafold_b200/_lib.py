@@ -85,6 +85,39 @@ class CastItem(C.Structure):
     _fields_ = [("src", _vp), ("dst", _vp), ("n", _i64), ("src_dtype", _i32), ("dst_dtype", _i32)]
 
 
+class RelposArgs(C.Structure):
+    _fields_ = [("B", _i32), ("H", _i32), ("Lq", _i32), ("Lk", _i32), ("rows", _i32),
+                ("dtype", _i32), ("w_dtype", _i32), ("dw_dtype", _i32),
+                ("n_edges", _i32), ("base_pos", _i32), ("step_pos", _i32), ("base_neg", _i32), ("step_neg", _i32),
+                ("pos_bytes", _i32), ("seg_bytes", _i32),
+                ("edges", C.POINTER(_i32)),
+                ("q_pos", _vp), ("k_pos", _vp), ("q_pos_stride", _i64), ("k_pos_stride", _i64),
+                ("q_seg", _vp), ("k_seg", _vp), ("q_seg_stride", _i64), ("k_seg_stride", _i64),
+                ("weight", _vp), ("bias", _vp), ("d_bias", _vp), ("d_weight", _vp),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class QkRotaryArgs(C.Structure):
+    _fields_ = [("B", _i32), ("N", _i32), ("L", _i32), ("H", _i32), ("Hk", _i32), ("D", _i32), ("R", _i32),
+                ("dtype", _i32), ("w_dtype", _i32), ("per_head", _i32), ("interleaved", _i32), ("pos_bytes", _i32), ("eps", _f32),
+                ("q", _vp), ("k", _vp), ("q_strides", _i64 * 5), ("k_strides", _i64 * 5),
+                ("q_weight", _vp), ("k_weight", _vp), ("inv_freq", _vp),
+                ("positions", _vp), ("pos_strides", _i64 * 3),
+                ("q_out", _vp), ("k_out", _vp),
+                ("dq_out", _vp), ("dk_out", _vp), ("dq", _vp), ("dk", _vp), ("dq_weight", _vp), ("dk_weight", _vp),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class WindowArgs(C.Structure):
+    _fields_ = [("B", _i32), ("N", _i32), ("Lq", _i32), ("Lk", _i32), ("H", _i32), ("Hk", _i32), ("D", _i32),
+                ("left", _i32), ("right", _i32), ("sinks", _i32), ("dtype", _i32), ("flags", _u32),
+                ("q", _vp), ("k", _vp), ("v", _vp),
+                ("q_strides", _i64 * 5), ("k_strides", _i64 * 5), ("v_strides", _i64 * 5),
+                ("mask", _vp), ("mask_strides", _i64 * 3),
+                ("o", _vp), ("lse", _vp), ("d_o", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
 # every symbol include/megafold_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "mf_evo_fwd": (C.c_int, [C.POINTER(EvoFwdArgs), _vp]),
@@ -109,6 +142,16 @@ SYMBOLS = {
     "mf_transition_fwd": (C.c_int, [C.POINTER(TransitionFwdArgs), _vp]),
     "mf_transition_bwd_workspace_bytes": (_sz, [C.POINTER(TransitionBwdArgs)]),
     "mf_transition_bwd": (C.c_int, [C.POINTER(TransitionBwdArgs), _vp]),
+    "mf_relpos_fwd": (C.c_int, [C.POINTER(RelposArgs), _vp]),
+    "mf_relpos_bwd_workspace_bytes": (_sz, [C.POINTER(RelposArgs)]),
+    "mf_relpos_bwd": (C.c_int, [C.POINTER(RelposArgs), _vp]),
+    "mf_qk_rotary_fwd": (C.c_int, [C.POINTER(QkRotaryArgs), _vp]),
+    "mf_qk_rotary_bwd_workspace_bytes": (_sz, [C.POINTER(QkRotaryArgs)]),
+    "mf_qk_rotary_bwd": (C.c_int, [C.POINTER(QkRotaryArgs), _vp]),
+    "mf_window_fwd_workspace_bytes": (_sz, [C.POINTER(WindowArgs)]),
+    "mf_window_fwd": (C.c_int, [C.POINTER(WindowArgs), _vp]),
+    "mf_window_bwd_workspace_bytes": (_sz, [C.POINTER(WindowArgs)]),
+    "mf_window_bwd": (C.c_int, [C.POINTER(WindowArgs), _vp]),
     "mf_cast_batch": (C.c_int, [C.POINTER(CastItem), _i32, _vp]),
     "mf_last_error_string": (C.c_char_p, []),
     "mf_version": (C.c_int, []),

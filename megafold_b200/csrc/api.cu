@@ -338,6 +338,126 @@ int mf_bias_layout(void* rows, void* planes, int32_t L, int32_t np, int32_t H, i
   return bias_layout(rows, planes, L, np, H, swap != 0, to_rows != 0, dtype, static_cast<cudaStream_t>(stream));
 }
 
+namespace {
+int check_relpos(const mf_relpos_args& a) {
+  MF_REQUIRE(a.B > 0 && a.H > 0 && a.Lq > 0 && a.Lk > 0, MF_ERR_BAD_ARG, "sizes must be positive (B=%d H=%d Lq=%d Lk=%d)", a.B, a.H, a.Lq, a.Lk);
+  MF_REQUIRE(float_dtype(a.dtype) && float_dtype(a.w_dtype), MF_ERR_BAD_ARG, "bias and weight must have floating types");
+  MF_REQUIRE(a.rows > 0 && a.rows <= MF_RELPOS_MAX_ROWS, MF_ERR_UNSUPPORTED, "a table of 1 to %d rows is supported, got %d", MF_RELPOS_MAX_ROWS, a.rows);
+  MF_REQUIRE(a.n_edges >= 0 && a.n_edges <= MF_RELPOS_MAX_EDGES && (a.n_edges == 0 || a.edges), MF_ERR_UNSUPPORTED, "at most %d edges are supported, got %d",
+             MF_RELPOS_MAX_EDGES, a.n_edges);
+  for (int i = 0; i < a.n_edges; ++i)
+    MF_REQUIRE(a.edges[i] >= (i ? a.edges[i - 1] : 1) && a.edges[i] <= MF_RELPOS_MAX_DISTANCE, MF_ERR_BAD_ARG,
+               "edges must be ascending distances of 1 to %d (edge %d is %d)", MF_RELPOS_MAX_DISTANCE, i, a.edges[i]);
+  MF_REQUIRE(!a.q_pos == !a.k_pos && !a.q_seg == !a.k_seg, MF_ERR_BAD_ARG, "positions and segments are given for queries and keys, or for neither");
+  MF_REQUIRE(!a.q_pos || a.pos_bytes == 4 || a.pos_bytes == 8, MF_ERR_BAD_ARG, "positions are 4 or 8 bytes wide");
+  MF_REQUIRE(!a.q_seg || a.seg_bytes == 4 || a.seg_bytes == 8, MF_ERR_BAD_ARG, "segments are 4 or 8 bytes wide");
+  MF_REQUIRE(a.H <= 65535, MF_ERR_UNSUPPORTED, "H=%d exceeds 65535", a.H);
+  return MF_OK;
+}
+int check_qk_rotary(const mf_qk_rotary_args& a) {
+  MF_REQUIRE(a.B > 0 && a.N > 0 && a.L > 0 && a.H > 0 && a.Hk > 0 && a.D > 0, MF_ERR_BAD_ARG, "sizes must be positive");
+  MF_REQUIRE(float_dtype(a.dtype) && (!a.q_weight || float_dtype(a.w_dtype)), MF_ERR_BAD_ARG, "q, k and the weights must have floating types");
+  MF_REQUIRE(a.D <= 256, MF_ERR_UNSUPPORTED, "head size %d > 256 is not supported", a.D);
+  MF_REQUIRE(a.R >= 0 && a.R <= a.D && a.R % 2 == 0, MF_ERR_BAD_ARG, "%d of %d elements cannot be rotated in pairs", a.R, a.D);
+  MF_REQUIRE(a.q && a.k && (a.R == 0 || a.inv_freq), MF_ERR_BAD_ARG, "q, k and inv_freq must not be NULL");
+  MF_REQUIRE(!a.q_weight == !a.k_weight, MF_ERR_BAD_ARG, "queries and keys both have a weight, or neither has");
+  MF_REQUIRE(!a.positions || a.pos_bytes == 4 || a.pos_bytes == 8, MF_ERR_BAD_ARG, "positions are 4 or 8 bytes wide");
+  MF_REQUIRE((int64_t)a.H + a.Hk <= 65535, MF_ERR_UNSUPPORTED, "more than 65535 heads");
+  return MF_OK;
+}
+int check_window(const mf_window_args& a) {
+  MF_REQUIRE(a.B > 0 && a.N > 0 && a.Lq > 0 && a.Lk > 0 && a.H > 0 && a.Hk > 0 && a.D > 0, MF_ERR_BAD_ARG,
+             "sizes must be positive (B=%d N=%d Lq=%d Lk=%d H=%d Hk=%d D=%d)", a.B, a.N, a.Lq, a.Lk, a.H, a.Hk, a.D);
+  MF_REQUIRE(float_dtype(a.dtype), MF_ERR_BAD_ARG, "q/k/v dtype %d is not a floating type", a.dtype);
+  MF_REQUIRE(a.H % a.Hk == 0, MF_ERR_BAD_ARG, "%d query heads cannot share %d key heads", a.H, a.Hk);
+  MF_REQUIRE(a.left >= 0 && a.right >= 0 && a.sinks >= 0, MF_ERR_BAD_ARG, "left, right and sinks must not be negative");
+  MF_REQUIRE(a.q && a.k && a.v, MF_ERR_BAD_ARG, "q, k and v must not be NULL");
+  MF_REQUIRE(a.D <= 128, MF_ERR_UNSUPPORTED, "head size %d > 128 is not supported", a.D);
+  MF_REQUIRE(a.Lq <= 1 << 29 && a.Lk <= 1 << 29, MF_ERR_UNSUPPORTED, "lengths above 2^29 are not supported");
+  MF_REQUIRE((int64_t)a.B * a.N <= 65535 && a.H <= 65535, MF_ERR_UNSUPPORTED, "B*N=%lld or H=%d exceeds 65535", (long long)a.B * a.N, a.H);
+  return MF_OK;
+}
+int check_workspace(const void* workspace, size_t given, size_t need) {
+  if (!need) return MF_OK;
+  MF_REQUIRE(workspace && given >= need, MF_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? given : (size_t)0);
+  MF_REQUIRE(((uintptr_t)workspace & 255) == 0, MF_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return MF_OK;
+}
+}  // namespace
+
+int mf_relpos_fwd(const mf_relpos_args* args, void* stream) {
+  Range nvtx_range("mf_relpos_fwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  int r = check_relpos(*args); if (r) return r;
+  MF_REQUIRE(args->weight && args->bias, MF_ERR_BAD_ARG, "weight and bias must not be NULL");
+  r = check_device(); if (r) return r;
+  return relpos_fwd(*args, static_cast<cudaStream_t>(stream));
+}
+
+size_t mf_relpos_bwd_workspace_bytes(const mf_relpos_args* args) { return args && check_relpos(*args) == MF_OK ? relpos_bwd_workspace(*args) : 0; }
+
+int mf_relpos_bwd(const mf_relpos_args* args, void* stream) {
+  Range nvtx_range("mf_relpos_bwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  int r = check_relpos(*args); if (r) return r;
+  MF_REQUIRE(args->d_bias && args->d_weight && float_dtype(args->dw_dtype), MF_ERR_BAD_ARG, "d_bias and d_weight must not be NULL, d_weight of a floating type");
+  r = check_device(); if (r) return r;
+  r = check_workspace(args->workspace, args->workspace_bytes, relpos_bwd_workspace(*args)); if (r) return r;
+  return relpos_bwd(*args, static_cast<cudaStream_t>(stream));
+}
+
+int mf_qk_rotary_fwd(const mf_qk_rotary_args* args, void* stream) {
+  Range nvtx_range("mf_qk_rotary_fwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  int r = check_qk_rotary(*args); if (r) return r;
+  MF_REQUIRE(args->q_out && args->k_out, MF_ERR_BAD_ARG, "q_out and k_out must not be NULL");
+  r = check_device(); if (r) return r;
+  return qk_rotary_fwd(*args, static_cast<cudaStream_t>(stream));
+}
+
+size_t mf_qk_rotary_bwd_workspace_bytes(const mf_qk_rotary_args* args) { return args && check_qk_rotary(*args) == MF_OK ? qk_rotary_bwd_workspace(*args) : 0; }
+
+int mf_qk_rotary_bwd(const mf_qk_rotary_args* args, void* stream) {
+  Range nvtx_range("mf_qk_rotary_bwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  int r = check_qk_rotary(*args); if (r) return r;
+  MF_REQUIRE(args->dq_out && args->dk_out && args->dq && args->dk, MF_ERR_BAD_ARG, "dq_out, dk_out, dq and dk must not be NULL");
+  MF_REQUIRE(!args->q_weight == !args->dq_weight && !args->k_weight == !args->dk_weight, MF_ERR_BAD_ARG, "the weights' gradients are given with the weights");
+  r = check_device(); if (r) return r;
+  r = check_workspace(args->workspace, args->workspace_bytes, qk_rotary_bwd_workspace(*args)); if (r) return r;
+  return qk_rotary_bwd(*args, static_cast<cudaStream_t>(stream));
+}
+
+size_t mf_window_fwd_workspace_bytes(const mf_window_args* args) { return 0; }
+
+int mf_window_fwd(const mf_window_args* args, void* stream) {
+  Range nvtx_range("mf_window_fwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  const mf_window_args& a = *args;
+  int r = check_window(a); if (r) return r;
+  MF_REQUIRE(a.o, MF_ERR_BAD_ARG, "o must not be NULL");
+  r = check_device(); if (r) return r;
+  r = window_fwd_simt(a, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
+}
+
+size_t mf_window_bwd_workspace_bytes(const mf_window_args* args) { return args && check_window(*args) == MF_OK ? window_bwd_simt_workspace(*args) : 0; }
+
+int mf_window_bwd(const mf_window_args* args, void* stream) {
+  Range nvtx_range("mf_window_bwd");
+  MF_REQUIRE(args, MF_ERR_BAD_ARG, "args is NULL");
+  const mf_window_args& a = *args;
+  int r = check_window(a); if (r) return r;
+  MF_REQUIRE(a.o && a.d_o && a.lse, MF_ERR_BAD_ARG, "o, d_o and lse must not be NULL");
+  MF_REQUIRE(a.dq && a.dk && a.dv, MF_ERR_BAD_ARG, "dq, dk and dv must not be NULL");
+  r = check_device(); if (r) return r;
+  r = check_workspace(a.workspace, a.workspace_bytes, mf_window_bwd_workspace_bytes(args)); if (r) return r;
+  r = window_bwd_simt(a, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
+}
+
 int mf_cast_batch(const mf_cast_item* items, int32_t n_items, void* stream) {
   Range nvtx_range("mf_cast_batch");
   MF_REQUIRE(items && n_items > 0 && n_items <= MF_CAST_MAX, MF_ERR_BAD_ARG, "between 1 and %d arrays are converted at once, got %d", MF_CAST_MAX, n_items);

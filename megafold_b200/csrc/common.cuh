@@ -192,6 +192,16 @@ int gate_bwd(const void* d, const void* o, const void* g, int64_t gs, void* d_o,
 int bias_layout(void* rows, void* planes, int L, int np, int H, bool swap, bool to_rows, int dtype, cudaStream_t st);
 int cast_batch(const mf_cast_item* items, int n_items, cudaStream_t st);
 
+int relpos_fwd(const mf_relpos_args& a, cudaStream_t st);
+size_t relpos_bwd_workspace(const mf_relpos_args& a);
+int relpos_bwd(const mf_relpos_args& a, cudaStream_t st);
+int qk_rotary_fwd(const mf_qk_rotary_args& a, cudaStream_t st);
+size_t qk_rotary_bwd_workspace(const mf_qk_rotary_args& a);
+int qk_rotary_bwd(const mf_qk_rotary_args& a, cudaStream_t st);
+int window_fwd_simt(const mf_window_args& a, cudaStream_t st);
+size_t window_bwd_simt_workspace(const mf_window_args& a);
+int window_bwd_simt(const mf_window_args& a, cudaStream_t st);
+
 int swiglu_fwd(const void* x, void* y, int64_t M, int inner, int dtype, cudaStream_t st);
 int swiglu_bwd(const void* x, const void* dy, void* dx, int64_t M, int inner, int dtype, cudaStream_t st);
 

@@ -1,0 +1,378 @@
+// RMS norm of every head of queries and keys and their rotation by position, in one pass, and its backward.
+//
+//   y = x * rstd * w,  rstd = (mean_d x^2 + eps)^-1/2;   out = the pairs of y's first R elements turned by pos * inv_freq, the rest of y
+//   g = d_out turned back;  dx = rstd * (w g - hat * mean_d(w g hat)),  hat = x * rstd;   dw = sum over tokens (and heads) of g * hat
+//
+// A head's row is a few threads, each with V pairs: two pieces of V elements that turn together (R / 2 apart, or adjacent where
+// pairs are interleaved), so that nothing but the sum of squares crosses threads.  Angles are formed and
+// reduced in 64 bits (a position of a million times a frequency in 32 bits is off by 0.06); a thread computes its V angles once for all heads of its token that it goes through.  Sums and norms are
+// fp32, the outputs are rounded once.  The weights' gradients are summed in a fixed order: a thread over its tokens, a block over its threads
+// in shared memory, a second kernel over the blocks.
+//
+// Bound: HBM; for single tokens latency.
+#include "common.cuh"
+
+namespace mf {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RotP {
+  int N, L, H, Hk, D, R;
+  int64_t tokens;                           // B * N * L
+  const void *q, *k; int64_t qs[5], ks[5];
+  const void *qw, *kw; int w_dtype; int64_t w_head;      // weights (NULL: ones); elements between heads, 0: shared
+  const float* inv_freq;
+  const void* pos; int64_t ps[3]; bool pos64;            // NULL: the index along L
+  float eps;
+  int heads_per;                            // heads that a thread goes through
+  int log_lpr;                              // threads of a row
+  void *q_out, *k_out;                      // contiguous
+  const void *dq_out, *dk_out; void *dq, *dk;
+  float* parts;                             // [gridDim.y][gridDim.x][2][D]
+};
+
+// Sine and cosine of pos * f, in half turns: the whole quarters are taken off in 64 bits, exactly but for the one rounding of the
+// product with 1 / pi, and what is left, at most a quarter, goes to CUDA's sincospif.
+__device__ __forceinline__ void turn_of(double pos, float f, float& s, float& c) {
+  const double t = pos * (double)f * 0.31830988618379067154, k = rint(2. * t);
+  float sr, cr;
+  sincospif((float)fma(k, -0.5, t), &sr, &cr);
+  const int quarter = (int)((long long)k & 3);
+  const float s1 = quarter & 1 ? cr : sr, c1 = quarter & 1 ? sr : cr;
+  s = quarter & 2 ? -s1 : s1;
+  c = quarter == 1 || quarter == 2 ? -c1 : c1;
+}
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
+
+// A thread's unit u of a row: V pairs, or, behind the rotated part, up to 2 V elements that are not turned.
+template <int V, bool IL>
+struct Unit {
+  int a, b;                 // first elements of the two pieces
+  bool turned, has_a, has_b;
+  __device__ __forceinline__ Unit(int u, int R, int D) {
+    const int nr = R / 2 / V;
+    turned = u < nr;
+    if (turned) { a = IL ? 2 * V * u : V * u; b = IL ? a + V : R / 2 + a; has_a = has_b = true; }
+    else { a = R + 2 * V * (u - nr); b = a + V; has_a = a < D; has_b = b < D; }
+  }
+};
+// x[0..V) and x[V..2V) hold the first and second elements of the V pairs (or the two pieces of an unturned unit)
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void load_unit(const T* row, int64_t sd, const Unit<V, IL>& u, float (&x)[2 * V]) {
+  Piece<T, V> p, q;
+  if constexpr (V == 1) {
+    p.v[0] = u.has_a ? row[u.a * sd] : from_f<T>(0.f);
+    q.v[0] = u.has_b ? row[u.b * sd] : from_f<T>(0.f);
+  } else {
+    if (u.has_a) p = *reinterpret_cast<const Piece<T, V>*>(row + u.a); else for (int e = 0; e < V; ++e) p.v[e] = from_f<T>(0.f);
+    if (u.has_b) q = *reinterpret_cast<const Piece<T, V>*>(row + u.b); else for (int e = 0; e < V; ++e) q.v[e] = from_f<T>(0.f);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (IL && V > 1) {
+      x[e] = to_f(2 * e < V ? p.v[2 * e] : q.v[2 * e - V]);
+      x[V + e] = to_f(2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]);
+    } else {
+      x[e] = to_f(p.v[e]); x[V + e] = to_f(q.v[e]);
+    }
+  }
+}
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void store_unit(T* row, const Unit<V, IL>& u, const float (&x)[2 * V]) {
+  Piece<T, V> p, q;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (IL && V > 1) {
+      (2 * e < V ? p.v[2 * e] : q.v[2 * e - V]) = from_f<T>(x[e]);
+      (2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]) = from_f<T>(x[V + e]);
+    } else {
+      p.v[e] = from_f<T>(x[e]); q.v[e] = from_f<T>(x[V + e]);
+    }
+  }
+  if (u.has_a) *reinterpret_cast<Piece<T, V>*>(row + u.a) = p;
+  if (u.has_b) *reinterpret_cast<Piece<T, V>*>(row + u.b) = q;
+}
+// index in a row of D elements of x[e] / of x[V + e]
+template <int V, bool IL>
+__device__ __forceinline__ int element(const Unit<V, IL>& u, int e) {
+  if constexpr (IL) { const int i = e < V ? 2 * e : 2 * (e - V) + 1; return u.a + i; }      // the pieces are adjacent
+  else return e < V ? u.a + e : u.b + e - V;
+}
+
+template <int V, bool IL>
+__device__ __forceinline__ void load_weight(const void* w, int64_t at, int dt, const Unit<V, IL>& u, int D, float (&out)[2 * V]) {
+#pragma unroll
+  for (int e = 0; e < 2 * V; ++e) {
+    const int i = element<V, IL>(u, e);
+    out[e] = i >= D ? 0.f : w ? load_rt(w, at + i, dt) : 1.f;
+  }
+}
+__device__ __forceinline__ float row_sum(float v, int lpr) {
+  for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// blockIdx.y = group of heads_per heads (of the H + Hk of queries and keys); threads of a block walk tokens.
+// UPL: units of a thread.  (Every thread of a warp takes part in each sum: rows that do not exist are zeros.)
+template <typename T, int V, int UPL, bool IL, bool BWD>
+__global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_constant__ RotP p) {
+  const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr, slots = kThreads >> p.log_lpr;
+  const int heads = p.H + p.Hk, g0 = blockIdx.y * p.heads_per, g1 = g0 + p.heads_per < heads ? g0 + p.heads_per : heads;
+  const float inv_d = 1.f / p.D;
+  float dwq[BWD ? UPL : 1][2 * V] = {}, dwk[BWD ? UPL : 1][2 * V] = {};
+  const int64_t stride = (int64_t)gridDim.x * slots, rounds = (p.tokens + stride - 1) / stride;
+  for (int64_t it = 0; it < rounds; ++it) {
+    const int64_t tok = it * stride + (int64_t)blockIdx.x * slots + slot;
+    const bool live = tok < p.tokens;
+    const int64_t bn = live ? tok / p.L : 0, l = live ? tok - bn * p.L : 0, b = bn / p.N, n = bn - b * p.N;
+    double pos = (double)l;
+    if (p.pos) {
+      const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
+      pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
+    }
+    float cs[UPL][V], sn[UPL][V];
+#pragma unroll
+    for (int k = 0; k < UPL; ++k) {
+      const int u = lane + k * lpr;
+      const bool turned = u < p.R / 2 / V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        cs[k][e] = 1.f; sn[k][e] = 0.f;
+        if (turned && live) turn_of(pos, p.inv_freq[u * V + e], sn[k][e], cs[k][e]);
+      }
+    }
+    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1] + l * p.qs[2];
+    const T* kk = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1] + l * p.ks[2];
+#pragma unroll 2
+    for (int g = g0; g < g1; ++g) {
+      const bool is_q = g < p.H;
+      const int h = is_q ? g : g - p.H;
+      const T* row = is_q ? q + h * p.qs[3] : kk + h * p.ks[3];
+      const int64_t sd = is_q ? p.qs[4] : p.ks[4], out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
+      const void* w = is_q ? p.qw : p.kw;
+      float x[UPL][2 * V], ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) {
+        Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+        u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+        load_unit<T, V, IL>(row, sd, u, x[k]);
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) ss = fmaf(x[k][e], x[k][e], ss);
+      }
+      float d[BWD ? UPL : 1][2 * V];
+      if constexpr (BWD) {
+        const T* dr = static_cast<const T*>(is_q ? p.dq_out : p.dk_out) + out_at;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+          load_unit<T, V, IL>(dr, 1, u, d[k]);
+        }
+      }
+      const float rstd = rsqrtf(fmaf(row_sum(ss, lpr), inv_d, p.eps));
+      if constexpr (!BWD) {
+        T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + out_at;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+          float wt[2 * V];
+          load_weight<V, IL>(w, h * p.w_head, p.w_dtype, u, p.D, wt);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float y1 = x[k][e] * rstd * wt[e], y2 = x[k][V + e] * rstd * wt[V + e];
+            x[k][e] = u.turned ? y1 * cs[k][e] - y2 * sn[k][e] : y1;
+            x[k][V + e] = u.turned ? y2 * cs[k][e] + y1 * sn[k][e] : y2;
+          }
+          store_unit<T, V, IL>(out, u, x[k]);
+        }
+      } else {
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+          float wt[2 * V];
+          load_weight<V, IL>(w, h * p.w_head, p.w_dtype, u, p.D, wt);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float d1 = d[k][e], d2 = d[k][V + e];
+            d[k][e] = u.turned ? d1 * cs[k][e] + d2 * sn[k][e] : d1;
+            d[k][V + e] = u.turned ? d2 * cs[k][e] - d1 * sn[k][e] : d2;
+          }
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) {
+            x[k][e] *= rstd;                                   // hat
+            const float t = d[k][e] * x[k][e];
+            if (is_q) dwq[k][e] += t; else dwk[k][e] += t;
+            d[k][e] *= wt[e];
+            dot = fmaf(d[k][e], x[k][e], dot);
+          }
+        }
+        dot = row_sum(dot, lpr) * inv_d;
+        T* out = static_cast<T*>(is_q ? p.dq : p.dk) + out_at;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) x[k][e] = rstd * fmaf(-x[k][e], dot, d[k][e]);
+          store_unit<T, V, IL>(out, u, x[k]);
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!p.parts) return;
+    extern __shared__ float sum[];                             // [slots][D]
+    float* out = p.parts + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) {
+        const Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) {
+          const int i = element<V, IL>(u, e);
+          if (i < p.D && (u.turned || i >= p.R)) sum[slot * p.D + i] = which ? dwk[k][e] : dwq[k][e];
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.D; i += kThreads) {
+        float s = 0.f;
+        for (int k = 0; k < slots; ++k) s += sum[k * p.D + i];
+        out[which * p.D + i] = s;
+      }
+    }
+  }
+}
+
+// Weight gradients: row x of [2][heads or 1][D] is the sum of its blocks' rows, a warp an element.
+__global__ void __launch_bounds__(kThreads) qk_rotary_join_kernel(const float* __restrict__ parts, int gx, int gy, int D, int H, int Hk, bool per_head, void* __restrict__ dqw,
+                                                                  void* __restrict__ dkw, int w_dtype) {
+  const int x = (blockIdx.x * kThreads + threadIdx.x) >> 5, l = threadIdx.x & 31;
+  const int q_rows = per_head ? H : 1, k_rows = per_head ? Hk : 1;
+  if (x >= (q_rows + k_rows) * D) return;
+  const int row = x / D, i = x - row * D;
+  const bool is_k = row >= q_rows;
+  const int y0 = per_head ? row : 0, y1 = per_head ? row + 1 : gy;        // per head: a group of blocks each, queries' heads first
+  double s = 0.;
+  for (int64_t k = (int64_t)y0 * gx + l; k < (int64_t)y1 * gx; k += 32) s += parts[(k * 2 + is_k) * D + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (l) return;
+  if (is_k) store_rt(dkw, (int64_t)(row - q_rows) * D + i, w_dtype, (float)s);
+  else store_rt(dqw, (int64_t)row * D + i, w_dtype, (float)s);
+}
+
+RotP rot_params(const mf_qk_rotary_args& a) {
+  RotP p{};
+  p.N = a.N; p.L = a.L; p.H = a.H; p.Hk = a.Hk; p.D = a.D; p.R = a.R; p.tokens = (int64_t)a.B * a.N * a.L;
+  p.q = a.q; p.k = a.k;
+  for (int i = 0; i < 5; ++i) { p.qs[i] = a.q_strides[i]; p.ks[i] = a.k_strides[i]; }
+  p.qw = a.q_weight; p.kw = a.k_weight; p.w_dtype = a.w_dtype; p.w_head = a.per_head ? a.D : 0;
+  p.inv_freq = a.inv_freq; p.pos = a.positions; p.pos64 = a.pos_bytes == 8;
+  for (int i = 0; i < 3; ++i) p.ps[i] = a.pos_strides[i];
+  p.eps = a.eps; p.q_out = a.q_out; p.k_out = a.k_out;
+  p.dq_out = a.dq_out; p.dk_out = a.dk_out; p.dq = a.dq; p.dk = a.dk;
+  return p;
+}
+
+// elements of a piece: the widest load that sizes, strides and addresses allow
+int piece(const mf_qk_rotary_args& a, bool bwd) {
+  const int es = (int)dtype_size(a.dtype);
+  for (int v = 16 / es; v > 1; v /= 2) {
+    bool ok = a.R / 2 % v == 0 && (a.D - a.R) % v == 0 && a.q_strides[4] == 1 && a.k_strides[4] == 1;
+    for (int i = 0; i < 4; ++i) ok = ok && a.q_strides[i] % v == 0 && a.k_strides[i] % v == 0;
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (bwd ? (uintptr_t)a.dq_out | (uintptr_t)a.dk_out | (uintptr_t)a.dq | (uintptr_t)a.dk
+                                                                : (uintptr_t)a.q_out | (uintptr_t)a.k_out);
+    if (ok && at % (v * es) == 0) return v;
+  }
+  return 1;
+}
+int units_per(int V) { return V >= 4 ? 1 : V == 2 ? 2 : 4; }
+
+struct Plan { int log_lpr, heads_per, gx, gy; };
+Plan plan(const mf_qk_rotary_args& a, int V, bool bwd) {
+  Plan c;
+  const int units = a.R / 2 / V + (a.D - a.R + 2 * V - 1) / (2 * V), lanes = (units + units_per(V) - 1) / units_per(V);
+  c.log_lpr = 0;
+  while ((1 << c.log_lpr) < lanes) ++c.log_lpr;
+  const int slots = kThreads >> c.log_lpr, heads = a.H + a.Hk;
+  const int64_t tokens = (int64_t)a.B * a.N * a.L, blocks = (tokens + slots - 1) / slots, want = 8 * (int64_t)tcx::sm_count();
+  // every head of a token in one thread, which computes the angles once; fewer where that leaves processors idle, and one where
+  // each head has a weight of its own whose gradient a block sums
+  c.heads_per = heads;
+  if (bwd && a.per_head && a.dq_weight) c.heads_per = 1;
+  while (c.heads_per > 1 && blocks * ((heads + c.heads_per - 1) / c.heads_per) < want) c.heads_per = (c.heads_per + 1) / 2;
+  c.gy = (heads + c.heads_per - 1) / c.heads_per;
+  int64_t gx = blocks;
+  if (bwd) { const int64_t most = (want + c.gy - 1) / c.gy; if (gx > most) gx = most; }
+  if (gx > 0x7fffffff) gx = 0x7fffffff;
+  c.gx = (int)gx;
+  return c;
+}
+
+template <typename T, int V, bool BWD>
+int run(const mf_qk_rotary_args& a, cudaStream_t st) {
+  constexpr int UPL = V >= 4 ? 1 : V == 2 ? 2 : 4;
+  RotP p = rot_params(a);
+  const Plan c = plan(a, V, BWD);
+  p.log_lpr = c.log_lpr; p.heads_per = c.heads_per;
+  size_t smem = 0;
+  if (BWD && a.dq_weight) {
+    p.parts = static_cast<float*>(a.workspace);
+    smem = sizeof(float) * (kThreads >> c.log_lpr) * a.D;
+  }
+  const auto go = [&](auto il) -> int {
+    constexpr auto kern = qk_rotary_kernel<T, V, UPL, decltype(il)::value, BWD>;
+    if (int e = opt_in_smem<kern>(smem)) return e;
+    kern<<<dim3(c.gx, c.gy), kThreads, smem, st>>>(p);
+    MF_LAUNCHED("qk_rotary_kernel");
+    return MF_OK;
+  };
+  if (int e = a.interleaved ? go(std::true_type{}) : go(std::false_type{})) return e;
+  if (BWD && a.dq_weight) {
+    const int rows = a.per_head ? a.H + a.Hk : 2;
+    qk_rotary_join_kernel<<<(rows * a.D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(p.parts, c.gx, c.gy, a.D, a.H, a.Hk, a.per_head != 0, a.dq_weight, a.dk_weight,
+                                                                                                a.w_dtype);
+    MF_LAUNCHED("qk_rotary_join_kernel");
+  }
+  return MF_OK;
+}
+template <typename T, bool BWD>
+int dispatch(const mf_qk_rotary_args& a, cudaStream_t st) {
+  switch (piece(a, BWD)) {
+    case 8: if constexpr (sizeof(T) == 2) return run<T, 8, BWD>(a, st);
+    case 4: return run<T, 4, BWD>(a, st);
+    case 2: return run<T, 2, BWD>(a, st);
+    default: return run<T, 1, BWD>(a, st);
+  }
+}
+}  // namespace
+
+int qk_rotary_fwd(const mf_qk_rotary_args& a, cudaStream_t st) {
+  int r = MF_OK;
+  MF_DISPATCH_FLOAT(a.dtype, T, r = (dispatch<T, false>(a, st)));
+  return r;
+}
+size_t qk_rotary_bwd_workspace(const mf_qk_rotary_args& a) {
+  if (!a.dq_weight) return 0;
+  size_t most = 0;
+  for (int v = 1; v <= 16 / (int)dtype_size(a.dtype); v *= 2) {       // whichever width the alignment allows
+    if (a.R / 2 % v || (a.D - a.R) % v) break;
+    const Plan c = plan(a, v, true);
+    const size_t n = sizeof(float) * 2 * a.D * (size_t)c.gx * c.gy;
+    if (n > most) most = n;
+  }
+  return most;
+}
+int qk_rotary_bwd(const mf_qk_rotary_args& a, cudaStream_t st) {
+  int r = MF_OK;
+  MF_DISPATCH_FLOAT(a.dtype, T, r = (dispatch<T, true>(a, st)));
+  return r;
+}
+
+}  // namespace mf

@@ -50,6 +50,16 @@ struct Api {
   MF_ENTRY(mf_transition_fwd);
   MF_ENTRY(mf_transition_bwd_workspace_bytes);
   MF_ENTRY(mf_transition_bwd);
+  MF_ENTRY(mf_relpos_fwd);
+  MF_ENTRY(mf_relpos_bwd_workspace_bytes);
+  MF_ENTRY(mf_relpos_bwd);
+  MF_ENTRY(mf_qk_rotary_fwd);
+  MF_ENTRY(mf_qk_rotary_bwd_workspace_bytes);
+  MF_ENTRY(mf_qk_rotary_bwd);
+  MF_ENTRY(mf_window_fwd_workspace_bytes);
+  MF_ENTRY(mf_window_fwd);
+  MF_ENTRY(mf_window_bwd_workspace_bytes);
+  MF_ENTRY(mf_window_bwd);
   MF_ENTRY(mf_cast_batch);
   MF_ENTRY(mf_last_error_string);
 } api;
@@ -70,6 +80,9 @@ void load(const std::string& path) {
   MF_LOAD(mf_swiglu_fwd); MF_LOAD(mf_swiglu_bwd);
   MF_LOAD(mf_transition_fwd_workspace_bytes); MF_LOAD(mf_transition_fwd);
   MF_LOAD(mf_transition_bwd_workspace_bytes); MF_LOAD(mf_transition_bwd);
+  MF_LOAD(mf_relpos_fwd); MF_LOAD(mf_relpos_bwd_workspace_bytes); MF_LOAD(mf_relpos_bwd);
+  MF_LOAD(mf_qk_rotary_fwd); MF_LOAD(mf_qk_rotary_bwd_workspace_bytes); MF_LOAD(mf_qk_rotary_bwd);
+  MF_LOAD(mf_window_fwd_workspace_bytes); MF_LOAD(mf_window_fwd); MF_LOAD(mf_window_bwd_workspace_bytes); MF_LOAD(mf_window_bwd);
   MF_LOAD(mf_cast_batch); MF_LOAD(mf_last_error_string);
 #undef MF_LOAD
 }
@@ -744,6 +757,323 @@ Tensor pair_bias(const Tensor& x, const Tensor& lw, const Tensor& lb, const Tens
   return PairBiasFn::apply(x, lw, lb, w, H);
 }
 
+// ---- relative position bias ---------------------------------------------------------------------------------------------
+// The pairs' buckets in whole numbers: see mf_relpos_args.  q_pos and k_pos undefined: the queries are the last of the keys.
+struct Relpos {
+  Tensor q_pos, k_pos, q_seg, k_seg;
+  std::vector<int32_t> edges;
+  int64_t base_pos, step_pos, base_neg, step_neg, B, Lq, Lk;
+};
+Tensor whole_numbers(const OptTensor& t, const char* what) {
+  if (!t || !t->defined()) return Tensor();
+  TORCH_CHECK_TYPE(t->scalar_type() == at::kInt || t->scalar_type() == at::kLong, what, " must be int32 or int64, got ", t->scalar_type());
+  TORCH_CHECK_VALUE(t->dim() == 1 || t->dim() == 2, what, " must be [L] or [B, L], got ", shape(*t));
+  const Tensor r = t->dim() == 1 ? t->unsqueeze(0) : *t;
+  return r.size(1) > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+Relpos relpos_plan(const Tensor& weight, const OptTensor& q_pos, const OptTensor& k_pos, int64_t Lq, int64_t Lk, const OptTensor& q_seg, const OptTensor& k_seg,
+                   const std::vector<int64_t>& edges, const std::array<int64_t, 4>& rows) {
+  Relpos r;
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.is_floating_point(), "weight must be a floating [rows, heads], got ", shape(weight));
+  r.q_pos = whole_numbers(q_pos, "q_positions"); r.k_pos = whole_numbers(k_pos, "k_positions");
+  r.q_seg = whole_numbers(q_seg, "q_segments"); r.k_seg = whole_numbers(k_seg, "k_segments");
+  TORCH_CHECK_VALUE(r.q_pos.defined() == r.k_pos.defined() && r.q_seg.defined() == r.k_seg.defined(), "positions and segments are given for queries and keys, or for neither");
+  r.Lq = r.q_pos.defined() ? r.q_pos.size(1) : Lq; r.Lk = r.k_pos.defined() ? r.k_pos.size(1) : Lk;
+  TORCH_CHECK_VALUE(r.Lq >= 0 && r.Lk >= 0 && r.Lq < (1 << 30) && r.Lk < (1 << 30), "bad lengths ", r.Lq, " and ", r.Lk);
+  r.B = 1;
+  bool empty = false;
+  for (const Tensor* t : {&r.q_pos, &r.k_pos, &r.q_seg, &r.k_seg})
+    if (t->defined()) { r.B = std::max(r.B, t->size(0)); empty = empty || t->size(0) == 0; }
+  if (empty) r.B = 0;
+  for (const Tensor* t : {&r.q_pos, &r.k_pos, &r.q_seg, &r.k_seg}) {
+    if (!t->defined()) continue;
+    const int64_t L = t == &r.q_pos || t == &r.q_seg ? r.Lq : r.Lk;
+    TORCH_CHECK_VALUE((t->size(0) == 1 || t->size(0) == r.B) && t->size(1) == L, "positions and segments do not fit together: ", shape(*t), " where [", r.B, ", ", L, "] is needed");
+    TORCH_CHECK_VALUE(t->device() == weight.device(), "positions, segments and weight must be on one device");
+  }
+  if (r.q_pos.defined()) TORCH_CHECK_TYPE(r.q_pos.scalar_type() == r.k_pos.scalar_type(), "q_positions and k_positions must share a type");
+  if (r.q_seg.defined()) TORCH_CHECK_TYPE(r.q_seg.scalar_type() == r.k_seg.scalar_type(), "q_segments and k_segments must share a type");
+  for (int64_t e : edges) r.edges.push_back((int32_t)e);
+  r.base_pos = rows[0]; r.step_pos = rows[1]; r.base_neg = rows[2]; r.step_neg = rows[3];
+  return r;
+}
+mf_relpos_args relpos_args(const Relpos& r, int64_t rows, int64_t H, at::ScalarType dtype) {
+  mf_relpos_args a{};
+  a.B = (int32_t)r.B; a.H = (int32_t)H; a.Lq = (int32_t)r.Lq; a.Lk = (int32_t)r.Lk; a.rows = (int32_t)rows;
+  a.dtype = dtype_code(dtype);
+  a.n_edges = (int32_t)r.edges.size(); a.edges = r.edges.data();
+  a.base_pos = (int32_t)r.base_pos; a.step_pos = (int32_t)r.step_pos; a.base_neg = (int32_t)r.base_neg; a.step_neg = (int32_t)r.step_neg;
+  auto step = [](const Tensor& t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : (int64_t)0; };
+  a.q_pos = ptr(r.q_pos); a.k_pos = ptr(r.k_pos); a.q_pos_stride = step(r.q_pos); a.k_pos_stride = step(r.k_pos);
+  a.q_seg = ptr(r.q_seg); a.k_seg = ptr(r.k_seg); a.q_seg_stride = step(r.q_seg); a.k_seg_stride = step(r.k_seg);
+  a.pos_bytes = r.q_pos.defined() ? (int32_t)r.q_pos.element_size() : 8; a.seg_bytes = r.q_seg.defined() ? (int32_t)r.q_seg.element_size() : 8;
+  return a;
+}
+Tensor relpos_fwd_raw(const Tensor& weight, const Relpos& r, at::ScalarType dtype) {
+  const int64_t rows = weight.size(0), H = weight.size(1);
+  Tensor bias = at::empty({r.B, 1, H, r.Lq, r.Lk}, weight.options().dtype(dtype));
+  if (bias.numel() == 0) return bias;
+  mf_relpos_args a = relpos_args(r, rows, H, dtype);
+  a.w_dtype = dtype_code(weight.scalar_type());
+  a.weight = weight.data_ptr(); a.bias = bias.data_ptr();
+  check(api.mf_relpos_fwd(&a, stream_of(weight)), "mf_relpos_fwd");
+  return bias;
+}
+struct RelposFn : torch::autograd::Function<RelposFn> {
+  static Variable forward(AutogradContext* ctx, const Tensor& weight_, const Relpos& r, at::ScalarType dtype) {
+    const c10::cuda::CUDAGuard guard(weight_.device());
+    const Tensor weight = plain(weight_).contiguous();
+    ctx->save_for_backward({r.q_pos, r.k_pos, r.q_seg, r.k_seg});
+    ctx->saved_data["edges"] = std::vector<int64_t>(r.edges.begin(), r.edges.end());
+    ctx->saved_data["sizes"] = std::vector<int64_t>{r.base_pos, r.step_pos, r.base_neg, r.step_neg, r.B, r.Lq, r.Lk, weight.size(0), weight.size(1),
+                                                    (int64_t)weight.scalar_type()};
+    return relpos_fwd_raw(weight, r, dtype);
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const auto z = ctx->saved_data["sizes"].toIntVector();
+    Relpos r{s[0], s[1], s[2], s[3], {}, z[0], z[1], z[2], z[3], z[4], z[5], z[6]};
+    for (int64_t e : ctx->saved_data["edges"].toIntVector()) r.edges.push_back((int32_t)e);
+    const c10::cuda::CUDAGuard guard(g[0].device());
+    const Tensor d_bias = plain(g[0]).contiguous();
+    Tensor dw = at::empty({z[7], z[8]}, d_bias.options().dtype((at::ScalarType)z[9]));
+    if (d_bias.numel() == 0) return {dw.zero_(), Tensor(), Tensor()};
+    mf_relpos_args a = relpos_args(r, z[7], z[8], d_bias.scalar_type());
+    a.w_dtype = a.dw_dtype = dtype_code(dw.scalar_type());
+    a.d_bias = d_bias.data_ptr(); a.d_weight = dw.data_ptr();
+    Tensor ws = workspace(api.mf_relpos_bwd_workspace_bytes(&a), d_bias);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    check(api.mf_relpos_bwd(&a, stream_of(d_bias)), "mf_relpos_bwd");
+    return {dw, Tensor(), Tensor()};
+  }
+};
+Tensor relative_position_bias(const Tensor& weight, const OptTensor& q_pos, const OptTensor& k_pos, int64_t Lq, int64_t Lk, const OptTensor& q_seg,
+                              const OptTensor& k_seg, const std::vector<int64_t>& edges, const std::array<int64_t, 4>& rows, std::optional<at::ScalarType> dtype) {
+  const Tensor qp = or_none(q_pos), kp = or_none(k_pos), qs = or_none(q_seg), ks = or_none(k_seg);
+  require_cuda({&weight, &qp, &kp, &qs, &ks});
+  const c10::cuda::CUDAGuard guard(weight.device());
+  const Relpos r = relpos_plan(weight, q_pos, k_pos, Lq, Lk, q_seg, k_seg, edges, rows);
+  const auto out = dtype.value_or(weight.scalar_type());
+  TORCH_CHECK_TYPE(out == at::kFloat || out == at::kBFloat16 || out == at::kHalf, "megafold_b200: unsupported dtype ", out);
+  if (!at::GradMode::is_enabled()) {
+    refuse_transforms({&weight});
+    return relpos_fwd_raw(plain(weight).contiguous(), r, out);
+  }
+  return RelposFn::apply(weight, r, out);
+}
+
+// ---- norm and rotation of queries and keys ------------------------------------------------------------------------------
+struct Rotary { Tensor q, k, qw, kw, freq, pos; double eps; bool interleaved; };
+void check_rotary(const Rotary& t) {
+  TORCH_CHECK_VALUE(t.q.dim() == 5 && t.k.dim() == 5, "q and k must be [B, N_seq, N_res, Head, Dim], got ", shape(t.q), " and ", shape(t.k));
+  const auto &q = t.q.sizes(), &k = t.k.sizes();
+  TORCH_CHECK_VALUE(q[0] == k[0] && q[1] == k[1] && q[2] == k[2] && q[4] == k[4], "q and k differ in more than their heads: ", shape(t.q), " ", shape(t.k));
+  TORCH_CHECK_TYPE(t.q.scalar_type() == t.k.scalar_type(), "q and k must share a dtype");
+  TORCH_CHECK_VALUE(t.qw.defined() == t.kw.defined(), "queries and keys both have a weight, or neither has");
+  if (t.qw.defined()) {
+    const bool shared = t.qw.dim() == 1 && t.kw.dim() == 1 && t.qw.size(0) == q[4] && t.kw.size(0) == q[4];
+    const bool each = t.qw.dim() == 2 && t.kw.dim() == 2 && t.qw.size(0) == q[3] && t.kw.size(0) == k[3] && t.qw.size(1) == q[4] && t.kw.size(1) == q[4];
+    TORCH_CHECK_VALUE(shared || each, "the weights must be [Dim], or [Head, Dim], for queries and keys alike, got ", shape(t.qw), " and ", shape(t.kw));
+    TORCH_CHECK_TYPE(t.qw.scalar_type() == t.kw.scalar_type(), "the weights must share a dtype");
+  }
+  TORCH_CHECK_VALUE(t.freq.dim() == 1 && 2 * t.freq.size(0) <= q[4], "inv_freq must hold a frequency for each pair of at most Dim elements, got ", shape(t.freq));
+  TORCH_CHECK_TYPE(t.freq.scalar_type() == at::kFloat, "inv_freq must be float32");
+  TORCH_CHECK_VALUE(!t.freq.requires_grad(), "inv_freq has no gradient");
+  if (t.pos.defined()) {
+    TORCH_CHECK_TYPE(t.pos.scalar_type() == at::kInt || t.pos.scalar_type() == at::kLong, "positions must be int32 or int64, got ", t.pos.scalar_type());
+    TORCH_CHECK_VALUE(t.pos.dim() >= 1 && t.pos.dim() <= 3 && t.pos.size(-1) == q[2] && (t.pos.dim() < 2 || t.pos.size(-2) == 1 || t.pos.size(-2) == q[1]) &&
+                          (t.pos.dim() < 3 || t.pos.size(0) == 1 || t.pos.size(0) == q[0]),
+                      "positions must be [N_res], [N_seq, N_res] or [B, N_seq, N_res], got ", shape(t.pos));
+  }
+  for (const Tensor* x : {&t.k, &t.qw, &t.kw, &t.freq, &t.pos})
+    TORCH_CHECK_VALUE(!x->defined() || x->device() == t.q.device(), "all tensors must be on one device");
+}
+mf_qk_rotary_args rotary_args(const Rotary& t) {
+  mf_qk_rotary_args a{};
+  a.B = (int32_t)t.q.size(0); a.N = (int32_t)t.q.size(1); a.L = (int32_t)t.q.size(2); a.H = (int32_t)t.q.size(3); a.Hk = (int32_t)t.k.size(3);
+  a.D = (int32_t)t.q.size(4); a.R = (int32_t)(2 * t.freq.size(0));
+  a.dtype = dtype_code(t.q.scalar_type()); a.w_dtype = t.qw.defined() ? dtype_code(t.qw.scalar_type()) : MF_F32;
+  a.per_head = t.qw.defined() && t.qw.dim() == 2; a.interleaved = t.interleaved; a.eps = (float)t.eps;
+  a.q = t.q.data_ptr(); a.k = t.k.data_ptr();
+  for (int i = 0; i < 5; ++i) { a.q_strides[i] = t.q.stride(i); a.k_strides[i] = t.k.stride(i); }
+  a.q_weight = ptr(t.qw); a.k_weight = ptr(t.kw); a.inv_freq = static_cast<const float*>(ptr(t.freq));
+  a.pos_bytes = 8;
+  if (t.pos.defined()) {
+    a.positions = t.pos.data_ptr(); a.pos_bytes = (int32_t)t.pos.element_size();
+    for (int i = 0; i < 3; ++i) {
+      const int64_t d = t.pos.dim() - 3 + i;
+      a.pos_strides[i] = d >= 0 && t.pos.size(d) > 1 ? t.pos.stride(d) : 0;
+    }
+  }
+  return a;
+}
+std::tuple<Tensor, Tensor> rotary_fwd_raw(const Rotary& t) {
+  Tensor qo = at::empty(t.q.sizes(), t.q.options()), ko = at::empty(t.k.sizes(), t.k.options());
+  if (qo.numel() == 0 || ko.numel() == 0) {
+    TORCH_CHECK_VALUE(qo.numel() == 0 && ko.numel() == 0, "q and k must both have heads");
+    return {qo, ko};
+  }
+  mf_qk_rotary_args a = rotary_args(t);
+  a.q_out = qo.data_ptr(); a.k_out = ko.data_ptr();
+  check(api.mf_qk_rotary_fwd(&a, stream_of(t.q)), "mf_qk_rotary_fwd");
+  return {qo, ko};
+}
+Rotary rotary_operands(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& freq, const Tensor& pos, double eps, bool interleaved) {
+  Rotary t{plain(q), plain(k), plain(qw), plain(kw), freq, pos, eps, interleaved};
+  if (t.qw.defined()) { t.qw = t.qw.contiguous(); t.kw = t.kw.contiguous(); }
+  t.freq = plain(freq).contiguous();
+  return t;
+}
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static tensor_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& freq, const OptTensor& pos,
+                             double eps, bool interleaved) {
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Rotary t = rotary_operands(q, k, or_none(qw), or_none(kw), freq, or_none(pos), eps, interleaved);
+    auto [qo, ko] = rotary_fwd_raw(t);
+    ctx->save_for_backward({t.q, t.k, t.qw, t.kw, t.freq, t.pos});
+    ctx->saved_data["eps"] = eps; ctx->saved_data["interleaved"] = interleaved;
+    return {qo, ko};
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    const Rotary t{s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+    const Tensor dqo = plain(g[0]).contiguous(), dko = plain(g[1]).contiguous();
+    Tensor dq = at::empty(t.q.sizes(), t.q.options()), dk = at::empty(t.k.sizes(), t.k.options()), dqw, dkw;
+    if (t.qw.defined()) { dqw = at::empty(t.qw.sizes(), t.qw.options()); dkw = at::empty(t.kw.sizes(), t.kw.options()); }
+    if (dq.numel() == 0) {
+      if (dqw.defined()) { dqw.zero_(); dkw.zero_(); }
+      return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+    mf_qk_rotary_args a = rotary_args(t);
+    a.dq_out = dqo.data_ptr(); a.dk_out = dko.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dq_weight = ptr(dqw); a.dk_weight = ptr(dkw);
+    Tensor ws = workspace(api.mf_qk_rotary_bwd_workspace_bytes(&a), t.q);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    check(api.mf_qk_rotary_bwd(&a, stream_of(t.q)), "mf_qk_rotary_bwd");
+    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& freq, const OptTensor& pos, double eps,
+                                          bool interleaved) {
+  const Tensor w1 = or_none(qw), w2 = or_none(kw), ps = or_none(pos);
+  require_cuda({&q, &k, &w1, &w2, &freq, &ps});
+  check_rotary(Rotary{q, k, w1, w2, freq, ps, eps, interleaved});
+  if (!at::GradMode::is_enabled()) {
+    refuse_transforms({&q, &k, &w1, &w2});
+    const c10::cuda::CUDAGuard guard(q.device());
+    return rotary_fwd_raw(rotary_operands(q, k, w1, w2, freq, ps, eps, interleaved));
+  }
+  auto r = RotaryFn::apply(q, k, qw, kw, freq, pos, eps, interleaved);
+  return {r[0], r[1]};
+}
+
+// ---- sliding-window attention ---------------------------------------------------------------------------------------------
+struct Span { int64_t left, right, sinks; };
+void check_window(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, const Span& s) {
+  TORCH_CHECK_VALUE(q.dim() == 5 && k.dim() == 5, "Q and K must be [B, N_seq, N_res, Head, Dim], got ", shape(q), " and ", shape(k));
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "K and V shapes differ: ", shape(k), " ", shape(v));
+  TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(4) == k.size(4), "Q and K do not fit together: ", shape(q), " ", shape(k));
+  TORCH_CHECK_VALUE(k.size(3) > 0 && q.size(3) % k.size(3) == 0, "the heads of Q must be a multiple of those of K, got ", q.size(3), " and ", k.size(3));
+  TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "Q, K, V must share a dtype");
+  TORCH_CHECK_VALUE(s.left >= 0 && s.right >= 0 && s.sinks >= 0, "left, right and sinks must not be negative, got ", s.left, ", ", s.right, " and ", s.sinks);
+  if (mask.defined()) {
+    TORCH_CHECK_TYPE(mask.scalar_type() == at::kBool || mask.scalar_type() == at::kByte, "mask must be a bool or uint8 keep-mask, got ", mask.scalar_type());
+    TORCH_CHECK_VALUE(mask.dim() == 5 && mask.size(2) == 1 && mask.size(3) == 1 && mask.size(4) == k.size(2) && (mask.size(0) == 1 || mask.size(0) == k.size(0)) &&
+                          (mask.size(1) == 1 || mask.size(1) == k.size(1)), "mask must be [B, N_seq, 1, 1, N_keys], got ", shape(mask));
+  }
+  for (const Tensor* t : {&k, &v, &mask}) TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), "all tensors must be on one device");
+}
+mf_window_args window_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, const Span& s, int64_t flags) {
+  mf_window_args a{};
+  auto i32 = [](int64_t x) { return (int32_t)std::min<int64_t>(x, INT32_MAX); };
+  a.B = i32(q.size(0)); a.N = i32(q.size(1)); a.Lq = i32(q.size(2)); a.Lk = i32(k.size(2)); a.H = i32(q.size(3)); a.Hk = i32(k.size(3)); a.D = i32(q.size(4));
+  a.left = i32(s.left); a.right = i32(s.right); a.sinks = i32(s.sinks);
+  a.dtype = dtype_code(q.scalar_type()); a.flags = (uint32_t)flags;
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+  for (int i = 0; i < 5; ++i) { a.q_strides[i] = q.stride(i); a.k_strides[i] = k.stride(i); a.v_strides[i] = v.stride(i); }
+  if (mask.defined()) {
+    a.mask = mask.data_ptr();
+    a.mask_strides[0] = mask.size(0) == 1 ? 0 : mask.stride(0); a.mask_strides[1] = mask.size(1) == 1 ? 0 : mask.stride(1); a.mask_strides[2] = mask.stride(4);
+  }
+  return a;
+}
+std::tuple<Tensor, Tensor> window_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& mask_, int64_t left, int64_t right, int64_t sinks,
+                                          int64_t flags, bool want_lse) {
+  const Tensor mask = or_none(mask_);
+  Tensor hold[3];
+  const Tensor &q = plain(q_, hold[0]), &k = plain(k_, hold[1]), &v = plain(v_, hold[2]);
+  require_cuda({&q, &k, &v, &mask});
+  const Span s{left, right, sinks};
+  check_window(q, k, v, mask, s);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor o = at::empty(q.sizes(), q.options()), lse;
+  if (want_lse) lse = empty_f32({q.size(0), q.size(1), q.size(3), q.size(2)}, q);
+  if (q.numel() == 0 || k.numel() == 0) {
+    if (lse.defined()) lse.fill_(-INFINITY);
+    return {o.zero_(), lse};
+  }
+  mf_window_args a = window_args(q, k, v, mask, s, flags);
+  a.o = o.data_ptr(); a.lse = static_cast<float*>(ptr(lse));
+  Tensor ws;
+  if (const size_t need = api.mf_window_fwd_workspace_bytes(&a)) {
+    ws = workspace(need, q);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+  }
+  check(api.mf_window_fwd(&a, stream_of(q)), "mf_window_fwd");
+  return {o, lse};
+}
+std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& mask_, int64_t left,
+                                                   int64_t right, int64_t sinks, const Tensor& o_, const Tensor& lse, int64_t flags) {
+  const Tensor mask = or_none(mask_);
+  Tensor hold[3];
+  const Tensor &q = plain(q_, hold[0]), &k = plain(k_, hold[1]), &v = plain(v_, hold[2]);
+  require_cuda({&d_o_, &q, &k, &v, &mask, &o_, &lse});
+  const Span s{left, right, sinks};
+  check_window(q, k, v, mask, s);
+  TORCH_CHECK_VALUE(d_o_.sizes() == q.sizes() && o_.sizes() == q.sizes(), "d_o and o must have the shape of Q, ", shape(q), ", got ", shape(d_o_), " and ", shape(o_));
+  TORCH_CHECK_TYPE(d_o_.scalar_type() == q.scalar_type() && o_.scalar_type() == q.scalar_type() && lse.scalar_type() == at::kFloat, "d_o and o must have the dtype of Q, lse float32");
+  TORCH_CHECK_VALUE(lse.is_contiguous() && lse.numel() == q.size(0) * q.size(1) * q.size(2) * q.size(3), "lse must hold a value for each query row, got ", shape(lse));
+  for (const Tensor* t : {&d_o_, &o_, &lse}) TORCH_CHECK_VALUE(t->device() == q.device(), "all tensors must be on one device");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor d_o = plain(d_o_).contiguous(), o = plain(o_).contiguous();
+  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dv = at::empty(k.sizes(), q.options());
+  if (q.numel() == 0 || k.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_()};
+  mf_window_args a = window_args(q, k, v, mask, s, flags);
+  a.o = o.data_ptr(); a.d_o = d_o.data_ptr(); a.lse = const_cast<float*>(lse.data_ptr<float>());
+  a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
+  Tensor ws = workspace(api.mf_window_bwd_workspace_bytes(&a), q);
+  a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+  check(api.mf_window_bwd(&a, stream_of(q)), "mf_window_bwd");
+  return {dq, dk, dv};
+}
+struct WindowFn : torch::autograd::Function<WindowFn> {
+  static Variable forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t left, int64_t right, int64_t sinks) {
+    auto [o, lse] = window_forward(q, k, v, mask, left, right, sinks, 0, true);
+    ctx->save_for_backward({q, k, v, or_none(mask), o, lse});
+    ctx->saved_data["span"] = std::vector<int64_t>{left, right, sinks};
+    return o;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const auto w = ctx->saved_data["span"].toIntVector();
+    auto [dq, dk, dv] = window_backward(g[0], s[0], s[1], s[2], s[3].defined() ? OptTensor(s[3]) : OptTensor(), w[0], w[1], w[2], s[4], s[5], 0);
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t left, int64_t right, int64_t sinks) {
+  const Tensor m = or_none(mask);
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    refuse_transforms({&q, &k, &v, &m});
+    return std::get<0>(window_forward(q, k, v, mask, left, right, sinks, 0, false));
+  }
+  require_cuda({&q, &k, &v, &m});
+  check_window(q, k, v, m, Span{left, right, sinks});
+  return WindowFn::apply(q, k, v, mask, left, right, sinks);
+}
+
 // std::array of tensors, undefined ones as None
 template <size_t N>
 std::array<OptTensor, N> optional(std::array<Tensor, N> r) {
@@ -780,4 +1110,21 @@ PYBIND11_MODULE(_native, m) {
   m.def("triangle", &triangle, release());
   m.def("gated_attention", &gated_attention, release());
   m.def("pair_bias", &pair_bias, release());
+  m.def("relative_position_bias", [](const Tensor& weight, const OptTensor& q_pos, const OptTensor& k_pos, int64_t Lq, int64_t Lk, const OptTensor& q_seg,
+                                     const OptTensor& k_seg, const std::vector<int64_t>& edges, const std::array<int64_t, 4>& rows,
+                                     const std::optional<pybind11::object>& dtype) {
+    std::optional<at::ScalarType> dt;
+    if (dtype) {
+      TORCH_CHECK_TYPE(THPDtype_Check(dtype->ptr()), "dtype must be a torch.dtype");
+      dt = reinterpret_cast<THPDtype*>(dtype->ptr())->scalar_type;
+    }
+    pybind11::gil_scoped_release no_gil;
+    return relative_position_bias(weight, q_pos, k_pos, Lq, Lk, q_seg, k_seg, edges, rows, dt);
+  });
+  m.def("qk_norm_rotary", &qk_norm_rotary, release());
+  m.def("window_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t left, int64_t right, int64_t sinks, int64_t flags) {
+    return window_forward(q, k, v, mask, left, right, sinks, flags, true);
+  }, release());
+  m.def("window_backward", &window_backward, release());
+  m.def("window_attention", &window_attention, release());
 }

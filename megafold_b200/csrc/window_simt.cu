@@ -1,0 +1,370 @@
+// Sliding-window attention with sinks on CUDA cores, fp32 arithmetic throughout: fp32 tensors, and what the tensor-core kernels do
+// not take (head sizes that are no multiple of 8, unaligned or non-adjacent elements).
+//
+// Tiles and products are those of the dense attention's CUDA-core kernels.  Forward: a block per (b, n, h, 64 queries) walks the
+// key tiles that its rows see, with the running maximum and sum of the softmax.  Backward, two kinds of blocks in one launch:
+// dQ per 64 queries, and dK / dV per 64 keys and chunk of their list of query blocks.  Nothing is added atomically: every
+// result is a sum in a fixed order.  Bound: FP32 issue (66 % of it goes to the multiply-adds).
+//
+// Masked keys are read as zeros: whatever their rows hold (NaN, too) reaches nothing.  A row that sees no key gives 0, and a
+// log-sum-exp of -inf, and passes no gradient.
+#include "simt_tiles.cuh"
+#include "window_common.cuh"
+
+namespace mf {
+namespace win {
+
+namespace {
+using namespace simt;
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_tile(void* out, int heads, int64_t bn, int h, int L, int D, int row0, int ty, int tx, const float (&acc)[4][DP / 16],
+                                           const float (&f)[4]) {
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int l = row0 + ty + 16 * a;
+    if (l >= L) continue;
+    T* row = static_cast<T*>(out) + ((bn * L + l) * heads + h) * D;
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) {
+      const int d = tx * (DP / 16) + e;
+      if (d < D) row[d] = from_f<T>(acc[a][e] * f[a]);
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_constant__ WinP p) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int kOp = kTile * (DP + 4);
+  float *Qs = smem, *Ks = Qs + kOp, *Vs = Ks + kOp, *Ps = Vs + kOp;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int h = blockIdx.y, hk = h / p.G, bn = blockIdx.z, b = bn / p.N, n = bn - b * p.N, i0 = blockIdx.x * kTile;
+  const int i1 = i0 + kTile < p.Lq ? i0 + kTile : p.Lq;
+  load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+  const auto keep = [&](int j) { return kept(p, b, n, j); };
+  float acc[4][DP / 16], m[4], l[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    m[a] = -INFINITY; l[a] = 0.f;
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) acc[a][e] = 0.f;
+  }
+  const KeyTiles tiles = key_tiles<kTile>(p, i0, i1);
+  for (int t = 0; t < tiles.count(); ++t) {
+    const int j0 = tiles.at(t) * kTile;
+    __syncthreads();
+    load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    bool see[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) see[c] = j0 + tx + 16 * c < p.Lk && keep(j0 + tx + 16 * c);
+    __syncthreads();
+    float s[4][4] = {};
+    dot_tile<DP>(Qs, Ks, ty, tx, s);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int i = i0 + ty + 16 * a;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[a][c] = see[c] && in_window(p, i, j0 + tx + 16 * c) ? s[a][c] * p.scale : -INFINITY;
+      const float m_new = fmaxf(m[a], row_max(fmaxf(fmaxf(s[a][0], s[a][1]), fmaxf(s[a][2], s[a][3]))));
+      const float m_ref = m_new == -INFINITY ? 0.f : m_new;         // nothing seen so far
+      const float corr = expf(m[a] - m_ref);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float pr = expf(s[a][c] - m_ref);
+        sum += pr;
+        Ps[(ty + 16 * a) * kPPitch + tx + 16 * c] = pr;
+      }
+      l[a] = l[a] * corr + row_sum(sum);
+      m[a] = m_new;
+#pragma unroll
+      for (int e = 0; e < DP / 16; ++e) acc[a][e] *= corr;
+    }
+    __syncwarp();                // a row's probabilities are written and read by the same half warp
+    sum_tile<DP>(Ps, Vs, ty, tx, acc);
+  }
+  float inv[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) inv[a] = l[a] > 0.f ? 1.f / l[a] : l[a] == 0.f ? 0.f : l[a];      // NaN stays
+  store_tile<T, DP>(p.o, p.H, bn, h, p.Lq, p.D, i0, ty, tx, acc, inv);
+  if (tx == 0 && p.lse)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int i = i0 + ty + 16 * a;
+      if (i < p.Lq) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = m[a] + logf(l[a]);
+    }
+}
+
+// P and dS of one logit from its product sums
+__device__ __forceinline__ void p_ds(const WinP& p, bool see, float s, float dp, float lse, float dl, float& pr, float& ds) {
+  pr = see ? expf(fmaf(s, p.scale, -lse)) : 0.f;
+  ds = see ? pr * (dp - dl) : 0.f;
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* parts, float* smem, int bn, int hk, int x) {
+  constexpr int kOp = kTile * (DP + 4);
+  float *Ks = smem, *Vs = Ks + kOp, *Qs = Vs + kOp, *Gs = Qs + kOp, *Ps = Gs + kOp, *Ds = Ps + kTile * kPPitch;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, b = bn / p.N, n = bn - b * p.N;
+  int tile, part;
+  plan_item(c, x, tile, part);
+  const int j0 = tile * kTile, len = list_length<kTile, kTile>(p, tile), e0 = part * c.chunk;
+  if (part > 0 && e0 >= len) return;
+  const auto keep = [&](int j) { return kept(p, b, n, j); };
+  load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
+  load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+  int lo, hi;
+  query_range(p, j0, j0 + kTile < p.Lk ? j0 + kTile : p.Lk, lo, hi);
+  const int first = lo / kTile, per_head = hi > lo ? (hi + kTile - 1) / kTile - first : 1;
+  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+  bool see[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) see[a] = j0 + ty + 16 * a < p.Lk && keep(j0 + ty + 16 * a);
+  for (int e = e0; e < len && e < e0 + c.chunk; ++e) {
+    const int h = hk * p.G + e / per_head, i0 = (first + e % per_head) * kTile;
+    __syncthreads();
+    load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+    const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
+    load_tile<T, DP>(Gs, p.d_o, gs, p.g_vec, b, n, h, i0, p.Lq, p.D);
+    float lse[4], dl[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + tx + 16 * k;
+      const int64_t row = ((int64_t)bn * p.H + h) * p.Lq + i;
+      lse[k] = i < p.Lq ? p.lse[row] : 0.f; dl[k] = i < p.Lq ? p.delta[row] : 0.f;
+    }
+    __syncthreads();
+    float s[4][4] = {}, dp[4][4] = {};
+    dot_tile<DP>(Ks, Qs, ty, tx, s);
+    dot_tile<DP>(Vs, Gs, ty, tx, dp);
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + tx + 16 * k, j = j0 + ty + 16 * a;
+        float pr, ds;
+        p_ds(p, see[a] && i < p.Lq && in_window(p, i, j), s[a][k], dp[a][k], lse[k], dl[k], pr, ds);
+        Ps[(ty + 16 * a) * kPPitch + tx + 16 * k] = pr;
+        Ds[(ty + 16 * a) * kPPitch + tx + 16 * k] = ds;
+      }
+    __syncwarp();
+    sum_tile<DP>(Ps, Gs, ty, tx, dv);
+    sum_tile<DP>(Ds, Qs, ty, tx, dk);
+  }
+  if (x < c.split_x) {
+    float* out = part_of<kTile>(parts, c, p, (int64_t)bn * p.Hk + hk, x);
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int e = 0; e < DP / 16; ++e) {
+        const int d = tx * (DP / 16) + e, row = ty + 16 * a;
+        if (d < p.D) { out[row * p.D + d] = dk[a][e]; out[(kTile + row) * p.D + d] = dv[a][e]; }
+      }
+    return;
+  }
+  const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {p.scale, p.scale, p.scale, p.scale};
+  store_tile<T, DP>(p.dk, p.Hk, bn, hk, p.Lk, p.D, j0, ty, tx, dk, sc);
+  store_tile<T, DP>(p.dv, p.Hk, bn, hk, p.Lk, p.D, j0, ty, tx, dv, one);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h, int i0) {
+  constexpr int kOp = kTile * (DP + 4);
+  float *Ks = smem, *Vs = Ks + kOp, *Qs = Vs + kOp, *Gs = Qs + kOp, *Ds = Gs + kOp;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, b = bn / p.N, n = bn - b * p.N, hk = h / p.G;
+  const int i1 = i0 + kTile < p.Lq ? i0 + kTile : p.Lq;
+  load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+  const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
+  load_tile<T, DP>(Gs, p.d_o, gs, p.g_vec, b, n, h, i0, p.Lq, p.D);
+  const auto keep = [&](int j) { return kept(p, b, n, j); };
+  float dq[4][DP / 16] = {}, lse[4], dl[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int i = i0 + ty + 16 * a;
+    const int64_t row = ((int64_t)bn * p.H + h) * p.Lq + i;
+    lse[a] = i < p.Lq ? p.lse[row] : 0.f; dl[a] = i < p.Lq ? p.delta[row] : 0.f;
+  }
+  const KeyTiles tiles = key_tiles<kTile>(p, i0, i1);
+  for (int t = 0; t < tiles.count(); ++t) {
+    const int j0 = tiles.at(t) * kTile;
+    __syncthreads();
+    load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    bool see[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) see[c] = j0 + tx + 16 * c < p.Lk && keep(j0 + tx + 16 * c);
+    __syncthreads();
+    float s[4][4] = {}, dp[4][4] = {};
+    dot_tile<DP>(Qs, Ks, ty, tx, s);
+    dot_tile<DP>(Gs, Vs, ty, tx, dp);
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = i0 + ty + 16 * a;
+        float pr, ds;
+        p_ds(p, see[c] && i < p.Lq && in_window(p, i, j0 + tx + 16 * c), s[a][c], dp[a][c], lse[a], dl[a], pr, ds);
+        Ds[(ty + 16 * a) * kPPitch + tx + 16 * c] = ds;
+      }
+    __syncwarp();
+    sum_tile<DP>(Ds, Ks, ty, tx, dq);
+  }
+  const float sc[4] = {p.scale, p.scale, p.scale, p.scale};
+  store_tile<T, DP>(p.dq, p.H, bn, h, p.Lq, p.D, i0, ty, tx, dq, sc);
+}
+
+// blocks [0, n_dkv) work on dK and dV (the longest first: tiles with sinks lead), the others on dQ
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) window_bwd_simt_kernel(const __grid_constant__ WinP p, const KeyPlan c, float* parts, int64_t n_dkv) {
+  extern __shared__ __align__(16) float smem[];
+  const int64_t u = blockIdx.x;
+  const int64_t heads = (int64_t)p.B * p.N * p.Hk;
+  if (u < n_dkv) {
+    const int x = (int)(u / heads);
+    const int64_t head = u - (int64_t)x * heads;
+    bwd_dkv<T, DP>(p, c, parts, smem, (int)(head / p.Hk), (int)(head % p.Hk), x);
+  } else {
+    const int64_t w = u - n_dkv, all = (int64_t)p.B * p.N * p.H;
+    const int t = (int)(w / all);
+    const int64_t head = w - t * all;
+    bwd_dq<T, DP>(p, smem, (int)(head / p.H), (int)(head % p.H), t * kTile);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) window_delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, float* __restrict__ delta, int64_t rows, int Lq, int H,
+                                                           int D, bool vec) {
+  // four threads per (b, n, i, h)
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 2;
+  const int q = threadIdx.x & 3;
+  float s = 0.f;
+  if (row < rows) {
+    const T *po = o + row * D, *pg = d_o + row * D;
+    constexpr int V = 16 / sizeof(T);
+    if (vec) {
+      for (int d = q * V; d < D; d += 4 * V) {
+        __align__(16) T a[V];
+        __align__(16) T g[V];
+        *reinterpret_cast<uint4*>(a) = __ldg(reinterpret_cast<const uint4*>(po + d));
+        *reinterpret_cast<uint4*>(g) = __ldg(reinterpret_cast<const uint4*>(pg + d));
+#pragma unroll
+        for (int e = 0; e < V; ++e) s = fmaf(to_f(a[e]), to_f(g[e]), s);
+      }
+    } else {
+      for (int d = q; d < D; d += 4) s = fmaf(to_f(po[d]), to_f(pg[d]), s);
+    }
+  }
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  if (row < rows && q == 0) {
+    const int h = (int)(row % H);
+    const int64_t t = row / H, bn = t / Lq;
+    delta[(bn * H + h) * Lq + (t - bn * Lq)] = s;
+  }
+}
+
+template <typename T>
+int run_fwd(const WinP& p, cudaStream_t st) {
+  const auto go = [&](auto dp) -> int {
+    constexpr int DP = decltype(dp)::value;
+    constexpr size_t smem = sizeof(float) * (3 * kTile * (DP + 4) + kTile * kPPitch);
+    constexpr auto kern = window_fwd_simt_kernel<T, DP>;
+    if (int e = opt_in_smem<kern>(smem)) return e;
+    kern<<<dim3((p.Lq + kTile - 1) / kTile, p.H, p.B * p.N), kThreads, smem, st>>>(p);
+    MF_LAUNCHED("window_fwd_simt_kernel");
+    return MF_OK;
+  };
+  return p.D <= 32 ? go(std::integral_constant<int, 32>{}) : p.D <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+}
+
+template <typename T>
+int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
+  const auto go = [&](auto dp) -> int {
+    constexpr int DP = decltype(dp)::value;
+    constexpr size_t smem = sizeof(float) * (4 * kTile * (DP + 4) + 2 * kTile * kPPitch);
+    constexpr auto kern = window_bwd_simt_kernel<T, DP>;
+    if (int e = opt_in_smem<kern>(smem)) return e;
+    const int64_t n_dkv = (int64_t)c.x_total * p.B * p.N * p.Hk, blocks = n_dkv + (int64_t)((p.Lq + kTile - 1) / kTile) * p.B * p.N * p.H;
+    MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%lld blocks of 64 rows are more than one launch takes", (long long)blocks);
+    kern<<<(unsigned)blocks, kThreads, smem, st>>>(p, c, parts, n_dkv);
+    MF_LAUNCHED("window_bwd_simt_kernel");
+    return MF_OK;
+  };
+  int r = p.D <= 32 ? go(std::integral_constant<int, 32>{}) : p.D <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+  if (r || !c.split_x) return r;
+  const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink;
+  window_join_kernel<T, kTile, kTile><<<dim3(tiles, p.Hk, p.B * p.N), 256, 0, st>>>(p, c, parts);
+  MF_LAUNCHED("window_join_kernel");
+  return MF_OK;
+}
+
+bool rows_vec(const void* ptr, const int64_t* s, int D, size_t es) {
+  const int64_t q = 4;
+  return s[4] == 1 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) % (4 * es)) == 0 && s[0] % q == 0 && s[1] % q == 0 && s[2] % q == 0 && s[3] % q == 0;
+}
+
+KeyPlan simt_plan(const WinP& p) { return key_plan<kTile, kTile>(p, 2 * tcx::sm_count()); }
+}  // namespace
+
+WinP window_params(const mf_window_args& a) {
+  WinP p{};
+  p.B = a.B; p.N = a.N; p.Lq = a.Lq; p.Lk = a.Lk; p.H = a.H; p.Hk = a.Hk; p.D = a.D; p.G = a.H / a.Hk;
+  const int reach = a.Lq + a.Lk;                       // wider than that sees no more
+  p.left = a.left < reach ? a.left : reach; p.right = a.right < reach ? a.right : reach;
+  p.sinks = a.sinks < a.Lk ? a.sinks : a.Lk;
+  p.off = a.Lk - a.Lq;
+  p.scale = 1.f / sqrtf((float)a.D);
+  p.q = a.q; p.k = a.k; p.v = a.v;
+  for (int i = 0; i < 5; ++i) { p.qs[i] = a.q_strides[i]; p.ks[i] = a.k_strides[i]; p.vs[i] = a.v_strides[i]; }
+  p.mask = static_cast<const uint8_t*>(a.mask);
+  for (int i = 0; i < 3; ++i) p.ms[i] = a.mask_strides[i];
+  p.o = a.o; p.lse = a.lse; p.d_o = a.d_o; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv;
+  const size_t es = dtype_size(a.dtype);
+  const int64_t gs[5] = {0, 0, 0, a.D, 1};
+  p.q_vec = rows_vec(a.q, p.qs, a.D, es); p.k_vec = rows_vec(a.k, p.ks, a.D, es); p.v_vec = rows_vec(a.v, p.vs, a.D, es);
+  p.g_vec = rows_vec(a.d_o, gs, a.D, es);
+  return p;
+}
+
+int window_delta(const WinP& p, int dtype, float* delta, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.N * p.Lq * p.H, blocks = (rows + 63) / 64;
+  MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "too many query rows");
+  const size_t es = dtype_size(dtype);
+  const bool vec = (p.D * es) % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.d_o)) & 15) == 0;
+  MF_DISPATCH_FLOAT(dtype, T, {
+    window_delta_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(p.o), static_cast<const T*>(p.d_o), delta, rows, p.Lq, p.H, p.D, vec);
+    MF_LAUNCHED("window_delta_kernel");
+  });
+  return MF_OK;
+}
+
+}  // namespace win
+
+using namespace win;
+
+int window_fwd_simt(const mf_window_args& a, cudaStream_t st) {
+  const WinP p = window_params(a);
+  int r = MF_OK;
+  MF_DISPATCH_FLOAT(a.dtype, T, r = run_fwd<T>(p, st));
+  return r;
+}
+
+size_t window_bwd_simt_workspace(const mf_window_args& a) {
+  const WinP p = window_params(a);
+  return align_up(sizeof(float) * (size_t)p.B * p.N * p.H * p.Lq, 256) + sizeof(float) * part_floats<kTile>(simt_plan(p), p);
+}
+
+int window_bwd_simt(const mf_window_args& a, cudaStream_t st) {
+  WinP p = window_params(a);
+  float* delta = static_cast<float*>(a.workspace);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + align_up(sizeof(float) * (size_t)p.B * p.N * p.H * p.Lq, 256));
+  if (int r = window_delta(p, a.dtype, delta, st)) return r;
+  p.delta = delta;
+  int r = MF_OK;
+  MF_DISPATCH_FLOAT(a.dtype, T, r = run_bwd<T>(p, simt_plan(p), parts, st));
+  return r;
+}
+
+}  // namespace mf
