@@ -437,8 +437,9 @@ int mf_window_fwd(const mf_window_args* args, void* stream) {
   int r = check_window(a); if (r) return r;
   MF_REQUIRE(a.o, MF_ERR_BAD_ARG, "o must not be NULL");
   r = check_device(); if (r) return r;
-  r = window_fwd_simt(a, static_cast<cudaStream_t>(stream));
-  if (r == MF_OK) set_last_path("simt");
+  const bool tc = window_fwd_tc_supported(a);
+  r = tc ? window_fwd_tc(a, static_cast<cudaStream_t>(stream)) : window_fwd_simt(a, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path(tc ? "tcgen05" : "simt");
   return r;
 }
 

@@ -1,0 +1,307 @@
+// Sliding-window attention with sinks, forward, on the tensor cores (tcgen05 + TMEM + TMA): 16-bit tensors, head sizes that are
+// multiples of 8 up to 128.
+//
+// A CTA takes 128 queries of one head and walks the blocks of 64 keys that they see.  Warps 0-3: a thread owns a query row
+// (a TMEM lane): running maximum and sum, P over the scores in TMEM.  Warp 4 fetches Q, K and V by TMA, warp 5 issues the products
+//
+//   S(t) = Q K(t)^T  -> one of NB buffers of 64 columns        O += P(t) V(t)   (P as TMEM A operand, V MN-major)
+//
+// in the order S(0) [S(1)] PV(0) S(NB) PV(1) ..., so that a score buffer's P has been read when the next scores go into it.  O stays in
+// TMEM and is brought to a new maximum only when that grew by more than 2^8 in the exponent.  A window makes short walks
+// (5 blocks at 64 + 64 keys), so nothing is pipelined across items: several CTAs share an SM instead (3 up to DP = 64, with
+// one score buffer each, 2 at DP = 128 with two) and fill each other's waits.
+//
+// Blocks that a row does not see whole go through a 64-bit mask a row (window, sinks, end of the keys, key mask); rows of V whose
+// key is masked are overwritten with zeros in shared memory, since 0 * NaN would reach the sum.  P is rounded to the
+// operands' type (the matrix instruction's), its sum is of the unrounded fp32 values.
+//
+// All waits are bounded; on expiry the CTA leaves without touching its outputs and the host sees mf_async_status() != 0.
+#include "window_tc_common.cuh"
+
+namespace mf {
+namespace win {
+namespace {
+
+constexpr int kQ = 128, kK = 64, kThreads = 192;
+
+template <int DP> struct Cfg {
+  static constexpr int NB = DP == 128 ? 2 : 1;                  // score buffers
+  static constexpr int NS = DP == 128 ? 2 : 3;                  // K and V stages
+  static constexpr int CTAS = DP == 128 ? 2 : 3;                // on an SM
+  static constexpr uint32_t COLS = DP == 128 ? 256 : 128;       // TMEM
+  static constexpr int QB = Geo<DP>::TILE(kQ), KB = Geo<DP>::TILE(kK);
+  static constexpr size_t SMEM = 1024 + QB + 2 * NS * KB;
+};
+
+struct FwdP {
+  WinP w;
+  Coords cq, ck, cv;
+  int n_qt, heads;          // heads = B * N * H
+  float c1;                 // D^-1/2 * log2(e)
+  uint32_t fmt;
+  int* status;
+};
+
+template <int NS, int NB> struct Bars {
+  uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_ready[NB], p_ready[NB], pv_done;
+};
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads, Cfg<DP>::CTAS)
+window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                     const __grid_constant__ FwdP f) {
+  using C = Cfg<DP>;
+  using G = Geo<DP>;
+  constexpr int NS = C::NS, NB = C::NB;
+  const WinP& p = f.w;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *sQ = smem, *sK = sQ + C::QB, *sV = sK + NS * C::KB;
+  __shared__ Bars<NS, NB> bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+  if (tid == 0) {
+    abort_s = 0;
+    mbar_init(&bar.q_full, 1);
+    for (int i = 0; i < NS; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
+    for (int i = 0; i < NB; ++i) { mbar_init(&bar.s_ready[i], 1); mbar_init(&bar.p_ready[i], 128); }
+    mbar_init(&bar.pv_done, 1);
+    mbar_fence_init();
+    prefetch_tmap(&mq); prefetch_tmap(&mk); prefetch_tmap(&mv);
+  }
+  if (warp == 0) { tmem_alloc(&tmem_base_s, C::COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  volatile int* abort_flag = &abort_s;
+  const uint32_t t0 = uniform(tmem_base_s);
+  const uint32_t tO = t0 + NB * 64;
+
+  // the last queries first: where windows are cut off at the start of the keys those have the most to do
+  const int qt = f.n_qt - 1 - (int)(blockIdx.x / f.heads), head = blockIdx.x % f.heads;
+  const int h = head % p.H, bn = head / p.H, n = bn % p.N, b = bn / p.N, hk = h / p.G;
+  const int i0 = qt * kQ, i1 = i0 + kQ < p.Lq ? i0 + kQ : p.Lq;
+  const KeyTiles tiles = key_tiles<kK>(p, i0, i1);
+  const int T_ = tiles.count();
+
+  if (warp == 4) {
+    // ------------------------------------------------------------------------------------------------ copies
+    if (elect_one() && T_ > 0) {
+      mbar_expect_tx(&bar.q_full, C::QB);
+      load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h, i0, n * f.cq.n_mul, b * f.cq.b_mul);
+      int t = 0;
+      for (; t < T_; ++t) {
+        const int s = t % NS, j0 = tiles.at(t) * kK;
+        if (t >= NS) { wait_or_flag(&bar.k_empty[s], (t / NS - 1) & 1, abort_flag); wait_or_flag(&bar.v_empty[s], (t / NS - 1) & 1, abort_flag); }
+        if (*abort_flag) break;
+        mbar_expect_tx(&bar.k_full[s], C::KB);
+        load_tile_tma<DP>(sK + s * C::KB, &mk, &bar.k_full[s], kK, hk, j0, n * f.ck.n_mul, b * f.ck.b_mul);
+        mbar_expect_tx(&bar.v_full[s], C::KB);
+        load_tile_tma<DP>(sV + s * C::KB, &mv, &bar.v_full[s], kK, hk, j0, n * f.cv.n_mul, b * f.cv.b_mul);
+      }
+      // none may land after this CTA has left
+      drain_ring(&bar.q_full, 1, 1); drain_ring(bar.k_full, t, NS); drain_ring(bar.v_full, t, NS);
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------------------------------------ products
+    const uint32_t id_s = idesc_f16(128, kK, f.fmt, 0, 0), id_o = idesc_f16(128, DP, f.fmt, 0, 1);
+    const uint32_t q_lo = desc_lo(smem_u32(sQ), 16);
+    auto scores = [&](int t) {                    // false: given up
+      const int s = t % NS;
+      wait_or_flag(&bar.k_full[s], (t / NS) & 1, abort_flag);
+      if (__any_sync(0xffffffffu, *abort_flag)) return false;
+      tc_fence_after();
+      const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16), d = t0 + (t % NB) * 64;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) mma_ss_el(d, q_lo + k_step<DP>(ks, kQ), G::HI, k_lo + k_step<DP>(ks, kK), G::HI, id_s, ks > 0);
+      tc_commit_el(&bar.k_empty[s]);
+      tc_commit_el(&bar.s_ready[t % NB]);
+      return true;
+    };
+    if (T_ > 0) {
+      wait_or_flag(&bar.q_full, 0, abort_flag);
+      bool ok = true;
+      for (int t = 0; ok && t < NB && t < T_; ++t) ok = scores(t);
+      for (int t = 0; ok && t < T_; ++t) {
+        const int s = t % NS;
+        wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);
+        wait_or_flag(&bar.p_ready[t % NB], (t / NB) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        tc_fence_after();
+        const uint32_t v_lo = desc_lo(smem_u32(sV + s * C::KB), kK * G::ROWB), a = t0 + (t % NB) * 64;
+#pragma unroll
+        for (int ks = 0; ks < kK / 16; ++ks) mma_ts_el(tO, a + ks * 8, v_lo + ks * (16 * G::ROWB / 16), G::HI, id_o, t > 0 || ks > 0);
+        tc_commit_el(&bar.v_empty[s]);
+        tc_commit_el(&bar.pv_done);
+        if (t + NB < T_) ok = scores(t + NB);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------------ softmax
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int r = warp * 32 + lane, i = i0 + r, at = i + p.off;
+    const uint8_t* mask = p.mask ? p.mask + b * p.ms[0] + n * p.ms[1] : nullptr;
+    auto mask_bytes = [&](int t, uint32_t (&mb)[2]) {
+      const int j = tiles.at(t) * kK + lane;
+      mb[0] = j < p.Lk && mask[(int64_t)j * p.ms[2]]; mb[1] = j + 32 < p.Lk && mask[(int64_t)(j + 32) * p.ms[2]];
+    };
+    uint32_t mb[2] = {1, 1};
+    if (mask && T_ > 0) mask_bytes(0, mb);
+    float m = -INFINITY, l = 0.f;                 // m: the maximum that the sums refer to
+    for (int t = 0; t < T_; ++t) {
+      const int j0 = tiles.at(t) * kK;
+      uint32_t keep[2] = {~0u, ~0u};
+      if (mask) {
+        keep[0] = __ballot_sync(0xffffffffu, mb[0]); keep[1] = __ballot_sync(0xffffffffu, mb[1]);
+        if (t + 1 < T_) mask_bytes(t + 1, mb);
+      }
+      wait_or_flag(&bar.s_ready[t % NB], (t / NB) & 1, abort_flag);
+      if (__any_sync(0xffffffffu, *abort_flag)) break;
+      tc_fence_after();
+      const uint32_t tS = t0 + lanes + (t % NB) * 64;
+      uint32_t s0[32], s1[32];
+      tmem_ld32(tS, s0);
+      tmem_ld32(tS + 32, s1);
+      tmem_ld_wait(s0, s1);
+      if (!(all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + kK) && (keep[0] & keep[1]) == ~0u)) {
+        const uint32_t b0 = seen32(p, at, j0) & keep[0], b1 = seen32(p, at, j0 + 32) & keep[1];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          if (!(b0 >> e & 1)) s0[e] = 0xff800000u;
+          if (!(b1 >> e & 1)) s1[e] = 0xff800000u;
+        }
+      }
+      float mx = m;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) mx = max3f(max3f(mx, __uint_as_float(s0[e]), __uint_as_float(s0[e + 1])), __uint_as_float(s1[e]), __uint_as_float(s1[e + 1]));
+      float corr = 1.f;
+      if ((mx - m) * f.c1 > 8.f) {                // also from -inf
+        corr = ex2f((m - mx) * f.c1);
+        m = mx;
+        l *= corr;
+      }
+      const float off = m == -INFINITY ? 0.f : -m * f.c1;       // nothing seen so far: every logit is -inf
+      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const float2 x = fma2(make_float2(__uint_as_float(s0[e]), __uint_as_float(s0[e + 1])), c2, o2);
+        const float2 y = fma2(make_float2(__uint_as_float(s1[e]), __uint_as_float(s1[e + 1])), c2, o2);
+        const float2 px = make_float2(ex2f(x.x), ex2f(x.y)), py = make_float2(ex2f(y.x), ex2f(y.y));
+        sum[0] = add2(sum[0], px); sum[1] = add2(sum[1], py);
+        s0[e / 2] = Pack2<T>::pack(px.x, px.y);
+        s1[e / 2] = Pack2<T>::pack(py.x, py.y);
+      }
+      {
+        uint32_t (&w0)[16] = *reinterpret_cast<uint32_t (*)[16]>(s0);
+        uint32_t (&w1)[16] = *reinterpret_cast<uint32_t (*)[16]>(s1);
+        tmem_st16(tS, w0);
+        tmem_st16(tS + 16, w1);
+      }
+      const float2 s2 = add2(sum[0], sum[1]);
+      l += s2.x + s2.y;
+      // P V of the block before: O may be changed, and has to be complete to be
+      if (t > 0) {
+        wait_or_flag(&bar.pv_done, (t - 1) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o32[32];
+            tmem_ld32(tO + lanes + c * 32, o32);
+            tmem_ld_wait();
+            pin32(o32);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o32[e] = __float_as_uint(__uint_as_float(o32[e]) * corr);
+            tmem_st32(tO + lanes + c * 32, o32);
+          }
+        }
+      }
+      if (mask) {
+        // masked keys' rows of V (the keys beyond Lk are zeros already)
+        const int left = p.Lk - j0;
+        const uint32_t z0 = ~keep[0] & ones32(left), z1 = ~keep[1] & ones32(left - 32);
+        if (z0 | z1) {
+          const int s = t % NS;
+          wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);
+          const int row = r >> 1;                 // two threads a row
+          if ((row < 32 ? z0 >> row : z1 >> (row - 32)) & 1) {
+            uint8_t* at_row = sV + s * C::KB + row * G::ROWB + (r & 1) * (G::ROWB / 2);
+#pragma unroll
+            for (int pn = 0; pn < G::PANELS; ++pn)
+#pragma unroll
+              for (int x = 0; x < G::ROWB / 32; ++x) *reinterpret_cast<uint4*>(at_row + pn * kK * G::ROWB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bar.p_ready[t % NB]);
+    }
+    if (T_ > 0) wait_or_flag(&bar.pv_done, (T_ - 1) & 1, abort_flag);
+    tc_fence_after();
+    if (!__any_sync(0xffffffffu, *abort_flag)) {
+      T* out = static_cast<T*>(p.o) + (((int64_t)bn * p.Lq + i) * p.H + h) * p.D;
+      const int64_t step = (int64_t)p.H * p.D;
+      if (T_ > 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+          if (c * 32 < p.D) store_rows<T>(tO + lanes + c * 32, inv, out + c * 32, step, i, p.Lq, p.D - c * 32);
+      } else if (i < p.Lq) {
+        for (int d = 0; d < p.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (p.lse && i < p.Lq) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = l == 0.f ? -INFINITY : (m * f.c1 + lg2f(l)) * kLn2;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && abort_s) *reinterpret_cast<volatile int*>(f.status) = 1;
+  if (warp == 0) tmem_dealloc(t0, C::COLS);
+}
+
+template <int DP, typename T>
+int launch(const mf_window_args& a, cudaStream_t st) {
+  using C = Cfg<DP>;
+  using G = Geo<DP>;
+  FwdP f{};
+  f.w = window_params(a);
+  CUtensorMap mq, mk, mv;
+  if (int r = operand_map(&mq, &f.cq, a.q, a.dtype, a.B, a.N, a.Lq, a.H, a.D, a.q_strides, G::COLS, kQ)) return r;
+  if (int r = operand_map(&mk, &f.ck, a.k, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.k_strides, G::COLS, kK)) return r;
+  if (int r = operand_map(&mv, &f.cv, a.v, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.v_strides, G::COLS, kK)) return r;
+  f.n_qt = (a.Lq + kQ - 1) / kQ; f.heads = a.B * a.N * a.H;
+  f.c1 = kLog2e / sqrtf((float)a.D);
+  f.fmt = a.dtype == MF_BF16 ? 1u : 0u;
+  f.status = status_word();
+  MF_REQUIRE(f.status, MF_ERR_CUDA, "could not allocate the device status word");
+  MF_REQUIRE(tc_async_status() == 0, MF_ERR_CUDA, "an earlier tensor-core kernel gave up on a bounded wait; results are invalid");
+  const int64_t grid = (int64_t)f.n_qt * f.heads;
+  MF_REQUIRE((int64_t)a.B * a.N * a.H <= 0x7fffffff && grid <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%lld tiles of 128 queries are more than one launch takes", (long long)grid);
+  constexpr auto kern = window_fwd_tc_kernel<DP, T>;
+  if (int e = opt_in_smem<kern>(C::SMEM)) return e;
+  kern<<<(unsigned)grid, kThreads, C::SMEM, st>>>(mq, mk, mv, f);
+  MF_LAUNCHED("window_fwd_tc_kernel");
+  return MF_OK;
+}
+template <typename T>
+int by_size(const mf_window_args& a, cudaStream_t st) {
+  return a.D <= 32 ? launch<32, T>(a, st) : a.D <= 64 ? launch<64, T>(a, st) : launch<128, T>(a, st);
+}
+}  // namespace
+
+bool window_tc_supported(const mf_window_args& a) {
+  return !(a.flags & MF_FLAG_FORCE_SIMT) && (a.dtype == MF_BF16 || a.dtype == MF_F16) && a.D % 8 == 0 && operand_ok(a.q, a.q_strides, a.B, a.N, a.Lq, a.H) &&
+         operand_ok(a.k, a.k_strides, a.B, a.N, a.Lk, a.Hk) && operand_ok(a.v, a.v_strides, a.B, a.N, a.Lk, a.Hk);
+}
+}  // namespace win
+
+bool window_fwd_tc_supported(const mf_window_args& a) { return win::window_tc_supported(a) && ((uintptr_t)a.o & 15) == 0; }
+int window_fwd_tc(const mf_window_args& a, cudaStream_t st) {
+  return a.dtype == MF_BF16 ? win::by_size<__nv_bfloat16>(a, st) : win::by_size<__half>(a, st);
+}
+
+}  // namespace mf
