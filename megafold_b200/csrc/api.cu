@@ -428,7 +428,10 @@ int mf_qk_rotary_bwd(const mf_qk_rotary_args* args, void* stream) {
   return qk_rotary_bwd(*args, static_cast<cudaStream_t>(stream));
 }
 
-size_t mf_window_fwd_workspace_bytes(const mf_window_args* args) { return 0; }
+size_t mf_window_fwd_workspace_bytes(const mf_window_args* args) {
+  if (!args || check_window(*args) != MF_OK) return 0;
+  return window_fwd_tc_supported(*args) ? window_fwd_tc_workspace(*args) : window_fwd_simt_workspace(*args);
+}
 
 int mf_window_fwd(const mf_window_args* args, void* stream) {
   Range nvtx_range("mf_window_fwd");
@@ -437,6 +440,7 @@ int mf_window_fwd(const mf_window_args* args, void* stream) {
   int r = check_window(a); if (r) return r;
   MF_REQUIRE(a.o, MF_ERR_BAD_ARG, "o must not be NULL");
   r = check_device(); if (r) return r;
+  r = check_workspace(a.workspace, a.workspace_bytes, mf_window_fwd_workspace_bytes(args)); if (r) return r;
   const bool tc = window_fwd_tc_supported(a);
   r = tc ? window_fwd_tc(a, static_cast<cudaStream_t>(stream)) : window_fwd_simt(a, static_cast<cudaStream_t>(stream));
   if (r == MF_OK) set_last_path(tc ? "tcgen05" : "simt");

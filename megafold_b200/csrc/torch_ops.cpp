@@ -1016,7 +1016,7 @@ std::tuple<Tensor, Tensor> window_forward(const Tensor& q_, const Tensor& k_, co
   }
   mf_window_args a = window_args(q, k, v, mask, s, flags);
   a.o = o.data_ptr(); a.lse = static_cast<float*>(ptr(lse));
-  Tensor ws;
+  Tensor ws;                        // a few queries: parts of rows
   if (const size_t need = api.mf_window_fwd_workspace_bytes(&a)) {
     ws = workspace(need, q);
     a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();

@@ -4,6 +4,10 @@
 //
 // So the keys of a tile of queries are a run of tiles around it and a run of tiles at the front, and the queries of a tile of
 // keys are one run: around it, or from it to the end where the tile holds a sink.
+//
+// A tile of queries holds the rows of all heads that share a key head: row r is query r / pack, head r % pack of the group (pack = G, or
+// 1 where more heads share a key head than a tile has rows).  Keys are then read once for the group, the tile's window
+// is only as wide as its few queries need, and a single token fills G rows instead of one.
 #pragma once
 
 #include "common.cuh"
@@ -13,6 +17,7 @@ namespace win {
 
 struct WinP {
   int B, N, Lq, Lk, H, Hk, D, G;         // G = H / Hk query heads share a key head
+  int pack;                              // heads in a tile of queries
   int left, right, sinks, off;           // off = Lk - Lq: position of query 0
   float scale;                           // D^-1/2
   const void *q, *k, *v;
@@ -59,10 +64,14 @@ __host__ __device__ __forceinline__ void query_range(const WinP& p, int j0, int 
 }
 
 // ---- the work on dK and dV ------------------------------------------------------------------------------------------
-// A tile of KT keys sums over a list of (head of the group, block of QB queries).  The list of a tile with sinks runs to the last
+// A tile of KT keys sums over a list of (pack of heads, block of QB rows).  The list of a tile with sinks runs to the last
 // query, however narrow the window, and a short sequence has few tiles: lists are cut into chunks of `chunk` entries, a block
 // of threads each, whose fp32 sums are added in a fixed order by a second kernel.  x enumerates (tile, chunk), tiles with
 // sinks first; the first split_x of them are parts.
+// queries of a tile of ROWS rows; groups of `pack` heads; lists of a key head
+template <int ROWS> __host__ __device__ __forceinline__ int queries_of(const WinP& p) { return ROWS / p.pack; }
+__host__ __device__ __forceinline__ int head_groups(const WinP& p) { return p.H / p.pack; }
+
 struct KeyPlan {
   int n_tiles, n_sink, chunk, nc_sink, nc_rest, x_total, split_x;
 };
@@ -70,7 +79,8 @@ template <int KT, int QB>
 __host__ __device__ __forceinline__ int list_length(const WinP& p, int tile) {
   int lo, hi;
   query_range(p, tile * KT, tile * KT + KT < p.Lk ? tile * KT + KT : p.Lk, lo, hi);
-  return hi > lo ? p.G * ((hi + QB - 1) / QB - lo / QB) : 0;
+  const int q = queries_of<QB>(p);
+  return hi > lo ? p.G / p.pack * ((hi + q - 1) / q - lo / q) : 0;
 }
 template <int KT, int QB>
 KeyPlan key_plan(const WinP& p, int blocks_wanted) {
@@ -133,6 +143,35 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
     static_cast<T*>(which ? p.dv : p.dk)[((bn * p.Lk + j) * p.Hk + blockIdx.y) * p.D + d] = from_f<T>(s);
   }
 }
+
+// ---- few queries ------------------------------------------------------------------------------------------------------
+// Where the tiles of queries do not occupy the processors, the key tiles of each are split over `splits` blocks.  Each leaves its
+// normalised fp32 row and the row's log-sum-exp in `parts` ([splits][B, N, Lq, H][D], then [splits][B, N, Lq, H]), and a second kernel
+// weighs them.
+struct Split {
+  int splits;
+  float* parts;
+  int64_t rows;             // B * N * Lq * H
+  __device__ __forceinline__ float* row(int s, int64_t r, int D) const { return parts + ((int64_t)s * rows + r) * D; }
+  __device__ __forceinline__ float& lse(int s, int64_t r, int D) const { return parts[(int64_t)splits * rows * D + (int64_t)s * rows + r]; }
+};
+template <int ROWS, int KT>
+int split_count(const WinP& p, int blocks_wanted) {
+  const int q = queries_of<ROWS>(p);
+  const int64_t tiles = (p.Lq + q - 1) / q, blocks = tiles * p.B * p.N * head_groups(p);
+  if (2 * blocks > blocks_wanted) return 1;
+  int most = 0;                                            // key tiles of a tile of queries; few of them, or blocks would be many
+  for (int64_t t = 0; t < tiles; ++t) {
+    const int i0 = (int)t * q, n = key_tiles<KT>(p, i0, i0 + q < p.Lq ? i0 + q : p.Lq).count();
+    if (n > most) most = n;
+  }
+  int64_t s = blocks_wanted / blocks;
+  if (s > most / 2) s = most / 2;                          // two tiles at least, or the joining costs more than it saves
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+inline size_t split_bytes(const WinP& p, int splits) { return splits == 1 ? 0 : sizeof(float) * (size_t)splits * p.B * p.N * p.Lq * p.H * (p.D + 1); }
+int window_split_join(const WinP& p, int dtype, const Split& s, cudaStream_t st);
 
 WinP window_params(const mf_window_args& a);
 int window_delta(const WinP& p, int dtype, float* delta, cudaStream_t st);       // delta [B, N, H, Lq] = sum over d of d_o * o

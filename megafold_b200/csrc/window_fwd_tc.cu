@@ -1,7 +1,7 @@
 // Sliding-window attention with sinks, forward, on the tensor cores (tcgen05 + TMEM + TMA): 16-bit tensors, head sizes that are
 // multiples of 8 up to 128.
 //
-// A CTA takes 128 queries of one head and walks the blocks of 64 keys that they see.  Warps 0-3: a thread owns a query row
+// A CTA takes 128 rows of queries (of the heads that share a key head) and walks the blocks of 64 keys that they see.  Warps 0-3: a thread owns a query row
 // (a TMEM lane): running maximum and sum, P over the scores in TMEM.  Warp 4 fetches Q, K and V by TMA, warp 5 issues the products
 //
 //   S(t) = Q K(t)^T  -> one of NB buffers of 64 columns        O += P(t) V(t)   (P as TMEM A operand, V MN-major)
@@ -36,7 +36,9 @@ template <int DP> struct Cfg {
 struct FwdP {
   WinP w;
   Coords cq, ck, cv;
-  int n_qt, heads;          // heads = B * N * H
+  Split sp;
+  int n_qt, groups;         // tiles of queries; groups of heads in all sequences
+  int q_bytes;              // of a tile's rows of queries
   float c1;                 // D^-1/2 * log2(e)
   uint32_t fmt;
   int* status;
@@ -80,20 +82,21 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const uint32_t tO = t0 + NB * 64;
 
   // the last queries first: where windows are cut off at the start of the keys those have the most to do
-  const int qt = f.n_qt - 1 - (int)(blockIdx.x / f.heads), head = blockIdx.x % f.heads;
-  const int h = head % p.H, bn = head / p.H, n = bn % p.N, b = bn / p.N, hk = h / p.G;
-  const int i0 = qt * kQ, i1 = i0 + kQ < p.Lq ? i0 + kQ : p.Lq;
+  const int part = blockIdx.x % f.sp.splits, item = blockIdx.x / f.sp.splits;
+  const int qt = f.n_qt - 1 - item / f.groups, group = item % f.groups;
+  const int bn = group / head_groups(p), h0 = (group - bn * head_groups(p)) * p.pack, n = bn % p.N, b = bn / p.N, hk = h0 / p.G;
+  const int nq = queries_of<kQ>(p), i0 = qt * nq, i1 = i0 + nq < p.Lq ? i0 + nq : p.Lq;
   const KeyTiles tiles = key_tiles<kK>(p, i0, i1);
-  const int T_ = tiles.count();
+  const int first = (int)((int64_t)tiles.count() * part / f.sp.splits), T_ = (int)((int64_t)tiles.count() * (part + 1) / f.sp.splits) - first;
 
   if (warp == 4) {
     // ------------------------------------------------------------------------------------------------ copies
     if (elect_one() && T_ > 0) {
-      mbar_expect_tx(&bar.q_full, C::QB);
-      load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h, i0, n * f.cq.n_mul, b * f.cq.b_mul);
+      mbar_expect_tx(&bar.q_full, f.q_bytes);
+      load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h0, i0, n * f.cq.n_mul, b * f.cq.b_mul);
       int t = 0;
       for (; t < T_; ++t) {
-        const int s = t % NS, j0 = tiles.at(t) * kK;
+        const int s = t % NS, j0 = tiles.at(first + t) * kK;
         if (t >= NS) { wait_or_flag(&bar.k_empty[s], (t / NS - 1) & 1, abort_flag); wait_or_flag(&bar.v_empty[s], (t / NS - 1) & 1, abort_flag); }
         if (*abort_flag) break;
         mbar_expect_tx(&bar.k_full[s], C::KB);
@@ -141,17 +144,18 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const int r = warp * 32 + lane, i = i0 + r, at = i + p.off;
+    const int r = warp * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
+    const bool live = l_ < nq && i < p.Lq;
     const uint8_t* mask = p.mask ? p.mask + b * p.ms[0] + n * p.ms[1] : nullptr;
     auto mask_bytes = [&](int t, uint32_t (&mb)[2]) {
-      const int j = tiles.at(t) * kK + lane;
+      const int j = tiles.at(first + t) * kK + lane;
       mb[0] = j < p.Lk && mask[(int64_t)j * p.ms[2]]; mb[1] = j + 32 < p.Lk && mask[(int64_t)(j + 32) * p.ms[2]];
     };
     uint32_t mb[2] = {1, 1};
     if (mask && T_ > 0) mask_bytes(0, mb);
     float m = -INFINITY, l = 0.f;                 // m: the maximum that the sums refer to
     for (int t = 0; t < T_; ++t) {
-      const int j0 = tiles.at(t) * kK;
+      const int j0 = tiles.at(first + t) * kK;
       uint32_t keep[2] = {~0u, ~0u};
       if (mask) {
         keep[0] = __ballot_sync(0xffffffffu, mb[0]); keep[1] = __ballot_sync(0xffffffffu, mb[1]);
@@ -244,17 +248,31 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
     if (T_ > 0) wait_or_flag(&bar.pv_done, (T_ - 1) & 1, abort_flag);
     tc_fence_after();
     if (!__any_sync(0xffffffffu, *abort_flag)) {
-      T* out = static_cast<T*>(p.o) + (((int64_t)bn * p.Lq + i) * p.H + h) * p.D;
-      const int64_t step = (int64_t)p.H * p.D;
-      if (T_ > 0) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t row = ((int64_t)bn * p.Lq + i) * p.H + h;
+      const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m * f.c1 + lg2f(l)) * kLn2;
+      if (f.sp.splits > 1) {
+        float* out = f.sp.row(part, row, p.D);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
-          if (c * 32 < p.D) store_rows<T>(tO + lanes + c * 32, inv, out + c * 32, step, i, p.Lq, p.D - c * 32);
-      } else if (i < p.Lq) {
-        for (int d = 0; d < p.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < DP / 32; ++c) {
+          if (c * 32 >= p.D) break;
+          uint32_t o32[32];
+          if (T_ > 0) { tmem_ld32(tO + lanes + c * 32, o32); tmem_ld_wait(); pin32(o32); }
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (live && c * 32 + e < p.D) out[c * 32 + e] = T_ > 0 ? __uint_as_float(o32[e]) * inv : 0.f;
+        }
+        if (live) f.sp.lse(part, row, p.D) = lse;
+      } else {
+        T* out = static_cast<T*>(p.o) + row * p.D;
+        if (T_ > 0) {
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c)
+            if (c * 32 < p.D) store_rows_at<T>(tO + lanes + c * 32, inv, live ? out + c * 32 : nullptr, p.D - c * 32);
+        } else if (live) {
+          for (int d = 0; d < p.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (p.lse && live) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = lse;
       }
-      if (p.lse && i < p.Lq) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = l == 0.f ? -INFINITY : (m * f.c1 + lg2f(l)) * kLn2;
     }
   }
   tc_fence_before();
@@ -263,6 +281,8 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   if (warp == 0) tmem_dealloc(t0, C::COLS);
 }
 
+int tc_splits(const WinP& p) { return split_count<kQ, kK>(p, 2 * sm_count()); }
+
 template <int DP, typename T>
 int launch(const mf_window_args& a, cudaStream_t st) {
   using C = Cfg<DP>;
@@ -270,22 +290,25 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   FwdP f{};
   f.w = window_params(a);
   CUtensorMap mq, mk, mv;
-  if (int r = operand_map(&mq, &f.cq, a.q, a.dtype, a.B, a.N, a.Lq, a.H, a.D, a.q_strides, G::COLS, kQ)) return r;
-  if (int r = operand_map(&mk, &f.ck, a.k, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.k_strides, G::COLS, kK)) return r;
-  if (int r = operand_map(&mv, &f.cv, a.v, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.v_strides, G::COLS, kK)) return r;
-  f.n_qt = (a.Lq + kQ - 1) / kQ; f.heads = a.B * a.N * a.H;
+  if (int r = operand_map(&mq, &f.cq, a.q, a.dtype, a.B, a.N, a.Lq, a.H, a.D, a.q_strides, G::COLS, f.w.pack, queries_of<kQ>(f.w))) return r;
+  if (int r = operand_map(&mk, &f.ck, a.k, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.k_strides, G::COLS, 1, kK)) return r;
+  if (int r = operand_map(&mv, &f.cv, a.v, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.v_strides, G::COLS, 1, kK)) return r;
+  const int nq = queries_of<kQ>(f.w);
+  f.n_qt = (a.Lq + nq - 1) / nq; f.groups = a.B * a.N * head_groups(f.w);
+  f.q_bytes = nq * f.w.pack * DP * 2;
+  f.sp = Split{tc_splits(f.w), static_cast<float*>(a.workspace), (int64_t)a.B * a.N * a.Lq * a.H};
   f.c1 = kLog2e / sqrtf((float)a.D);
   f.fmt = a.dtype == MF_BF16 ? 1u : 0u;
   f.status = status_word();
   MF_REQUIRE(f.status, MF_ERR_CUDA, "could not allocate the device status word");
   MF_REQUIRE(tc_async_status() == 0, MF_ERR_CUDA, "an earlier tensor-core kernel gave up on a bounded wait; results are invalid");
-  const int64_t grid = (int64_t)f.n_qt * f.heads;
+  const int64_t grid = (int64_t)f.n_qt * f.groups * f.sp.splits;
   MF_REQUIRE((int64_t)a.B * a.N * a.H <= 0x7fffffff && grid <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%lld tiles of 128 queries are more than one launch takes", (long long)grid);
   constexpr auto kern = window_fwd_tc_kernel<DP, T>;
   if (int e = opt_in_smem<kern>(C::SMEM)) return e;
   kern<<<(unsigned)grid, kThreads, C::SMEM, st>>>(mq, mk, mv, f);
   MF_LAUNCHED("window_fwd_tc_kernel");
-  return MF_OK;
+  return f.sp.splits > 1 ? window_split_join(f.w, a.dtype, f.sp, st) : MF_OK;
 }
 template <typename T>
 int by_size(const mf_window_args& a, cudaStream_t st) {
@@ -300,6 +323,10 @@ bool window_tc_supported(const mf_window_args& a) {
 }  // namespace win
 
 bool window_fwd_tc_supported(const mf_window_args& a) { return win::window_tc_supported(a) && ((uintptr_t)a.o & 15) == 0; }
+size_t window_fwd_tc_workspace(const mf_window_args& a) {
+  const win::WinP p = win::window_params(a);
+  return win::split_bytes(p, win::tc_splits(p));
+}
 int window_fwd_tc(const mf_window_args& a, cudaStream_t st) {
   return a.dtype == MF_BF16 ? win::by_size<__nv_bfloat16>(a, st) : win::by_size<__half>(a, st);
 }

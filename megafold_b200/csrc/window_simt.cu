@@ -1,9 +1,9 @@
 // Sliding-window attention with sinks on CUDA cores, fp32 arithmetic throughout: fp32 tensors, and what the tensor-core kernels do
 // not take (head sizes that are no multiple of 8, unaligned or non-adjacent elements).
 //
-// Tiles and products are those of the dense attention's CUDA-core kernels.  Forward: a block per (b, n, h, 64 queries) walks the
+// Tiles and products are those of the dense attention's CUDA-core kernels.  Forward: a block per (b, n, 64 rows of queries) walks the
 // key tiles that its rows see, with the running maximum and sum of the softmax.  Backward, two kinds of blocks in one launch:
-// dQ per 64 queries, and dK / dV per 64 keys and chunk of their list of query blocks.  Nothing is added atomically: every
+// dQ per 64 rows of queries, and dK / dV per 64 keys and chunk of their list of query blocks.  Nothing is added atomically: every
 // result is a sum in a fixed order.  Bound: FP32 issue (66 % of it goes to the multiply-adds).
 //
 // Masked keys are read as zeros: whatever their rows hold (NaN, too) reaches nothing.  A row that sees no key gives 0, and a
@@ -17,14 +17,63 @@ namespace win {
 namespace {
 using namespace simt;
 
+// Rows of a tile of queries: query i0 + r / pack, head h0 + r % pack; `i` is past Lq where there is none.
+struct Row { int i, h; };
+__device__ __forceinline__ Row query_row(const WinP& p, int i0, int h0, int r) {
+  const int l = r / p.pack;
+  return Row{l < queries_of<kTile>(p) ? i0 + l : p.Lq, h0 + r - l * p.pack};
+}
 template <typename T, int DP>
-__device__ __forceinline__ void store_tile(void* out, int heads, int64_t bn, int h, int L, int D, int row0, int ty, int tx, const float (&acc)[4][DP / 16],
-                                           const float (&f)[4]) {
+__device__ __forceinline__ void load_queries(float* dst, const void* src, const int64_t* s, bool vec, const WinP& p, int b, int n, int i0, int h0) {
+  constexpr int pitch = DP + 4;
+  const T* base = static_cast<const T*>(src) + b * s[0] + n * s[1];
+#pragma unroll
+  for (int it = 0; it < kTile * DP / 4 / kThreads; ++it) {
+    const int idx = it * kThreads + threadIdx.x;
+    const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4;
+    const Row q = query_row(p, i0, h0, r);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (q.i < p.Lq && d < p.D) {
+      const T* at = base + q.i * s[2] + q.h * s[3];
+      if (vec) {
+        __align__(16) T e[4];
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(at + d));
+        else *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(at + d));
+        v = make_float4(to_f(e[0]), to_f(e[1]), to_f(e[2]), to_f(e[3]));
+      } else {
+        v.x = to_f(at[d * s[4]]);
+        if (d + 1 < p.D) v.y = to_f(at[(d + 1) * s[4]]);
+        if (d + 2 < p.D) v.z = to_f(at[(d + 2) * s[4]]);
+        if (d + 3 < p.D) v.w = to_f(at[(d + 3) * s[4]]);
+      }
+    }
+    *reinterpret_cast<float4*>(dst + r * pitch + d) = v;
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_keys(void* out, const WinP& p, int64_t bn, int h, int row0, int ty, int tx, const float (&acc)[4][DP / 16], float f) {
+  const int D = p.D;
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     const int l = row0 + ty + 16 * a;
-    if (l >= L) continue;
-    T* row = static_cast<T*>(out) + ((bn * L + l) * heads + h) * D;
+    if (l >= p.Lk) continue;
+    T* row = static_cast<T*>(out) + ((bn * p.Lk + l) * p.Hk + h) * D;
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) {
+      const int d = tx * (DP / 16) + e;
+      if (d < D) row[d] = from_f<T>(acc[a][e] * f);
+    }
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void store_queries(void* out, const WinP& p, int64_t bn, int i0, int h0, int ty, int tx, const float (&acc)[4][DP / 16], const float (&f)[4]) {
+  const int D = p.D;
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const Row q = query_row(p, i0, h0, ty + 16 * a);
+    if (q.i >= p.Lq) continue;
+    T* row = static_cast<T*>(out) + ((bn * p.Lq + q.i) * p.H + q.h) * D;
 #pragma unroll
     for (int e = 0; e < DP / 16; ++e) {
       const int d = tx * (DP / 16) + e;
@@ -34,14 +83,15 @@ __device__ __forceinline__ void store_tile(void* out, int heads, int64_t bn, int
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_constant__ WinP p) {
+__global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_constant__ WinP p, const Split sp) {
   extern __shared__ __align__(16) float smem[];
   constexpr int kOp = kTile * (DP + 4);
   float *Qs = smem, *Ks = Qs + kOp, *Vs = Ks + kOp, *Ps = Vs + kOp;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int h = blockIdx.y, hk = h / p.G, bn = blockIdx.z, b = bn / p.N, n = bn - b * p.N, i0 = blockIdx.x * kTile;
-  const int i1 = i0 + kTile < p.Lq ? i0 + kTile : p.Lq;
-  load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+  const int h0 = blockIdx.y * p.pack, hk = h0 / p.G, bn = blockIdx.z, b = bn / p.N, n = bn - b * p.N;
+  const int part = blockIdx.x % sp.splits, i0 = blockIdx.x / sp.splits * queries_of<kTile>(p);
+  const int i1 = i0 + queries_of<kTile>(p) < p.Lq ? i0 + queries_of<kTile>(p) : p.Lq;
+  load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
   const auto keep = [&](int j) { return kept(p, b, n, j); };
   float acc[4][DP / 16], m[4], l[4];
 #pragma unroll
@@ -51,7 +101,11 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
     for (int e = 0; e < DP / 16; ++e) acc[a][e] = 0.f;
   }
   const KeyTiles tiles = key_tiles<kTile>(p, i0, i1);
-  for (int t = 0; t < tiles.count(); ++t) {
+  const int t_end = (int)((int64_t)tiles.count() * (part + 1) / sp.splits);
+  int at[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) at[a] = query_row(p, i0, h0, ty + 16 * a).i;
+  for (int t = (int)((int64_t)tiles.count() * part / sp.splits); t < t_end; ++t) {
     const int j0 = tiles.at(t) * kTile;
     __syncthreads();
     load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
@@ -64,9 +118,8 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
     dot_tile<DP>(Qs, Ks, ty, tx, s);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const int i = i0 + ty + 16 * a;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[a][c] = see[c] && in_window(p, i, j0 + tx + 16 * c) ? s[a][c] * p.scale : -INFINITY;
+      for (int c = 0; c < 4; ++c) s[a][c] = see[c] && in_window(p, at[a], j0 + tx + 16 * c) ? s[a][c] * p.scale : -INFINITY;
       const float m_new = fmaxf(m[a], row_max(fmaxf(fmaxf(s[a][0], s[a][1]), fmaxf(s[a][2], s[a][3]))));
       const float m_ref = m_new == -INFINITY ? 0.f : m_new;         // nothing seen so far
       const float corr = expf(m[a] - m_ref);
@@ -88,12 +141,26 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
   float inv[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) inv[a] = l[a] > 0.f ? 1.f / l[a] : l[a] == 0.f ? 0.f : l[a];      // NaN stays
-  store_tile<T, DP>(p.o, p.H, bn, h, p.Lq, p.D, i0, ty, tx, acc, inv);
+  if (sp.splits > 1) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const Row q = query_row(p, i0, h0, ty + 16 * a);
+      if (q.i >= p.Lq) continue;
+      const int64_t r = ((int64_t)bn * p.Lq + q.i) * p.H + q.h;
+      float* row = sp.row(part, r, p.D);
+#pragma unroll
+      for (int e = 0; e < DP / 16; ++e)
+        if (tx * (DP / 16) + e < p.D) row[tx * (DP / 16) + e] = acc[a][e] * inv[a];
+      if (tx == 0) sp.lse(part, r, p.D) = m[a] + logf(l[a]);
+    }
+    return;
+  }
+  store_queries<T, DP>(p.o, p, bn, i0, h0, ty, tx, acc, inv);
   if (tx == 0 && p.lse)
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const int i = i0 + ty + 16 * a;
-      if (i < p.Lq) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = m[a] + logf(l[a]);
+      const Row q = query_row(p, i0, h0, ty + 16 * a);
+      if (q.i < p.Lq) p.lse[((int64_t)bn * p.H + q.h) * p.Lq + q.i] = m[a] + logf(l[a]);
     }
 }
 
@@ -117,23 +184,25 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
   load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
   int lo, hi;
   query_range(p, j0, j0 + kTile < p.Lk ? j0 + kTile : p.Lk, lo, hi);
-  const int first = lo / kTile, per_head = hi > lo ? (hi + kTile - 1) / kTile - first : 1;
+  const int nq = queries_of<kTile>(p), first = lo / nq, per_head = hi > lo ? (hi + nq - 1) / nq - first : 1;
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   bool see[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) see[a] = j0 + ty + 16 * a < p.Lk && keep(j0 + ty + 16 * a);
   for (int e = e0; e < len && e < e0 + c.chunk; ++e) {
-    const int h = hk * p.G + e / per_head, i0 = (first + e % per_head) * kTile;
+    const int h0 = hk * p.G + e / per_head * p.pack, i0 = (first + e % per_head) * nq;
     __syncthreads();
-    load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+    load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
     const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
-    load_tile<T, DP>(Gs, p.d_o, gs, p.g_vec, b, n, h, i0, p.Lq, p.D);
+    load_queries<T, DP>(Gs, p.d_o, gs, p.g_vec, p, b, n, i0, h0);
     float lse[4], dl[4];
+    int at[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = i0 + tx + 16 * k;
-      const int64_t row = ((int64_t)bn * p.H + h) * p.Lq + i;
-      lse[k] = i < p.Lq ? p.lse[row] : 0.f; dl[k] = i < p.Lq ? p.delta[row] : 0.f;
+      const Row q = query_row(p, i0, h0, tx + 16 * k);
+      at[k] = q.i;
+      const int64_t row = ((int64_t)bn * p.H + q.h) * p.Lq + q.i;
+      lse[k] = q.i < p.Lq ? p.lse[row] : 0.f; dl[k] = q.i < p.Lq ? p.delta[row] : 0.f;
     }
     __syncthreads();
     float s[4][4] = {}, dp[4][4] = {};
@@ -143,9 +212,9 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i = i0 + tx + 16 * k, j = j0 + ty + 16 * a;
+        const int j = j0 + ty + 16 * a;
         float pr, ds;
-        p_ds(p, see[a] && i < p.Lq && in_window(p, i, j), s[a][k], dp[a][k], lse[k], dl[k], pr, ds);
+        p_ds(p, see[a] && at[k] < p.Lq && in_window(p, at[k], j), s[a][k], dp[a][k], lse[k], dl[k], pr, ds);
         Ps[(ty + 16 * a) * kPPitch + tx + 16 * k] = pr;
         Ds[(ty + 16 * a) * kPPitch + tx + 16 * k] = ds;
       }
@@ -164,27 +233,28 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
       }
     return;
   }
-  const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_tile<T, DP>(p.dk, p.Hk, bn, hk, p.Lk, p.D, j0, ty, tx, dk, sc);
-  store_tile<T, DP>(p.dv, p.Hk, bn, hk, p.Lk, p.D, j0, ty, tx, dv, one);
+  store_keys<T, DP>(p.dk, p, bn, hk, j0, ty, tx, dk, p.scale);
+  store_keys<T, DP>(p.dv, p, bn, hk, j0, ty, tx, dv, 1.f);
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h, int i0) {
+__device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h0, int i0) {
   constexpr int kOp = kTile * (DP + 4);
   float *Ks = smem, *Vs = Ks + kOp, *Qs = Vs + kOp, *Gs = Qs + kOp, *Ds = Gs + kOp;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, b = bn / p.N, n = bn - b * p.N, hk = h / p.G;
-  const int i1 = i0 + kTile < p.Lq ? i0 + kTile : p.Lq;
-  load_tile<T, DP>(Qs, p.q, p.qs, p.q_vec, b, n, h, i0, p.Lq, p.D);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, b = bn / p.N, n = bn - b * p.N, hk = h0 / p.G;
+  const int i1 = i0 + queries_of<kTile>(p) < p.Lq ? i0 + queries_of<kTile>(p) : p.Lq;
+  load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
   const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
-  load_tile<T, DP>(Gs, p.d_o, gs, p.g_vec, b, n, h, i0, p.Lq, p.D);
+  load_queries<T, DP>(Gs, p.d_o, gs, p.g_vec, p, b, n, i0, h0);
   const auto keep = [&](int j) { return kept(p, b, n, j); };
   float dq[4][DP / 16] = {}, lse[4], dl[4];
+  int at[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const int i = i0 + ty + 16 * a;
-    const int64_t row = ((int64_t)bn * p.H + h) * p.Lq + i;
-    lse[a] = i < p.Lq ? p.lse[row] : 0.f; dl[a] = i < p.Lq ? p.delta[row] : 0.f;
+    const Row q = query_row(p, i0, h0, ty + 16 * a);
+    at[a] = q.i;
+    const int64_t row = ((int64_t)bn * p.H + q.h) * p.Lq + q.i;
+    lse[a] = q.i < p.Lq ? p.lse[row] : 0.f; dl[a] = q.i < p.Lq ? p.delta[row] : 0.f;
   }
   const KeyTiles tiles = key_tiles<kTile>(p, i0, i1);
   for (int t = 0; t < tiles.count(); ++t) {
@@ -203,16 +273,15 @@ __device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int i = i0 + ty + 16 * a;
         float pr, ds;
-        p_ds(p, see[c] && i < p.Lq && in_window(p, i, j0 + tx + 16 * c), s[a][c], dp[a][c], lse[a], dl[a], pr, ds);
+        p_ds(p, see[c] && at[a] < p.Lq && in_window(p, at[a], j0 + tx + 16 * c), s[a][c], dp[a][c], lse[a], dl[a], pr, ds);
         Ds[(ty + 16 * a) * kPPitch + tx + 16 * c] = ds;
       }
     __syncwarp();
     sum_tile<DP>(Ds, Ks, ty, tx, dq);
   }
   const float sc[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_tile<T, DP>(p.dq, p.H, bn, h, p.Lq, p.D, i0, ty, tx, dq, sc);
+  store_queries<T, DP>(p.dq, p, bn, i0, h0, ty, tx, dq, sc);
 }
 
 // blocks [0, n_dkv) work on dK and dV (the longest first: tiles with sinks lead), the others on dQ
@@ -226,10 +295,11 @@ __global__ void __launch_bounds__(kThreads) window_bwd_simt_kernel(const __grid_
     const int64_t head = u - (int64_t)x * heads;
     bwd_dkv<T, DP>(p, c, parts, smem, (int)(head / p.Hk), (int)(head % p.Hk), x);
   } else {
-    const int64_t w = u - n_dkv, all = (int64_t)p.B * p.N * p.H;
+    const int groups = head_groups(p);
+    const int64_t w = u - n_dkv, all = (int64_t)p.B * p.N * groups;
     const int t = (int)(w / all);
-    const int64_t head = w - t * all;
-    bwd_dq<T, DP>(p, smem, (int)(head / p.H), (int)(head % p.H), t * kTile);
+    const int64_t g = w - t * all;
+    bwd_dq<T, DP>(p, smem, (int)(g / groups), (int)(g % groups) * p.pack, t * queries_of<kTile>(p));
   }
 }
 
@@ -265,14 +335,46 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const T* __restrict__
   }
 }
 
+// a warp a row: the parts weighed by exp(their log-sum-exp)
 template <typename T>
-int run_fwd(const WinP& p, cudaStream_t st) {
+__global__ void __launch_bounds__(256) window_split_join_kernel(const __grid_constant__ WinP p, const Split sp) {
+  const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (r >= sp.rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < sp.splits; ++s) { const float x = sp.lse(s, r, p.D); m = x > m || x != x ? x : m; }      // NaN stays
+  float sum = 0.f;
+  const float m_ref = m == -INFINITY ? 0.f : m;
+  for (int s = 0; s < sp.splits; ++s) sum += expf(sp.lse(s, r, p.D) - m_ref);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int d = lane; d < p.D; d += 32) {
+    float o = 0.f;
+    for (int s = 0; s < sp.splits; ++s) {
+      const float w = expf(sp.lse(s, r, p.D) - m_ref);
+      if (w != 0.f) o = fmaf(w, sp.row(s, r, p.D)[d], o);
+    }
+    static_cast<T*>(p.o)[r * p.D + d] = from_f<T>(o * inv);
+  }
+  if (lane == 0 && p.lse) {
+    const int h = (int)(r % p.H);
+    const int64_t t = r / p.H, bn = t / p.Lq;
+    p.lse[(bn * p.H + h) * p.Lq + (t - bn * p.Lq)] = m + logf(sum);
+  }
+}
+
+int simt_splits(const WinP& p) { return split_count<kTile, kTile>(p, 2 * tcx::sm_count()); }
+
+template <typename T>
+int run_fwd(const WinP& p, const Split& sp, cudaStream_t st) {
   const auto go = [&](auto dp) -> int {
     constexpr int DP = decltype(dp)::value;
     constexpr size_t smem = sizeof(float) * (3 * kTile * (DP + 4) + kTile * kPPitch);
     constexpr auto kern = window_fwd_simt_kernel<T, DP>;
     if (int e = opt_in_smem<kern>(smem)) return e;
-    kern<<<dim3((p.Lq + kTile - 1) / kTile, p.H, p.B * p.N), kThreads, smem, st>>>(p);
+    const int q = queries_of<kTile>(p);
+    const int64_t gx = (int64_t)((p.Lq + q - 1) / q) * sp.splits;
+    MF_REQUIRE(gx <= 0x7fffffff, MF_ERR_UNSUPPORTED, "too many tiles of queries for one launch");
+    kern<<<dim3((unsigned)gx, head_groups(p), p.B * p.N), kThreads, smem, st>>>(p, sp);
     MF_LAUNCHED("window_fwd_simt_kernel");
     return MF_OK;
   };
@@ -286,7 +388,8 @@ int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
     constexpr size_t smem = sizeof(float) * (4 * kTile * (DP + 4) + 2 * kTile * kPPitch);
     constexpr auto kern = window_bwd_simt_kernel<T, DP>;
     if (int e = opt_in_smem<kern>(smem)) return e;
-    const int64_t n_dkv = (int64_t)c.x_total * p.B * p.N * p.Hk, blocks = n_dkv + (int64_t)((p.Lq + kTile - 1) / kTile) * p.B * p.N * p.H;
+    const int64_t n_dkv = (int64_t)c.x_total * p.B * p.N * p.Hk, q = queries_of<kTile>(p);
+    const int64_t blocks = n_dkv + (int64_t)((p.Lq + q - 1) / q) * p.B * p.N * head_groups(p);
     MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%lld blocks of 64 rows are more than one launch takes", (long long)blocks);
     kern<<<(unsigned)blocks, kThreads, smem, st>>>(p, c, parts, n_dkv);
     MF_LAUNCHED("window_bwd_simt_kernel");
@@ -311,6 +414,7 @@ KeyPlan simt_plan(const WinP& p) { return key_plan<kTile, kTile>(p, 2 * tcx::sm_
 WinP window_params(const mf_window_args& a) {
   WinP p{};
   p.B = a.B; p.N = a.N; p.Lq = a.Lq; p.Lk = a.Lk; p.H = a.H; p.Hk = a.Hk; p.D = a.D; p.G = a.H / a.Hk;
+  p.pack = p.G <= 64 ? p.G : 1;
   const int reach = a.Lq + a.Lk;                       // wider than that sees no more
   p.left = a.left < reach ? a.left : reach; p.right = a.right < reach ? a.right : reach;
   p.sinks = a.sinks < a.Lk ? a.sinks : a.Lk;
@@ -326,6 +430,14 @@ WinP window_params(const mf_window_args& a) {
   p.q_vec = rows_vec(a.q, p.qs, a.D, es); p.k_vec = rows_vec(a.k, p.ks, a.D, es); p.v_vec = rows_vec(a.v, p.vs, a.D, es);
   p.g_vec = rows_vec(a.d_o, gs, a.D, es);
   return p;
+}
+
+int window_split_join(const WinP& p, int dtype, const Split& s, cudaStream_t st) {
+  MF_DISPATCH_FLOAT(dtype, T, {
+    window_split_join_kernel<T><<<(unsigned)((s.rows + 7) / 8), 256, 0, st>>>(p, s);
+    MF_LAUNCHED("window_split_join_kernel");
+  });
+  return MF_OK;
 }
 
 int window_delta(const WinP& p, int dtype, float* delta, cudaStream_t st) {
@@ -344,11 +456,17 @@ int window_delta(const WinP& p, int dtype, float* delta, cudaStream_t st) {
 
 using namespace win;
 
+size_t window_fwd_simt_workspace(const mf_window_args& a) {
+  const WinP p = window_params(a);
+  return split_bytes(p, simt_splits(p));
+}
+
 int window_fwd_simt(const mf_window_args& a, cudaStream_t st) {
   const WinP p = window_params(a);
+  const Split sp{simt_splits(p), static_cast<float*>(a.workspace), (int64_t)p.B * p.N * p.Lq * p.H};
   int r = MF_OK;
-  MF_DISPATCH_FLOAT(a.dtype, T, r = run_fwd<T>(p, st));
-  return r;
+  MF_DISPATCH_FLOAT(a.dtype, T, r = run_fwd<T>(p, sp, st));
+  return r || sp.splits == 1 ? r : window_split_join(p, a.dtype, sp, st);
 }
 
 size_t window_bwd_simt_workspace(const mf_window_args& a) {
