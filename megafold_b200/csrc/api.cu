@@ -447,7 +447,10 @@ int mf_window_fwd(const mf_window_args* args, void* stream) {
   return r;
 }
 
-size_t mf_window_bwd_workspace_bytes(const mf_window_args* args) { return args && check_window(*args) == MF_OK ? window_bwd_simt_workspace(*args) : 0; }
+size_t mf_window_bwd_workspace_bytes(const mf_window_args* args) {
+  if (!args || check_window(*args) != MF_OK) return 0;
+  return window_bwd_tc_supported(*args) ? window_bwd_tc_workspace(*args) : window_bwd_simt_workspace(*args);
+}
 
 int mf_window_bwd(const mf_window_args* args, void* stream) {
   Range nvtx_range("mf_window_bwd");
@@ -458,8 +461,9 @@ int mf_window_bwd(const mf_window_args* args, void* stream) {
   MF_REQUIRE(a.dq && a.dk && a.dv, MF_ERR_BAD_ARG, "dq, dk and dv must not be NULL");
   r = check_device(); if (r) return r;
   r = check_workspace(a.workspace, a.workspace_bytes, mf_window_bwd_workspace_bytes(args)); if (r) return r;
-  r = window_bwd_simt(a, static_cast<cudaStream_t>(stream));
-  if (r == MF_OK) set_last_path("simt");
+  const bool tc = window_bwd_tc_supported(a);
+  r = tc ? window_bwd_tc(a, static_cast<cudaStream_t>(stream)) : window_bwd_simt(a, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path(tc ? "tcgen05" : "simt");
   return r;
 }
 

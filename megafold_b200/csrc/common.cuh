@@ -201,6 +201,9 @@ int qk_rotary_bwd(const mf_qk_rotary_args& a, cudaStream_t st);
 bool window_fwd_tc_supported(const mf_window_args& a);
 size_t window_fwd_tc_workspace(const mf_window_args& a);
 int window_fwd_tc(const mf_window_args& a, cudaStream_t st);
+bool window_bwd_tc_supported(const mf_window_args& a);
+size_t window_bwd_tc_workspace(const mf_window_args& a);
+int window_bwd_tc(const mf_window_args& a, cudaStream_t st);
 size_t window_fwd_simt_workspace(const mf_window_args& a);
 int window_fwd_simt(const mf_window_args& a, cudaStream_t st);
 size_t window_bwd_simt_workspace(const mf_window_args& a);
