@@ -101,12 +101,18 @@ __device__ __forceinline__ int element(const Unit<V, IL>& u, int e) {
   else return e < V ? u.a + e : u.b + e - V;
 }
 
+// the weights of a unit from a row of fp32 in shared memory
 template <int V, bool IL>
-__device__ __forceinline__ void load_weight(const void* w, int64_t at, int dt, const Unit<V, IL>& u, int D, float (&out)[2 * V]) {
+__device__ __forceinline__ void load_weight(const float* w, const Unit<V, IL>& u, float (&out)[2 * V]) {
 #pragma unroll
-  for (int e = 0; e < 2 * V; ++e) {
-    const int i = element<V, IL>(u, e);
-    out[e] = i >= D ? 0.f : w ? load_rt(w, at + i, dt) : 1.f;
+  for (int e = 0; e < V; ++e) {
+    const int a = u.has_a ? u.a : 0, b = u.has_b ? u.b : 0;                          // where there is nothing x is 0
+    if constexpr (IL && V > 1) {
+      out[e] = 2 * e < V ? w[a + 2 * e] : w[b + 2 * e - V];
+      out[V + e] = 2 * e + 1 < V ? w[a + 2 * e + 1] : w[b + 2 * e + 1 - V];
+    } else {
+      out[e] = w[a + e]; out[V + e] = w[b + e];
+    }
   }
 }
 __device__ __forceinline__ float row_sum(float v, int lpr) {
@@ -116,17 +122,53 @@ __device__ __forceinline__ float row_sum(float v, int lpr) {
 
 // blockIdx.y = group of heads_per heads (of the H + Hk of queries and keys); threads of a block walk tokens.
 // UPL: units of a thread.  (Every thread of a warp takes part in each sum: rows that do not exist are zeros.)
+// The weights of the block's heads wait in shared memory as fp32: read from global memory for each row, converted from a type known
+// at run time, they were most of the instructions (4 + 4 heads of 32, 147456 tokens: 96 us forward, 220 backward).
 template <typename T, int V, int UPL, bool IL, bool BWD>
 __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_constant__ RotP p) {
   const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr, slots = kThreads >> p.log_lpr;
   const int heads = p.H + p.Hk, g0 = blockIdx.y * p.heads_per, g1 = g0 + p.heads_per < heads ? g0 + p.heads_per : heads;
   const float inv_d = 1.f / p.D;
+  extern __shared__ __align__(16) float shared[];
+  float* const ws = shared;                                    // [1 (no weights), 2 (shared: q, k) or heads of the group][D]
+  if (!p.qw) {
+    for (int x = threadIdx.x; x < p.D; x += kThreads) ws[x] = 1.f;
+  } else if (!p.w_head) {
+    for (int x = threadIdx.x; x < 2 * p.D; x += kThreads) ws[x] = x < p.D ? load_rt(p.qw, x, p.w_dtype) : load_rt(p.kw, x - p.D, p.w_dtype);
+  } else {
+    for (int x = threadIdx.x; x < (g1 - g0) * p.D; x += kThreads) {
+      const int64_t at = (int64_t)g0 * p.D + x, nq = (int64_t)p.H * p.D;
+      ws[x] = at < nq ? load_rt(p.qw, at, p.w_dtype) : load_rt(p.kw, at - nq, p.w_dtype);
+    }
+  }
+  __syncthreads();
   float dwq[BWD ? UPL : 1][2 * V] = {}, dwk[BWD ? UPL : 1][2 * V] = {};
   const int64_t stride = (int64_t)gridDim.x * slots, rounds = (p.tokens + stride - 1) / stride;
   for (int64_t it = 0; it < rounds; ++it) {
     const int64_t tok = it * stride + (int64_t)blockIdx.x * slots + slot;
     const bool live = tok < p.tokens;
     const int64_t bn = live ? tok / p.L : 0, l = live ? tok - bn * p.L : 0, b = bn / p.N, n = bn - b * p.N;
+    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1] + l * p.qs[2];
+    const T* kk = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1] + l * p.ks[2];
+    auto unit = [&](int k) {
+      Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+      u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+      return u;
+    };
+    auto fetch = [&](int g, float (&x)[UPL][2 * V], float (&d)[BWD ? UPL : 1][2 * V]) {
+      const bool is_q = g < p.H;
+      const int h = is_q ? g : g - p.H;
+      const T* row = is_q ? q + h * p.qs[3] : kk + h * p.ks[3];
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(row, is_q ? p.qs[4] : p.ks[4], unit(k), x[k]);
+      if constexpr (BWD) {
+        const T* dr = static_cast<const T*>(is_q ? p.dq_out : p.dk_out) + (tok * (is_q ? p.H : p.Hk) + h) * p.D;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(dr, 1, unit(k), d[k]);
+      }
+    };
+    float x[UPL][2 * V], d[BWD ? UPL : 1][2 * V];
+    fetch(g0, x, d);                                           // on its way while the angles are formed
     double pos = (double)l;
     if (p.pos) {
       const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
@@ -143,48 +185,31 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
         if (turned && live) turn_of(pos, p.inv_freq[u * V + e], sn[k][e], cs[k][e]);
       }
     }
-    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1] + l * p.qs[2];
-    const T* kk = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1] + l * p.ks[2];
-#pragma unroll 2
     for (int g = g0; g < g1; ++g) {
       const bool is_q = g < p.H;
       const int h = is_q ? g : g - p.H;
-      const T* row = is_q ? q + h * p.qs[3] : kk + h * p.ks[3];
-      const int64_t sd = is_q ? p.qs[4] : p.ks[4], out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
-      const void* w = is_q ? p.qw : p.kw;
-      float x[UPL][2 * V], ss = 0.f;
+      const int64_t out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
+      const float* w = ws + (!p.qw ? 0 : !p.w_head ? (is_q ? 0 : p.D) : (g - g0) * p.D);
+      float ss = 0.f;
 #pragma unroll
-      for (int k = 0; k < UPL; ++k) {
-        Unit<V, IL> u(lane + k * lpr, p.R, p.D);
-        u.has_a = u.has_a && live; u.has_b = u.has_b && live;
-        load_unit<T, V, IL>(row, sd, u, x[k]);
+      for (int k = 0; k < UPL; ++k)
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) ss = fmaf(x[k][e], x[k][e], ss);
-      }
-      float d[BWD ? UPL : 1][2 * V];
-      if constexpr (BWD) {
-        const T* dr = static_cast<const T*>(is_q ? p.dq_out : p.dk_out) + out_at;
-#pragma unroll
-        for (int k = 0; k < UPL; ++k) {
-          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
-          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
-          load_unit<T, V, IL>(dr, 1, u, d[k]);
-        }
-      }
       const float rstd = rsqrtf(fmaf(row_sum(ss, lpr), inv_d, p.eps));
+      float xn[UPL][2 * V], dn[BWD ? UPL : 1][2 * V];
+      if (g + 1 < g1) fetch(g + 1, xn, dn);
       if constexpr (!BWD) {
         T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + out_at;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
-          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+          const Unit<V, IL> u = unit(k);
           float wt[2 * V];
-          load_weight<V, IL>(w, h * p.w_head, p.w_dtype, u, p.D, wt);
+          load_weight<V, IL>(w, u, wt);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float y1 = x[k][e] * rstd * wt[e], y2 = x[k][V + e] * rstd * wt[V + e];
-            x[k][e] = u.turned ? y1 * cs[k][e] - y2 * sn[k][e] : y1;
-            x[k][V + e] = u.turned ? y2 * cs[k][e] + y1 * sn[k][e] : y2;
+            x[k][e] = y1 * cs[k][e] - y2 * sn[k][e];           // by 1 and 0 where nothing turns
+            x[k][V + e] = y2 * cs[k][e] + y1 * sn[k][e];
           }
           store_unit<T, V, IL>(out, u, x[k]);
         }
@@ -192,14 +217,13 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
         float dot = 0.f;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
           float wt[2 * V];
-          load_weight<V, IL>(w, h * p.w_head, p.w_dtype, u, p.D, wt);
+          load_weight<V, IL>(w, unit(k), wt);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float d1 = d[k][e], d2 = d[k][V + e];
-            d[k][e] = u.turned ? d1 * cs[k][e] + d2 * sn[k][e] : d1;
-            d[k][V + e] = u.turned ? d2 * cs[k][e] - d1 * sn[k][e] : d2;
+            d[k][e] = d1 * cs[k][e] + d2 * sn[k][e];
+            d[k][V + e] = d2 * cs[k][e] - d1 * sn[k][e];
           }
 #pragma unroll
           for (int e = 0; e < 2 * V; ++e) {
@@ -214,18 +238,25 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
         T* out = static_cast<T*>(is_q ? p.dq : p.dk) + out_at;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          Unit<V, IL> u(lane + k * lpr, p.R, p.D);
-          u.has_a = u.has_a && live; u.has_b = u.has_b && live;
 #pragma unroll
           for (int e = 0; e < 2 * V; ++e) x[k][e] = rstd * fmaf(-x[k][e], dot, d[k][e]);
-          store_unit<T, V, IL>(out, u, x[k]);
+          store_unit<T, V, IL>(out, unit(k), x[k]);
         }
+      }
+      if (g + 1 < g1) {
+#pragma unroll
+        for (int k = 0; k < UPL; ++k)
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) {
+            x[k][e] = xn[k][e];
+            if constexpr (BWD) d[k][e] = dn[k][e];
+          }
       }
     }
   }
   if constexpr (BWD) {
     if (!p.parts) return;
-    extern __shared__ float sum[];                             // [slots][D]
+    float* const sum = shared;                                 // [slots][D]
     float* out = p.parts + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -249,22 +280,25 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
   }
 }
 
-// Weight gradients: row x of [2][heads or 1][D] is the sum of its blocks' rows, a warp an element.
-__global__ void __launch_bounds__(kThreads) qk_rotary_join_kernel(const float* __restrict__ parts, int gx, int gy, int D, int H, int Hk, bool per_head, void* __restrict__ dqw,
-                                                                  void* __restrict__ dkw, int w_dtype) {
-  const int x = (blockIdx.x * kThreads + threadIdx.x) >> 5, l = threadIdx.x & 31;
-  const int q_rows = per_head ? H : 1, k_rows = per_head ? Hk : 1;
-  if (x >= (q_rows + k_rows) * D) return;
-  const int row = x / D, i = x - row * D;
+// Weight gradients: blockIdx = (32 elements, row of [H or 1 + Hk or 1]); a row is the sum of its blocks' rows, 32 of them at a time.
+__global__ void __launch_bounds__(1024) qk_rotary_join_kernel(const float* __restrict__ parts, int gx, int gy, int D, int H, int Hk, bool per_head, void* __restrict__ dqw,
+                                                              void* __restrict__ dkw, int w_dtype) {
+  __shared__ float sums[32][33];
+  const int q_rows = per_head ? H : 1, row = blockIdx.y, i = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
   const bool is_k = row >= q_rows;
-  const int y0 = per_head ? row : 0, y1 = per_head ? row + 1 : gy;        // per head: a group of blocks each, queries' heads first
-  double s = 0.;
-  for (int64_t k = (int64_t)y0 * gx + l; k < (int64_t)y1 * gx; k += 32) s += parts[(k * 2 + is_k) * D + i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (l) return;
-  if (is_k) store_rt(dkw, (int64_t)(row - q_rows) * D + i, w_dtype, (float)s);
-  else store_rt(dqw, (int64_t)row * D + i, w_dtype, (float)s);
+  const int64_t k0 = per_head ? (int64_t)row * gx : 0, k1 = per_head ? k0 + gx : (int64_t)gy * gx;        // per head: a group of blocks each, queries' heads first
+  float s = 0.f;
+  if (i < D) {
+#pragma unroll 8
+    for (int64_t k = k0 + warp; k < k1; k += 32) s += parts[(k * 2 + is_k) * D + i];
+  }
+  sums[warp][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (warp || i >= D) return;
+  s = 0.f;
+  for (int k = 0; k < 32; ++k) s += sums[k][threadIdx.x];
+  if (is_k) store_rt(dkw, (int64_t)(row - q_rows) * D + i, w_dtype, s);
+  else store_rt(dqw, (int64_t)row * D + i, w_dtype, s);
 }
 
 RotP rot_params(const mf_qk_rotary_args& a) {
@@ -306,6 +340,8 @@ Plan plan(const mf_qk_rotary_args& a, int V, bool bwd) {
   // each head has a weight of its own whose gradient a block sums
   c.heads_per = heads;
   if (bwd && a.per_head && a.dq_weight) c.heads_per = 1;
+  if (a.per_head && a.q_weight)
+    while (c.heads_per > 1 && (size_t)c.heads_per * a.D * sizeof(float) > 24 * 1024) c.heads_per = (c.heads_per + 1) / 2;
   while (c.heads_per > 1 && blocks * ((heads + c.heads_per - 1) / c.heads_per) < want) c.heads_per = (c.heads_per + 1) / 2;
   c.gy = (heads + c.heads_per - 1) / c.heads_per;
   int64_t gx = blocks;
@@ -321,10 +357,11 @@ int run(const mf_qk_rotary_args& a, cudaStream_t st) {
   RotP p = rot_params(a);
   const Plan c = plan(a, V, BWD);
   p.log_lpr = c.log_lpr; p.heads_per = c.heads_per;
-  size_t smem = 0;
+  size_t smem = sizeof(float) * a.D * (!a.q_weight ? 1 : !a.per_head ? 2 : c.heads_per);
   if (BWD && a.dq_weight) {
     p.parts = static_cast<float*>(a.workspace);
-    smem = sizeof(float) * (kThreads >> c.log_lpr) * a.D;
+    const size_t sums = sizeof(float) * (kThreads >> c.log_lpr) * a.D;
+    if (sums > smem) smem = sums;
   }
   const auto go = [&](auto il) -> int {
     constexpr auto kern = qk_rotary_kernel<T, V, UPL, decltype(il)::value, BWD>;
@@ -336,7 +373,7 @@ int run(const mf_qk_rotary_args& a, cudaStream_t st) {
   if (int e = a.interleaved ? go(std::true_type{}) : go(std::false_type{})) return e;
   if (BWD && a.dq_weight) {
     const int rows = a.per_head ? a.H + a.Hk : 2;
-    qk_rotary_join_kernel<<<(rows * a.D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(p.parts, c.gx, c.gy, a.D, a.H, a.Hk, a.per_head != 0, a.dq_weight, a.dk_weight,
+    qk_rotary_join_kernel<<<dim3((a.D + 31) / 32, rows), 1024, 0, st>>>(p.parts, c.gx, c.gy, a.D, a.H, a.Hk, a.per_head != 0, a.dq_weight, a.dk_weight,
                                                                                                 a.w_dtype);
     MF_LAUNCHED("qk_rotary_join_kernel");
   }

@@ -31,18 +31,22 @@ __device__ __forceinline__ int64_t load_int(const void* p, int64_t i, bool wide)
 __device__ __forceinline__ int64_t q_position(const RelP& p, int b, int i) { return p.q_pos ? load_int(p.q_pos, b * p.qp_b + i, p.pos64) : (int64_t)i + (p.Lk - p.Lq); }
 __device__ __forceinline__ int64_t k_position(const RelP& p, int b, int j) { return p.k_pos ? load_int(p.k_pos, b * p.kp_b + j, p.pos64) : (int64_t)j; }
 
-// rows of the distances -reach .. reach
-__device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int tid, int nt) {
+// Rows of the distances -reach .. reach.  The edges go through shared memory (`tmp`, before anything else uses it): read at an index
+// that differs by lane from the kernel's parameters, 1600 distances took each block some 5 us.
+__device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int32_t* tmp, int tid, int nt) {
+  for (int x = tid; x < p.n_edges; x += nt) tmp[x] = p.edges[x];
+  __syncthreads();
   for (int x = tid; x <= 2 * p.reach; x += nt) {
     const int d = x - p.reach, n = d < 0 ? -d : d;
     int lo = 0, hi = p.n_edges;                  // edges not above n
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (p.edges[mid] <= n) lo = mid + 1; else hi = mid;
+      if (tmp[mid] <= n) lo = mid + 1; else hi = mid;
     }
     const int r = d > 0 ? p.base_pos + p.step_pos * lo : p.base_neg + p.step_neg * lo;
     lut[x] = (uint16_t)(r < 0 ? 0 : r >= p.rows ? p.rows - 1 : r);
   }
+  __syncthreads();
 }
 __device__ __forceinline__ int row_of(const RelP& p, const uint16_t* lut, int64_t d) {
   d = d < -p.reach ? -p.reach : d > p.reach ? p.reach : d;
@@ -65,11 +69,12 @@ __global__ void __launch_bounds__(kThreads) relpos_fwd_kernel(const __grid_const
   uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
   T* table = reinterpret_cast<T*>(smem + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [head of the group][row]
   const int h0 = blockIdx.z * heads, nh = h0 + heads <= p.H ? heads : p.H - h0;
+  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  fill_rows(p, lut, tmp, threadIdx.x, kThreads);
   for (int x = threadIdx.x; x < p.rows * nh; x += kThreads) {
     const int r = x / nh, h = x - r * nh;
     table[h * p.rows + r] = from_f<T>(load_rt(weight, (int64_t)r * p.H + h0 + h, p.w_dtype));
   }
-  fill_rows(p, lut, threadIdx.x, kThreads);
   __syncthreads();
   const int tpr = 1 << p.log_tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x >> p.log_tpr, slots = kThreads >> p.log_tpr;
   const int j0 = blockIdx.x * tpr * kC;
@@ -114,9 +119,10 @@ __global__ void __launch_bounds__(kThreads) relpos_fwd_kernel(const __grid_const
   }
 }
 
-// Backward: blockIdx = (column tile, rows, head).  Each thread sums into a column of its own of the block's table in shared memory
-// (no atomics: the sums' order is fixed), and only where the row changes: up to that it adds in a register, and away from
-// the diagonal whole sequences share a row.  The block's table goes to `parts` [gridDim.x * gridDim.y][H][rows].
+// Backward: blockIdx = (column tile, strip of rows, head).  A thread keeps a row of the table and a sum in registers for each of its
+// columns and walks down the rows of its strip: the distance of a column changes by one or so from row to row, so the table's
+// row seldom does.  Where it does, the sum goes to a column of the thread's own in the block's table in shared memory (no
+// atomics: the sums' order is fixed).  The block's table goes to `parts` [gridDim.x * gridDim.y][H][rows].
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
   using C = Cols<T, VEC>;
@@ -125,18 +131,42 @@ __global__ void __launch_bounds__(kThreads) relpos_bwd_kernel(const __grid_const
   const int nt = blockDim.x, tid = threadIdx.x;
   uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
   float* table = reinterpret_cast<float*>(smem + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [row][thread]
-  fill_rows(p, lut, tid, nt);
+  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  fill_rows(p, lut, tmp, tid, nt);
   for (int x = tid; x < p.rows * nt; x += nt) table[x] = 0.f;
+  float* mine = table + tid;                       // the only column that this thread touches before the last barrier
   __syncthreads();
-  float* mine = table + tid;
   const int tpr = 1 << p.log_tpr, lane = tid & (tpr - 1), slot = tid >> p.log_tpr, slots = nt >> p.log_tpr;
   const int j0 = blockIdx.x * tpr * kC, h = blockIdx.z;
-  const int64_t n_rows = (int64_t)p.B * p.Lq;
+  const int64_t n_rows = (int64_t)p.B * p.Lq, r_end = n_rows * (blockIdx.y + 1) / gridDim.y;
   int64_t kp[kC], ks[kC];
-  int kb = -1, cur = 0;
-  float acc = 0.f;
-  for (int64_t r = (int64_t)blockIdx.y * slots + slot; r < n_rows; r += (int64_t)gridDim.y * slots) {
+  int kb = -1, cur[kC];
+  float acc[kC];
+#pragma unroll
+  for (int e = 0; e < kC; ++e) { cur[e] = 0; acc[e] = 0.f; }
+  auto load = [&](int64_t r, T (&x)[kC]) {
+    const int64_t b = r / p.Lq, i = r - b * p.Lq;
+    const T* in = d_bias + ((b * p.H + h) * p.Lq + i) * p.Lk;
+    if constexpr (VEC) {
+      const int j = C::at(j0, lane, tpr, 0);
+      *reinterpret_cast<uint4*>(x) = r < r_end && j < p.Lk ? __ldcs(reinterpret_cast<const uint4*>(in + j)) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kC; ++e) {
+        const int j = C::at(j0, lane, tpr, e);
+        x[e] = r < r_end && j < p.Lk ? in[j] : from_f<T>(0.f);
+      }
+    }
+  };
+  int64_t r = n_rows * blockIdx.y / gridDim.y + slot;
+  __align__(16) T next[kC];
+  load(r, next);
+  for (; r < r_end; r += slots) {
     const int b = (int)(r / p.Lq), i = (int)(r - (int64_t)b * p.Lq);
+    float v[kC];
+#pragma unroll
+    for (int e = 0; e < kC; ++e) v[e] = to_f(next[e]);
+    load(r + slots, next);
     if (b != kb) {
       kb = b;
 #pragma unroll
@@ -146,53 +176,25 @@ __global__ void __launch_bounds__(kThreads) relpos_bwd_kernel(const __grid_const
         ks[e] = j < p.Lk && p.k_seg ? load_int(p.k_seg, b * p.ks_b + j, p.seg64) : 0;
       }
     }
-    const T* in = d_bias + (((int64_t)b * p.H + h) * p.Lq + i) * p.Lk;
-    float v[kC];
-    if constexpr (VEC) {
-      __align__(16) T x[kC];
-      const int j = C::at(j0, lane, tpr, 0);
-      *reinterpret_cast<uint4*>(x) = j < p.Lk ? __ldcs(reinterpret_cast<const uint4*>(in + j)) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int e = 0; e < kC; ++e) v[e] = to_f(x[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kC; ++e) {
-        const int j = C::at(j0, lane, tpr, e);
-        v[e] = j < p.Lk ? to_f(in[j]) : 0.f;
-      }
-    }
     const int64_t qp = q_position(p, b, i), qs = p.q_seg ? load_int(p.q_seg, b * p.qs_b + i, p.seg64) : 0;
-    int row[kC];
-    bool same = true;
 #pragma unroll
     for (int e = 0; e < kC; ++e) {
-      row[e] = row_of(p, lut, kp[e] - qp);
-      if (p.q_seg && ks[e] != qs) row[e] = p.rows - 1;
-      if (C::at(j0, lane, tpr, e) >= p.Lk) row[e] = e ? row[e - 1] : cur;      // a zero, wherever
-      same = same && row[e] == cur;
-    }
-    if (same) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < kC; ++e) s += v[e];
-      acc += s;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kC; ++e) {
-        if (row[e] != cur) { mine[cur * nt] += acc; cur = row[e]; acc = 0.f; }
-        acc += v[e];
-      }
+      int row = row_of(p, lut, kp[e] - qp);
+      if (p.q_seg && ks[e] != qs) row = p.rows - 1;
+      if (row != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row; acc[e] = 0.f; }
+      acc[e] += v[e];                              // zeros beyond Lk
     }
   }
-  mine[cur * nt] += acc;
+#pragma unroll
+  for (int e = 0; e < kC; ++e) mine[cur[e] * nt] += acc[e];
   __syncthreads();
   const int warp = tid >> 5, l = tid & 31;
   float* out = parts + ((int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * p.H + h) * p.rows;
-  for (int r = warp; r < p.rows; r += nt >> 5) {
+  for (int x = warp; x < p.rows; x += nt >> 5) {
     float s = 0.f;
-    for (int x = l; x < nt; x += 32) s += table[r * nt + x];
+    for (int y = l; y < nt; y += 32) s += table[x * nt + y];
     s = warp_sum(s);
-    if (l == 0) out[r] = s;
+    if (l == 0) out[x] = s;
   }
 }
 

@@ -544,12 +544,7 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   if ((r = opt_in_smem<dq>(QCfg<DP>::SMEM))) return r;
   dq<<<(unsigned)grid_q, kThreads, QCfg<DP>::SMEM, st>>>(mq, mg, mk64, mv64, f);
   MF_LAUNCHED("window_dq_tc_kernel");
-  if (f.plan.split_x) {
-    const int tiles = f.plan.nc_rest > 1 ? f.plan.n_tiles : f.plan.n_sink;
-    window_join_kernel<T, kKeys, kQB><<<dim3(tiles, p.Hk, p.B * p.N), 256, 0, st>>>(p, f.plan, f.parts);
-    MF_LAUNCHED("window_join_kernel");
-  }
-  return MF_OK;
+  return window_join<T, kKeys, kQB>(p, f.plan, f.parts, st);
 }
 template <typename T>
 int by_size(const mf_window_args& a, cudaStream_t st) {

@@ -123,25 +123,36 @@ __device__ __forceinline__ float* part_of(float* parts, const KeyPlan& c, const 
   return parts + (size_t)2 * KT * p.D * (head * c.split_x + x);
 }
 
-// adds the parts of the tiles that were split; blockIdx = (tile, key head, b * N + n)
+// Adds the parts of the tiles that were split, a thread an element: blockIdx = (piece of 256 elements, tile, head of all sequences).
+// (With a block a tile a long sequence's tile of sinks, 28 parts of it, took 163 us.)
 template <typename T, int KT, int QB>
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinP p, const KeyPlan c, const float* __restrict__ parts) {
-  const int tile = blockIdx.x, nc = tile < c.n_sink ? c.nc_sink : c.nc_rest;
+  const int tile = blockIdx.y, nc = tile < c.n_sink ? c.nc_sink : c.nc_rest;
   const int x0 = tile < c.n_sink ? tile * c.nc_sink : c.n_sink * c.nc_sink + (tile - c.n_sink) * c.nc_rest;
-  if (x0 >= c.split_x || nc == 1) return;
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (x0 >= c.split_x || nc == 1 || e >= 2 * KT * p.D) return;
+  const int which = e / (KT * p.D), r = e - which * KT * p.D, row = r / p.D, d = r - row * p.D, j = tile * KT + row;
+  if (j >= p.Lk) return;
   int used = (list_length<KT, QB>(p, tile) + c.chunk - 1) / c.chunk;
   if (used < 1) used = 1;
-  const int64_t bn = blockIdx.z, head = bn * p.Hk + blockIdx.y;
-  const float* src = part_of<KT>(const_cast<float*>(parts), c, p, head, x0);
+  const int64_t head = blockIdx.z, bn = head / p.Hk;
+  const float* src = part_of<KT>(const_cast<float*>(parts), c, p, head, x0) + e;
   const size_t step = (size_t)2 * KT * p.D;
-  for (int e = threadIdx.x; e < 2 * KT * p.D; e += 256) {
-    const int which = e / (KT * p.D), r = e - which * KT * p.D, row = r / p.D, d = r - row * p.D, j = tile * KT + row;
-    if (j >= p.Lk) continue;
-    float s = 0.f;
-    for (int k = 0; k < used; ++k) s += src[k * step + e];
-    if (which == 0) s *= p.scale;
-    static_cast<T*>(which ? p.dv : p.dk)[((bn * p.Lk + j) * p.Hk + blockIdx.y) * p.D + d] = from_f<T>(s);
-  }
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < used; ++k) s += src[k * step];
+  if (which == 0) s *= p.scale;
+  static_cast<T*>(which ? p.dv : p.dk)[((bn * p.Lk + j) * p.Hk + (head - bn * p.Hk)) * p.D + d] = from_f<T>(s);
+}
+template <typename T, int KT, int QB>
+int window_join(const WinP& p, const KeyPlan& c, const float* parts, cudaStream_t st) {
+  if (!c.split_x) return MF_OK;
+  const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink;
+  const int64_t heads = (int64_t)p.B * p.N * p.Hk;
+  MF_REQUIRE(tiles <= 65535 && heads <= 65535, MF_ERR_UNSUPPORTED, "%d tiles of %lld heads in parts are more than one launch takes", tiles, (long long)heads);
+  window_join_kernel<T, KT, QB><<<dim3((2 * KT * p.D + 255) / 256, tiles, (unsigned)heads), 256, 0, st>>>(p, c, parts);
+  MF_LAUNCHED("window_join_kernel");
+  return MF_OK;
 }
 
 // ---- few queries ------------------------------------------------------------------------------------------------------
@@ -159,7 +170,7 @@ template <int ROWS, int KT>
 int split_count(const WinP& p, int blocks_wanted) {
   const int q = queries_of<ROWS>(p);
   const int64_t tiles = (p.Lq + q - 1) / q, blocks = tiles * p.B * p.N * head_groups(p);
-  if (2 * blocks > blocks_wanted) return 1;
+  if (4 * blocks > blocks_wanted) return 1;                // joining costs some 5 us
   int most = 0;                                            // key tiles of a tile of queries; few of them, or blocks would be many
   for (int64_t t = 0; t < tiles; ++t) {
     const int i0 = (int)t * q, n = key_tiles<KT>(p, i0, i0 + q < p.Lq ? i0 + q : p.Lq).count();

@@ -335,25 +335,33 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const T* __restrict__
   }
 }
 
-// a warp a row: the parts weighed by exp(their log-sum-exp)
+// A warp a row: the parts weighed by exp(their log-sum-exp).  Lane s holds the weights of parts s and s + 32.
 template <typename T>
 __global__ void __launch_bounds__(256) window_split_join_kernel(const __grid_constant__ WinP p, const Split sp) {
   const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (r >= sp.rows) return;
-  float m = -INFINITY;
-  for (int s = 0; s < sp.splits; ++s) { const float x = sp.lse(s, r, p.D); m = x > m || x != x ? x : m; }      // NaN stays
-  float sum = 0.f;
-  const float m_ref = m == -INFINITY ? 0.f : m;
-  for (int s = 0; s < sp.splits; ++s) sum += expf(sp.lse(s, r, p.D) - m_ref);
+  float w[2], m = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    w[k] = lane + 32 * k < sp.splits ? sp.lse(lane + 32 * k, r, p.D) : -INFINITY;
+    m = fmaxf(m, w[k]);                                    // a NaN stays in w
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) { w[k] = expf(w[k] - (m == -INFINITY ? 0.f : m)); sum += w[k]; }
+  sum = warp_sum(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = lane; d < p.D; d += 32) {
+  for (int d0 = 0; d0 < p.D; d0 += 32) {
+    const int d = d0 + lane;
     float o = 0.f;
+#pragma unroll 4
     for (int s = 0; s < sp.splits; ++s) {
-      const float w = expf(sp.lse(s, r, p.D) - m_ref);
-      if (w != 0.f) o = fmaf(w, sp.row(s, r, p.D)[d], o);
+      const float ws = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+      if (ws != 0.f && d < p.D) o = fmaf(ws, sp.row(s, r, p.D)[d], o);
     }
-    static_cast<T*>(p.o)[r * p.D + d] = from_f<T>(o * inv);
+    if (d < p.D) static_cast<T*>(p.o)[r * p.D + d] = from_f<T>(o * inv);
   }
   if (lane == 0 && p.lse) {
     const int h = (int)(r % p.H);
@@ -396,11 +404,7 @@ int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
     return MF_OK;
   };
   int r = p.D <= 32 ? go(std::integral_constant<int, 32>{}) : p.D <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
-  if (r || !c.split_x) return r;
-  const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink;
-  window_join_kernel<T, kTile, kTile><<<dim3(tiles, p.Hk, p.B * p.N), 256, 0, st>>>(p, c, parts);
-  MF_LAUNCHED("window_join_kernel");
-  return MF_OK;
+  return r ? r : window_join<T, kTile, kTile>(p, c, parts, st);
 }
 
 bool rows_vec(const void* ptr, const int64_t* s, int D, size_t es) {
