@@ -351,7 +351,8 @@ int check_relpos(const mf_relpos_args& a) {
   MF_REQUIRE(!a.q_pos == !a.k_pos && !a.q_seg == !a.k_seg, MF_ERR_BAD_ARG, "positions and segments are given for queries and keys, or for neither");
   MF_REQUIRE(!a.q_pos || a.pos_bytes == 4 || a.pos_bytes == 8, MF_ERR_BAD_ARG, "positions are 4 or 8 bytes wide");
   MF_REQUIRE(!a.q_seg || a.seg_bytes == 4 || a.seg_bytes == 8, MF_ERR_BAD_ARG, "segments are 4 or 8 bytes wide");
-  MF_REQUIRE(a.H <= 65535, MF_ERR_UNSUPPORTED, "H=%d exceeds 65535", a.H);
+  MF_REQUIRE(a.H <= 65535 && a.B <= 65535, MF_ERR_UNSUPPORTED, "B=%d or H=%d exceeds 65535", a.B, a.H);
+  MF_REQUIRE(a.Lq < 1 << 30 && a.Lk < 1 << 30, MF_ERR_UNSUPPORTED, "lengths of 2^30 and more are not supported");
   return MF_OK;
 }
 int check_qk_rotary(const mf_qk_rotary_args& a) {
@@ -363,6 +364,7 @@ int check_qk_rotary(const mf_qk_rotary_args& a) {
   MF_REQUIRE(!a.q_weight == !a.k_weight, MF_ERR_BAD_ARG, "queries and keys both have a weight, or neither has");
   MF_REQUIRE(!a.positions || a.pos_bytes == 4 || a.pos_bytes == 8, MF_ERR_BAD_ARG, "positions are 4 or 8 bytes wide");
   MF_REQUIRE((int64_t)a.H + a.Hk <= 65535, MF_ERR_UNSUPPORTED, "more than 65535 heads");
+  MF_REQUIRE((int64_t)a.B * a.N <= 0x7fffffff && (int64_t)a.B * a.N * a.L <= 0x7fffffff, MF_ERR_UNSUPPORTED, "more than 2^31 tokens");
   return MF_OK;
 }
 int check_window(const mf_window_args& a) {

@@ -58,24 +58,30 @@ struct Unit {
     else { a = R + 2 * V * (u - nr); b = a + V; has_a = a < D; has_b = b < D; }
   }
 };
+// the two pieces of a unit as they are in memory
+template <typename T, int V> struct Raw { Piece<T, V> p, q; };
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void load_unit(const T* row, int64_t sd, const Unit<V, IL>& u, Raw<T, V>& r) {
+  if constexpr (V == 1) {
+    r.p.v[0] = u.has_a ? row[u.a * sd] : from_f<T>(0.f);
+    r.q.v[0] = u.has_b ? row[u.b * sd] : from_f<T>(0.f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.p.v[e] = r.q.v[e] = from_f<T>(0.f);
+    if (u.has_a) r.p = *reinterpret_cast<const Piece<T, V>*>(row + u.a);
+    if (u.has_b) r.q = *reinterpret_cast<const Piece<T, V>*>(row + u.b);
+  }
+}
 // x[0..V) and x[V..2V) hold the first and second elements of the V pairs (or the two pieces of an unturned unit)
 template <typename T, int V, bool IL>
-__device__ __forceinline__ void load_unit(const T* row, int64_t sd, const Unit<V, IL>& u, float (&x)[2 * V]) {
-  Piece<T, V> p, q;
-  if constexpr (V == 1) {
-    p.v[0] = u.has_a ? row[u.a * sd] : from_f<T>(0.f);
-    q.v[0] = u.has_b ? row[u.b * sd] : from_f<T>(0.f);
-  } else {
-    if (u.has_a) p = *reinterpret_cast<const Piece<T, V>*>(row + u.a); else for (int e = 0; e < V; ++e) p.v[e] = from_f<T>(0.f);
-    if (u.has_b) q = *reinterpret_cast<const Piece<T, V>*>(row + u.b); else for (int e = 0; e < V; ++e) q.v[e] = from_f<T>(0.f);
-  }
+__device__ __forceinline__ void unpack_unit(const Raw<T, V>& r, float (&x)[2 * V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     if constexpr (IL && V > 1) {
-      x[e] = to_f(2 * e < V ? p.v[2 * e] : q.v[2 * e - V]);
-      x[V + e] = to_f(2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]);
+      x[e] = to_f(2 * e < V ? r.p.v[2 * e] : r.q.v[2 * e - V]);
+      x[V + e] = to_f(2 * e + 1 < V ? r.p.v[2 * e + 1] : r.q.v[2 * e + 1 - V]);
     } else {
-      x[e] = to_f(p.v[e]); x[V + e] = to_f(q.v[e]);
+      x[e] = to_f(r.p.v[e]); x[V + e] = to_f(r.q.v[e]);
     }
   }
 }
@@ -125,7 +131,7 @@ __device__ __forceinline__ float row_sum(float v, int lpr) {
 // The weights of the block's heads wait in shared memory as fp32: read from global memory for each row, converted from a type known
 // at run time, they were most of the instructions (4 + 4 heads of 32, 147456 tokens: 96 us forward, 220 backward).
 template <typename T, int V, int UPL, bool IL, bool BWD>
-__global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_constant__ RotP p) {
+__global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary_kernel(const __grid_constant__ RotP p) {
   const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr, slots = kThreads >> p.log_lpr;
   const int heads = p.H + p.Hk, g0 = blockIdx.y * p.heads_per, g1 = g0 + p.heads_per < heads ? g0 + p.heads_per : heads;
   const float inv_d = 1.f / p.D;
@@ -143,11 +149,11 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
   }
   __syncthreads();
   float dwq[BWD ? UPL : 1][2 * V] = {}, dwk[BWD ? UPL : 1][2 * V] = {};
-  const int64_t stride = (int64_t)gridDim.x * slots, rounds = (p.tokens + stride - 1) / stride;
-  for (int64_t it = 0; it < rounds; ++it) {
-    const int64_t tok = it * stride + (int64_t)blockIdx.x * slots + slot;
+  const int64_t stride = (int64_t)gridDim.x * slots;
+  for (int64_t t0 = (int64_t)blockIdx.x * slots; t0 < p.tokens; t0 += stride) {
+    const int64_t tok = t0 + slot;
     const bool live = tok < p.tokens;
-    const int64_t bn = live ? tok / p.L : 0, l = live ? tok - bn * p.L : 0, b = bn / p.N, n = bn - b * p.N;
+    const uint32_t bn = live ? (uint32_t)tok / (uint32_t)p.L : 0, l = live ? (uint32_t)tok - bn * p.L : 0, b = bn / (uint32_t)p.N, n = bn - b * p.N;
     const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1] + l * p.qs[2];
     const T* kk = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1] + l * p.ks[2];
     auto unit = [&](int k) {
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
       u.has_a = u.has_a && live; u.has_b = u.has_b && live;
       return u;
     };
-    auto fetch = [&](int g, float (&x)[UPL][2 * V], float (&d)[BWD ? UPL : 1][2 * V]) {
+    auto fetch = [&](int g, Raw<T, V> (&x)[UPL], Raw<T, V> (&d)[BWD ? UPL : 1]) {
       const bool is_q = g < p.H;
       const int h = is_q ? g : g - p.H;
       const T* row = is_q ? q + h * p.qs[3] : kk + h * p.ks[3];
@@ -167,8 +173,8 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
         for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(dr, 1, unit(k), d[k]);
       }
     };
-    float x[UPL][2 * V], d[BWD ? UPL : 1][2 * V];
-    fetch(g0, x, d);                                           // on its way while the angles are formed
+    Raw<T, V> xr[UPL], dr[BWD ? UPL : 1];
+    fetch(g0, xr, dr);                                         // on its way while the angles are formed
     double pos = (double)l;
     if (p.pos) {
       const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
@@ -190,14 +196,16 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
       const int h = is_q ? g : g - p.H;
       const int64_t out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
       const float* w = ws + (!p.qw ? 0 : !p.w_head ? (is_q ? 0 : p.D) : (g - g0) * p.D);
-      float ss = 0.f;
+      float x[UPL][2 * V], d[BWD ? UPL : 1][2 * V], ss = 0.f;
 #pragma unroll
-      for (int k = 0; k < UPL; ++k)
+      for (int k = 0; k < UPL; ++k) {
+        unpack_unit<T, V, IL>(xr[k], x[k]);
+        if constexpr (BWD) unpack_unit<T, V, IL>(dr[k], d[k]);
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) ss = fmaf(x[k][e], x[k][e], ss);
+      }
+      if (g + 1 < g1) fetch(g + 1, xr, dr);
       const float rstd = rsqrtf(fmaf(row_sum(ss, lpr), inv_d, p.eps));
-      float xn[UPL][2 * V], dn[BWD ? UPL : 1][2 * V];
-      if (g + 1 < g1) fetch(g + 1, xn, dn);
       if constexpr (!BWD) {
         T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + out_at;
 #pragma unroll
@@ -242,15 +250,6 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_kernel(const __grid_consta
           for (int e = 0; e < 2 * V; ++e) x[k][e] = rstd * fmaf(-x[k][e], dot, d[k][e]);
           store_unit<T, V, IL>(out, unit(k), x[k]);
         }
-      }
-      if (g + 1 < g1) {
-#pragma unroll
-        for (int k = 0; k < UPL; ++k)
-#pragma unroll
-          for (int e = 0; e < 2 * V; ++e) {
-            x[k][e] = xn[k][e];
-            if constexpr (BWD) d[k][e] = dn[k][e];
-          }
       }
     }
   }
@@ -314,10 +313,13 @@ RotP rot_params(const mf_qk_rotary_args& a) {
   return p;
 }
 
-// elements of a piece: the widest load that sizes, strides and addresses allow
+// Elements of a piece: the widest load that sizes, strides and addresses allow, 16 bytes on the forward and 8 on the backward, where a
+// thread holds twice as much and the sums of the weights' gradients besides (with 16 bytes 176 registers, one block of
+// 256 threads on an SM).
+int piece_limit(int dtype, bool bwd) { return (bwd ? 8 : 16) / (int)dtype_size(dtype); }
 int piece(const mf_qk_rotary_args& a, bool bwd) {
   const int es = (int)dtype_size(a.dtype);
-  for (int v = 16 / es; v > 1; v /= 2) {
+  for (int v = piece_limit(a.dtype, bwd); v > 1; v /= 2) {
     bool ok = a.R / 2 % v == 0 && (a.D - a.R) % v == 0 && a.q_strides[4] == 1 && a.k_strides[4] == 1;
     for (int i = 0; i < 4; ++i) ok = ok && a.q_strides[i] % v == 0 && a.k_strides[i] % v == 0;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (bwd ? (uintptr_t)a.dq_out | (uintptr_t)a.dk_out | (uintptr_t)a.dq | (uintptr_t)a.dk
@@ -381,12 +383,11 @@ int run(const mf_qk_rotary_args& a, cudaStream_t st) {
 }
 template <typename T, bool BWD>
 int dispatch(const mf_qk_rotary_args& a, cudaStream_t st) {
-  switch (piece(a, BWD)) {
-    case 8: if constexpr (sizeof(T) == 2) return run<T, 8, BWD>(a, st);
-    case 4: return run<T, 4, BWD>(a, st);
-    case 2: return run<T, 2, BWD>(a, st);
-    default: return run<T, 1, BWD>(a, st);
-  }
+  constexpr int kMost = (BWD ? 8 : 16) / (int)sizeof(T);
+  const int v = piece(a, BWD);
+  if constexpr (kMost >= 8) if (v == 8) return run<T, 8, BWD>(a, st);
+  if constexpr (kMost >= 4) if (v == 4) return run<T, 4, BWD>(a, st);
+  return v == 2 ? run<T, 2, BWD>(a, st) : run<T, 1, BWD>(a, st);
 }
 }  // namespace
 
@@ -398,7 +399,7 @@ int qk_rotary_fwd(const mf_qk_rotary_args& a, cudaStream_t st) {
 size_t qk_rotary_bwd_workspace(const mf_qk_rotary_args& a) {
   if (!a.dq_weight) return 0;
   size_t most = 0;
-  for (int v = 1; v <= 16 / (int)dtype_size(a.dtype); v *= 2) {       // whichever width the alignment allows
+  for (int v = 1; v <= piece_limit(a.dtype, true); v *= 2) {       // whichever width the alignment allows
     if (a.R / 2 % v || (a.D - a.R) % v) break;
     const Plan c = plan(a, v, true);
     const size_t n = sizeof(float) * 2 * a.D * (size_t)c.gx * c.gy;

@@ -22,6 +22,7 @@ struct RelP {
   int64_t qp_b, kp_b, qs_b, ks_b;
   bool pos64, seg64;
   int log_tpr;                       // threads of a block that share a row of the bias
+  int strips;                        // blocks along the queries of a batch element
   int edges[MF_RELPOS_MAX_EDGES];
 };
 
@@ -31,8 +32,19 @@ __device__ __forceinline__ int64_t load_int(const void* p, int64_t i, bool wide)
 __device__ __forceinline__ int64_t q_position(const RelP& p, int b, int i) { return p.q_pos ? load_int(p.q_pos, b * p.qp_b + i, p.pos64) : (int64_t)i + (p.Lk - p.Lq); }
 __device__ __forceinline__ int64_t k_position(const RelP& p, int b, int j) { return p.k_pos ? load_int(p.k_pos, b * p.kp_b + j, p.pos64) : (int64_t)j; }
 
-// Rows of the distances -reach .. reach.  The edges go through shared memory (`tmp`, before anything else uses it): read at an index
-// that differs by lane from the kernel's parameters, 1600 distances took each block some 5 us.
+// Positions (and segments) in 32 bits, as differences from the first key's where all that a block sees lie within 2^30 of that; a block that
+// finds others reads them again where it needs them.
+constexpr int kFar = 1 << 30;
+struct Origin { int64_t pos, seg; };
+__device__ __forceinline__ Origin origin(const RelP& p, int b) { return Origin{k_position(p, b, 0), p.k_seg ? load_int(p.k_seg, b * p.ks_b, p.seg64) : 0}; }
+__device__ __forceinline__ int near_to(int64_t x, int64_t from, bool& near) {
+  const int64_t d = x - from;
+  near = near && d > -kFar && d < kFar;
+  return (int)d;
+}
+
+// Rows of the distances -reach .. reach.  The edges go through shared memory (`tmp`): read at an index that differs by lane from the
+// kernel's parameters, 1600 distances took each block some 5 us.
 __device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int32_t* tmp, int tid, int nt) {
   for (int x = tid; x < p.n_edges; x += nt) tmp[x] = p.edges[x];
   __syncthreads();
@@ -46,144 +58,155 @@ __device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int32_t*
     const int r = d > 0 ? p.base_pos + p.step_pos * lo : p.base_neg + p.step_neg * lo;
     lut[x] = (uint16_t)(r < 0 ? 0 : r >= p.rows ? p.rows - 1 : r);
   }
-  __syncthreads();
 }
-__device__ __forceinline__ int row_of(const RelP& p, const uint16_t* lut, int64_t d) {
-  d = d < -p.reach ? -p.reach : d > p.reach ? p.reach : d;
-  return lut[(int)d + p.reach];
+__device__ __forceinline__ int row_of(const RelP& p, const uint16_t* lut, int d) { return lut[(d < -p.reach ? -p.reach : d > p.reach ? p.reach : d) + p.reach]; }
+__device__ __forceinline__ int row_of_far(const RelP& p, const uint16_t* lut, int b, int i, int j) {
+  if (p.q_seg && load_int(p.q_seg, b * p.qs_b + i, p.seg64) != load_int(p.k_seg, b * p.ks_b + j, p.seg64)) return p.rows - 1;
+  const int64_t d = k_position(p, b, j) - q_position(p, b, i);
+  return row_of(p, lut, d < -p.reach ? -p.reach : d > p.reach ? p.reach : (int)d);
 }
 
-// A thread's eight columns of a tile of rows: C adjacent ones where rows are 16-byte aligned (16 bytes a store), else one every
-// tpr columns (a warp then covers adjacent elements).  Columns at and beyond Lk are left out.
+// Forward: blockIdx = (column tile, batch element and strip of queries, group of heads).  A thread's columns: 16 bytes of adjacent ones where
+// rows are 16-byte aligned, else eight, 32 apart, of its warp's 256 (a store of the warp then writes adjacent elements).
 template <typename T, bool VEC> struct Cols {
-  static constexpr int kC = VEC ? 16 / (int)sizeof(T) : 8;
-  static __device__ __forceinline__ int at(int j0, int lane, int tpr, int e) { return VEC ? j0 + lane * kC + e : j0 + e * tpr + lane; }
+  static constexpr int kC = VEC ? 16 / (int)sizeof(T) : 8, kStep = VEC ? 1 : 32;
+  static __device__ __forceinline__ int first(int j0, int lane) { return VEC ? j0 + lane * kC : j0 + (lane & ~31) * 8 + (lane & 31); }
 };
-
-// Forward: blockIdx = (column tile, rows, group of heads).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) relpos_fwd_kernel(const __grid_constant__ RelP p, const void* __restrict__ weight, T* __restrict__ bias, int heads) {
+__global__ void __launch_bounds__(kThreads, 4) relpos_fwd_kernel(const __grid_constant__ RelP p, const void* __restrict__ weight, T* __restrict__ bias, int heads) {
   using C = Cols<T, VEC>;
   constexpr int kC = C::kC;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
   uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
   T* table = reinterpret_cast<T*>(smem + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [head of the group][row]
+  const int tpr = 1 << p.log_tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x >> p.log_tpr, slots = kThreads >> p.log_tpr;
+  const int j = C::first(blockIdx.x * tpr * kC, lane), b = blockIdx.y / p.strips, strip = blockIdx.y - b * p.strips;
   const int h0 = blockIdx.z * heads, nh = h0 + heads <= p.H ? heads : p.H - h0;
-  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  const Origin o = origin(p, b);
+  int kp[kC], ks[kC];
+  bool near = true;
+#pragma unroll
+  for (int e = 0; e < kC; ++e) {
+    const int je = j + e * C::kStep;
+    kp[e] = je < p.Lk ? near_to(k_position(p, b, je), o.pos, near) : 0;
+    ks[e] = je < p.Lk && p.k_seg ? near_to(load_int(p.k_seg, b * p.ks_b + je, p.seg64), o.seg, near) : 0;
+  }
   fill_rows(p, lut, tmp, threadIdx.x, kThreads);
   for (int x = threadIdx.x; x < p.rows * nh; x += kThreads) {
     const int r = x / nh, h = x - r * nh;
     table[h * p.rows + r] = from_f<T>(load_rt(weight, (int64_t)r * p.H + h0 + h, p.w_dtype));
   }
   __syncthreads();
-  const int tpr = 1 << p.log_tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x >> p.log_tpr, slots = kThreads >> p.log_tpr;
-  const int j0 = blockIdx.x * tpr * kC;
-  const int64_t n_rows = (int64_t)p.B * p.Lq;
-  int64_t kp[kC], ks[kC];
-  int kb = -1;
-  for (int64_t r = (int64_t)blockIdx.y * slots + slot; r < n_rows; r += (int64_t)gridDim.y * slots) {
-    const int b = (int)(r / p.Lq), i = (int)(r - (int64_t)b * p.Lq);
-    if (b != kb) {
-      kb = b;
+  const int end = (int)((int64_t)p.Lq * (strip + 1) / p.strips);
+  for (int i = (int)((int64_t)p.Lq * strip / p.strips) + slot; i < end; i += slots) {
+    bool close = near;
+    const int qp = near_to(q_position(p, b, i), o.pos, close), qs = p.q_seg ? near_to(load_int(p.q_seg, b * p.qs_b + i, p.seg64), o.seg, close) : 0;
+    int row[kC];
+    if (close) {
 #pragma unroll
       for (int e = 0; e < kC; ++e) {
-        const int j = C::at(j0, lane, tpr, e);
-        kp[e] = j < p.Lk ? k_position(p, b, j) : 0;
-        ks[e] = j < p.Lk && p.k_seg ? load_int(p.k_seg, b * p.ks_b + j, p.seg64) : 0;
+        row[e] = row_of(p, lut, kp[e] - qp);
+        if (ks[e] != qs) row[e] = p.rows - 1;              // without segments both are 0
       }
-    }
-    const int64_t qp = q_position(p, b, i), qs = p.q_seg ? load_int(p.q_seg, b * p.qs_b + i, p.seg64) : 0;
-    int row[kC];
+    } else {
 #pragma unroll
-    for (int e = 0; e < kC; ++e) {
-      row[e] = row_of(p, lut, kp[e] - qp);
-      if (p.q_seg && ks[e] != qs) row[e] = p.rows - 1;
+      for (int e = 0; e < kC; ++e) row[e] = j + e * C::kStep < p.Lk ? row_of_far(p, lut, b, i, j + e * C::kStep) : 0;
     }
-    T* out = bias + (((int64_t)b * p.H + h0) * p.Lq + i) * p.Lk;
+    T* out = bias + (((int64_t)b * p.H + h0) * p.Lq + i) * p.Lk + j;
     const T* t = table;
+    const int left = p.Lk - j;
     for (int h = 0; h < nh; ++h, out += (int64_t)p.Lq * p.Lk, t += p.rows) {
       if constexpr (VEC) {
         __align__(16) T v[kC];
 #pragma unroll
         for (int e = 0; e < kC; ++e) v[e] = t[row[e]];
-        const int j = C::at(j0, lane, tpr, 0);
-        if (j < p.Lk) __stcs(reinterpret_cast<uint4*>(out + j), *reinterpret_cast<const uint4*>(v));
+        if (left > 0) __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(v));
       } else {
 #pragma unroll
-        for (int e = 0; e < kC; ++e) {
-          const int j = C::at(j0, lane, tpr, e);
-          if (j < p.Lk) out[j] = t[row[e]];
-        }
+        for (int e = 0; e < kC; ++e)
+          if (e * C::kStep < left) out[e * C::kStep] = t[row[e]];
       }
     }
   }
 }
 
-// Backward: blockIdx = (column tile, strip of rows, head).  A thread keeps a row of the table and a sum in registers for each of its
-// columns and walks down the rows of its strip: the distance of a column changes by one or so from row to row, so the table's
-// row seldom does.  Where it does, the sum goes to a column of the thread's own in the block's table in shared memory (no
-// atomics: the sums' order is fixed).  The block's table goes to `parts` [gridDim.x * gridDim.y][H][rows].
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
-  using C = Cols<T, VEC>;
-  constexpr int kC = C::kC;
+// Backward: blockIdx = (column tile, batch element and strip of queries, head).  A thread walks down diagonals: from one query to the next its
+// columns move by one too (around the tile's end to its start), so that the distance, and with it the table's row, stays the same
+// where positions run on.  It sums in registers and adds a sum to a column of its own of the block's table in shared memory when the row
+// changes (no atomics: the sums' order is fixed); walking down columns instead, a warp met such a change in most of its
+// steps and [2, 8, 1531, 1531] took 173 us.  The block's table goes to `parts` [gridDim.y * gridDim.x][H][rows].
+constexpr int kBwdCols = 8;
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 3) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
+  constexpr int kC = kBwdCols;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int nt = blockDim.x, tid = threadIdx.x;
-  uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
-  float* table = reinterpret_cast<float*>(smem + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [row][thread]
   __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  const int nt = blockDim.x, tid = threadIdx.x;
+  const int tpr = 1 << p.log_tpr, lane = tid & (tpr - 1), slot = tid >> p.log_tpr, slots = nt >> p.log_tpr, width_max = tpr * kC;
+  int32_t* kpos = reinterpret_cast<int32_t*>(smem);                                            // positions of the tile's keys
+  int32_t* kseg = kpos + width_max;
+  uint16_t* lut = reinterpret_cast<uint16_t*>(kseg + (p.k_seg ? width_max : 0));
+  float* table = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(lut) + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [row][thread]
+  const int j0 = blockIdx.x * width_max, h = blockIdx.z, b = blockIdx.y / p.strips, strip = blockIdx.y - b * p.strips;
+  const int width = p.Lk - j0 < width_max ? p.Lk - j0 : width_max;
+  const Origin o = origin(p, b);
+  bool near = true;
+  for (int x = tid; x < width; x += nt) {
+    kpos[x] = near_to(k_position(p, b, j0 + x), o.pos, near);
+    if (p.k_seg) kseg[x] = near_to(load_int(p.k_seg, b * p.ks_b + j0 + x, p.seg64), o.seg, near);
+  }
   fill_rows(p, lut, tmp, tid, nt);
   for (int x = tid; x < p.rows * nt; x += nt) table[x] = 0.f;
+  near = __syncthreads_and(near);
   float* mine = table + tid;                       // the only column that this thread touches before the last barrier
-  __syncthreads();
-  const int tpr = 1 << p.log_tpr, lane = tid & (tpr - 1), slot = tid >> p.log_tpr, slots = nt >> p.log_tpr;
-  const int j0 = blockIdx.x * tpr * kC, h = blockIdx.z;
-  const int64_t n_rows = (int64_t)p.B * p.Lq, r_end = n_rows * (blockIdx.y + 1) / gridDim.y;
-  int64_t kp[kC], ks[kC];
-  int kb = -1, cur[kC];
+  const int i0 = (int)((int64_t)p.Lq * strip / p.strips), end = (int)((int64_t)p.Lq * (strip + 1) / p.strips);
+  const T* in = d_bias + (((int64_t)b * p.H + h) * p.Lq) * p.Lk + j0;
+  // column e of this thread at query i is lane + e * tpr + (i - i0), around the width
+  const int columns = (width - lane + tpr - 1) >> p.log_tpr;       // of the tile's width; at most kC
+  int cur[kC];
   float acc[kC];
 #pragma unroll
   for (int e = 0; e < kC; ++e) { cur[e] = 0; acc[e] = 0.f; }
-  auto load = [&](int64_t r, T (&x)[kC]) {
-    const int64_t b = r / p.Lq, i = r - b * p.Lq;
-    const T* in = d_bias + ((b * p.H + h) * p.Lq + i) * p.Lk;
-    if constexpr (VEC) {
-      const int j = C::at(j0, lane, tpr, 0);
-      *reinterpret_cast<uint4*>(x) = r < r_end && j < p.Lk ? __ldcs(reinterpret_cast<const uint4*>(in + j)) : make_uint4(0u, 0u, 0u, 0u);
-    } else {
+  const int step = slots % width;
+  auto wrap = [&](int c) { return c >= width ? c - width : c; };
+  struct Cursor { int i, first; const T* row; };                   // of the loads, and of the sums two rows behind
+  auto start = [&]() { return Cursor{i0 + slot, (lane + slot) % width, in + (int64_t)(i0 + slot) * p.Lk}; };
+  auto next = [&](Cursor& c) { c.i += slots; c.first = wrap(c.first + step); c.row += (int64_t)slots * p.Lk; };
+  auto load = [&](Cursor& c, T (&x)[kC]) {
 #pragma unroll
-      for (int e = 0; e < kC; ++e) {
-        const int j = C::at(j0, lane, tpr, e);
-        x[e] = r < r_end && j < p.Lk ? in[j] : from_f<T>(0.f);
-      }
-    }
+    for (int e = 0; e < kC; ++e) x[e] = c.i < end && e < columns ? c.row[wrap(c.first + e * tpr)] : from_f<T>(0.f);
+    next(c);
   };
-  int64_t r = n_rows * blockIdx.y / gridDim.y + slot;
-  __align__(16) T next[kC];
-  load(r, next);
-  for (; r < r_end; r += slots) {
-    const int b = (int)(r / p.Lq), i = (int)(r - (int64_t)b * p.Lq);
-    float v[kC];
-#pragma unroll
-    for (int e = 0; e < kC; ++e) v[e] = to_f(next[e]);
-    load(r + slots, next);
-    if (b != kb) {
-      kb = b;
-#pragma unroll
-      for (int e = 0; e < kC; ++e) {
-        const int j = C::at(j0, lane, tpr, e);
-        kp[e] = j < p.Lk ? k_position(p, b, j) : 0;
-        ks[e] = j < p.Lk && p.k_seg ? load_int(p.k_seg, b * p.ks_b + j, p.seg64) : 0;
-      }
-    }
-    const int64_t qp = q_position(p, b, i), qs = p.q_seg ? load_int(p.q_seg, b * p.qs_b + i, p.seg64) : 0;
+  auto add = [&](Cursor& c, const T (&x)[kC]) {
+    bool close = near;
+    const int qp = near_to(q_position(p, b, c.i), o.pos, close), qs = p.q_seg ? near_to(load_int(p.q_seg, b * p.qs_b + c.i, p.seg64), o.seg, close) : 0;
 #pragma unroll
     for (int e = 0; e < kC; ++e) {
-      int row = row_of(p, lut, kp[e] - qp);
-      if (p.q_seg && ks[e] != qs) row = p.rows - 1;
+      if (e >= columns) break;
+      const int at = wrap(c.first + e * tpr);
+      int row;
+      if (close) {
+        row = row_of(p, lut, kpos[at] - qp);
+        if (p.q_seg && kseg[at] != qs) row = p.rows - 1;
+      } else {
+        row = row_of_far(p, lut, b, c.i, j0 + at);
+      }
       if (row != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row; acc[e] = 0.f; }
-      acc[e] += v[e];                              // zeros beyond Lk
+      acc[e] += to_f(x[e]);
     }
+    next(c);
+  };
+  Cursor in_at = start(), sum_at = start();
+  T x0[kC], x1[kC];                                // two rows under way
+  load(in_at, x0);
+  load(in_at, x1);
+  while (sum_at.i < end) {
+    T y[kC];
+#pragma unroll
+    for (int e = 0; e < kC; ++e) { y[e] = x0[e]; x0[e] = x1[e]; }
+    load(in_at, x1);
+    add(sum_at, y);
   }
 #pragma unroll
   for (int e = 0; e < kC; ++e) mine[cur[e] * nt] += acc[e];
@@ -223,28 +246,31 @@ RelP relpos_params(const mf_relpos_args& a) {
   return p;
 }
 size_t lut_bytes(const RelP& p) { return (2 * (2 * (size_t)p.reach + 1) + 15) & ~(size_t)15; }
-int log_threads(int Lk, int cols, int threads) {
-  int l = 0;
+int log_threads(int Lk, int cols, int least, int threads) {
+  int l = least;
   while ((1 << l) < threads && (1 << l) * cols < Lk) ++l;
   return l;
 }
 
-struct BwdPlan { int threads, tiles, strips; size_t smem; };
-BwdPlan bwd_plan(RelP& p, int cols) {
+struct BwdPlan { int threads, tiles, parts; size_t smem; };
+BwdPlan bwd_plan(RelP& p) {
   BwdPlan b;
   b.threads = kThreads;
   while (b.threads > 32 && (size_t)p.rows * b.threads * 4 > 72 * 1024) b.threads /= 2;
-  b.smem = lut_bytes(p) + (size_t)p.rows * b.threads * 4;
-  p.log_tpr = log_threads(p.Lk, cols, b.threads);
+  p.log_tpr = log_threads(p.Lk, kBwdCols, 5, b.threads);
   const int tpr = 1 << p.log_tpr, slots = b.threads >> p.log_tpr;
-  b.tiles = (p.Lk + tpr * cols - 1) / (tpr * cols);
-  // as many blocks as fit the processors, each with a few rows at least: a block's table costs about as much as four rows of it
-  const int fit = (int)(220 * 1024 / (b.smem + 1024));
-  const int64_t want = (int64_t)tcx::sm_count() * (fit < 1 ? 1 : fit > 2048 / b.threads ? 2048 / b.threads : fit);
-  int64_t strips = (want + (int64_t)p.H * b.tiles - 1) / ((int64_t)p.H * b.tiles);
-  const int64_t most = ((int64_t)p.B * p.Lq + 4 * slots - 1) / (4 * slots);
+  b.smem = lut_bytes(p) + (size_t)p.rows * b.threads * 4 + (size_t)tpr * kBwdCols * (p.k_seg ? 8 : 4);
+  b.tiles = (p.Lk + tpr * kBwdCols - 1) / (tpr * kBwdCols);
+  // as many blocks as fit the processors at once, each with two steps of its rows at least
+  int fit = (int)(220 * 1024 / (b.smem + 4096));
+  if (fit > 1024 / b.threads) fit = 1024 / b.threads;
+  const int64_t want = (int64_t)tcx::sm_count() * (fit < 1 ? 1 : fit), others = (int64_t)p.H * b.tiles * p.B;
+  int64_t strips = want / others;
+  const int64_t most = (p.Lq + 2 * slots - 1) / (2 * slots);
   if (strips > most) strips = most;
-  b.strips = (int)(strips < 1 ? 1 : strips > 65535 ? 65535 : strips);
+  if (strips > 65535 / p.B) strips = 65535 / p.B;
+  p.strips = (int)(strips < 1 ? 1 : strips);
+  b.parts = b.tiles * p.strips * p.B;
   return b;
 }
 bool vec_ok(const mf_relpos_args& a, const void* ptr) { return (a.Lk * dtype_size(a.dtype)) % 16 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -253,36 +279,37 @@ template <typename T, bool VEC>
 int run_fwd(const mf_relpos_args& a, cudaStream_t st) {
   RelP p = relpos_params(a);
   constexpr int kC = Cols<T, VEC>::kC;
-  p.log_tpr = log_threads(p.Lk, kC, kThreads);
+  p.log_tpr = log_threads(p.Lk, kC, VEC ? 0 : 5, kThreads);
   const int tpr = 1 << p.log_tpr, slots = kThreads >> p.log_tpr;
   const int tiles = (p.Lk + tpr * kC - 1) / (tpr * kC);
   // heads of a block: all of them, less where the table would take more than 48 KB or the rows do not occupy the processors
   int heads = p.H;
   while (heads > 1 && (size_t)heads * p.rows * sizeof(T) > 48 * 1024) heads = (heads + 1) / 2;
-  const int64_t row_blocks = ((int64_t)p.B * p.Lq + slots - 1) / slots, want = 4 * (int64_t)tcx::sm_count();
-  while (heads > 1 && row_blocks * tiles * ((p.H + heads - 1) / heads) < want) heads = (heads + 1) / 2;
+  const int64_t row_blocks = (p.Lq + slots - 1) / slots, want = 4 * (int64_t)tcx::sm_count();
+  while (heads > 1 && row_blocks * tiles * p.B * ((p.H + heads - 1) / heads) < want) heads = (heads + 1) / 2;
   const int groups = (p.H + heads - 1) / heads;
-  int64_t gy = (2 * want + (int64_t)tiles * groups - 1) / ((int64_t)tiles * groups);
-  if (gy > row_blocks) gy = row_blocks;
-  if (gy > 65535) gy = 65535;
+  int64_t strips = (2 * want + (int64_t)tiles * groups * p.B - 1) / ((int64_t)tiles * groups * p.B);
+  if (strips > row_blocks) strips = row_blocks;
+  if (strips > 65535 / p.B) strips = 65535 / p.B;
+  p.strips = (int)(strips < 1 ? 1 : strips);
   const size_t smem = lut_bytes(p) + (size_t)heads * p.rows * sizeof(T);
   constexpr auto kern = relpos_fwd_kernel<T, VEC>;
   if (int e = opt_in_smem<kern>(smem)) return e;
-  kern<<<dim3(tiles, (unsigned)gy, groups), kThreads, smem, st>>>(p, a.weight, static_cast<T*>(a.bias), heads);
+  kern<<<dim3(tiles, (unsigned)(p.strips * p.B), groups), kThreads, smem, st>>>(p, a.weight, static_cast<T*>(a.bias), heads);
   MF_LAUNCHED("relpos_fwd_kernel");
   return MF_OK;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 int run_bwd(const mf_relpos_args& a, cudaStream_t st) {
   RelP p = relpos_params(a);
-  const BwdPlan b = bwd_plan(p, Cols<T, VEC>::kC);
-  constexpr auto kern = relpos_bwd_kernel<T, VEC>;
+  const BwdPlan b = bwd_plan(p);
+  constexpr auto kern = relpos_bwd_kernel<T>;
   if (int e = opt_in_smem<kern>(b.smem)) return e;
   float* parts = static_cast<float*>(a.workspace);
-  kern<<<dim3(b.tiles, b.strips, p.H), b.threads, b.smem, st>>>(p, static_cast<const T*>(a.d_bias), parts);
+  kern<<<dim3(b.tiles, p.strips * p.B, p.H), b.threads, b.smem, st>>>(p, static_cast<const T*>(a.d_bias), parts);
   MF_LAUNCHED("relpos_bwd_kernel");
-  relpos_join_kernel<<<(p.rows * p.H + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(parts, b.tiles * b.strips, p.H, p.rows, a.d_weight, a.dw_dtype);
+  relpos_join_kernel<<<(p.rows * p.H + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(parts, b.parts, p.H, p.rows, a.d_weight, a.dw_dtype);
   MF_LAUNCHED("relpos_join_kernel");
   return MF_OK;
 }
@@ -294,18 +321,12 @@ int relpos_fwd(const mf_relpos_args& a, cudaStream_t st) {
   return r;
 }
 size_t relpos_bwd_workspace(const mf_relpos_args& a) {
-  size_t most = 0;
-  for (bool vec : {true, false}) {                 // whichever the alignment of d_bias asks for
-    RelP p = relpos_params(a);
-    const BwdPlan b = bwd_plan(p, vec ? 16 / (int)dtype_size(a.dtype) : 8);
-    const size_t n = sizeof(float) * (size_t)b.tiles * b.strips * p.H * p.rows;
-    if (n > most) most = n;
-  }
-  return most;
+  RelP p = relpos_params(a);
+  return sizeof(float) * (size_t)bwd_plan(p).parts * p.H * p.rows;
 }
 int relpos_bwd(const mf_relpos_args& a, cudaStream_t st) {
   int r = MF_OK;
-  MF_DISPATCH_FLOAT(a.dtype, T, r = vec_ok(a, a.d_bias) ? run_bwd<T, true>(a, st) : run_bwd<T, false>(a, st));
+  MF_DISPATCH_FLOAT(a.dtype, T, r = run_bwd<T>(a, st));
   return r;
 }
 

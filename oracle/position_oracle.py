@@ -2,6 +2,7 @@
 
 ``window`` also gives the bounds of the rounding errors of a kernel that keeps sums in 32 bits and rounds probabilities, their
 gradients and results to a type of unit roundoff ``u`` (half a step, ``finfo.eps / 2``)."""
+import functools
 import math
 
 import torch
@@ -19,16 +20,30 @@ def bucket(d, count, max_distance, scheme, bidirectional):
     near = side // 2
     if n < near:
         return shift + n
-    steps, k = side - near, 0
-    while k + 1 < steps and n ** steps * near ** (k + 1) >= max_distance ** (k + 1) * near ** steps:
-        k += 1
-    return shift + near + k
+    steps = side - near
+    entered = sum(n >= e for e in _entries(near, steps, max_distance))
+    return shift + near + entered
+
+
+@functools.lru_cache(None)
+def _entries(near, steps, max_distance):
+    """The smallest distances with log(n / near) / log(max_distance / near) * steps >= k, for k = 1 .. steps - 1."""
+    out, n = [], near
+    for k in range(1, steps):
+        while n ** steps < max_distance ** k * near ** (steps - k):
+            n += 1
+        out.append(n)
+    return tuple(out)
+
+
+@functools.lru_cache(None)
+def _table(count, max_distance, scheme, bidirectional):
+    return torch.tensor([bucket(x, count, max_distance, scheme, bidirectional) for x in range(-max_distance - 1, max_distance + 2)])
 
 
 def buckets(q_pos, k_pos, count, max_distance, scheme, bidirectional):
     d = (k_pos[:, None, :] - q_pos[:, :, None]).clamp(-max_distance - 1, max_distance + 1)
-    table = torch.tensor([bucket(x, count, max_distance, scheme, bidirectional) for x in range(-max_distance - 1, max_distance + 2)])
-    return table[d + max_distance + 1]
+    return _table(count, max_distance, scheme, bidirectional)[d + max_distance + 1]
 
 
 def relpos(weight, rows, d_bias=None):
