@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 3) relpos_bwd_kernel(const __grid_co
   for (int e = 0; e < kC; ++e) { cur[e] = 0; acc[e] = 0.f; }
   const int step = slots % width;
   auto wrap = [&](int c) { return c >= width ? c - width : c; };
+  auto wrap_in = [&](int c, int e) { return e < columns ? wrap(c) : 0; };
   struct Cursor { int i, first; const T* row; };                   // of the loads, and of the sums two rows behind
   auto start = [&]() { return Cursor{i0 + slot, (lane + slot) % width, in + (int64_t)(i0 + slot) * p.Lk}; };
   auto next = [&](Cursor& c) { c.i += slots; c.first = wrap(c.first + step); c.row += (int64_t)slots * p.Lk; };
@@ -181,20 +182,31 @@ __global__ void __launch_bounds__(kThreads, 3) relpos_bwd_kernel(const __grid_co
   auto add = [&](Cursor& c, const T (&x)[kC]) {
     bool close = near;
     const int qp = near_to(q_position(p, b, c.i), o.pos, close), qs = p.q_seg ? near_to(load_int(p.q_seg, b * p.qs_b + c.i, p.seg64), o.seg, close) : 0;
+    int row[kC];
+    if (close) {
 #pragma unroll
-    for (int e = 0; e < kC; ++e) {
-      if (e >= columns) break;
-      const int at = wrap(c.first + e * tpr);
-      int row;
-      if (close) {
-        row = row_of(p, lut, kpos[at] - qp);
-        if (p.q_seg && kseg[at] != qs) row = p.rows - 1;
-      } else {
-        row = row_of_far(p, lut, b, c.i, j0 + at);
+      for (int e = 0; e < kC; ++e) row[e] = kpos[wrap_in(c.first + e * tpr, e)];
+#pragma unroll
+      for (int e = 0; e < kC; ++e) row[e] = row_of(p, lut, row[e] - qp);
+      if (p.q_seg) {
+#pragma unroll
+        for (int e = 0; e < kC; ++e)
+          if (kseg[wrap_in(c.first + e * tpr, e)] != qs) row[e] = p.rows - 1;
       }
-      if (row != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row; acc[e] = 0.f; }
-      acc[e] += to_f(x[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kC; ++e) row[e] = row_of_far(p, lut, b, c.i, j0 + wrap_in(c.first + e * tpr, e));
     }
+    bool moved = false;
+#pragma unroll
+    for (int e = 0; e < kC; ++e) moved = moved || row[e] != cur[e];
+    if (__any_sync(0xffffffffu, moved)) {          // a warp is in one row of the bias: tpr is 32 at least
+#pragma unroll
+      for (int e = 0; e < kC; ++e)
+        if (row[e] != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row[e]; acc[e] = 0.f; }
+    }
+#pragma unroll
+    for (int e = 0; e < kC; ++e) acc[e] += to_f(x[e]);             // zeros for columns that are not there
     next(c);
   };
   Cursor in_at = start(), sum_at = start();
