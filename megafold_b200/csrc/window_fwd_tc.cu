@@ -2,13 +2,13 @@
 // multiples of 8 up to 128.
 //
 // A CTA takes 128 rows of queries (of the heads that share a key head) and walks the blocks of 64 keys that they see.  Warps 0-3: a thread owns a query row
-// (a TMEM lane): running maximum and sum, P over the scores in TMEM.  Warp 4 fetches Q, K and V by TMA, warp 5 issues the products
+// (a TMEM lane): running maximum and sum, P over the scores in TMEM.  Warp 4 fetches Q, K and V by TMA and issues the products
 //
 //   S(t) = Q K(t)^T  -> one of NB buffers of 64 columns        O += P(t) V(t)   (P as TMEM A operand, V MN-major)
 //
 // in the order S(0) [S(1)] PV(0) S(NB) PV(1) ..., so that a score buffer's P has been read when the next scores go into it.  O stays in
 // TMEM and is brought to a new maximum only when that grew by more than 2^8 in the exponent.  A window makes short walks
-// (5 blocks at 64 + 64 keys), so nothing is pipelined across items: several CTAs share an SM instead (3 up to DP = 64, with
+// (5 blocks at 64 + 64 keys), so nothing is pipelined across items: several CTAs share an SM instead (4 up to DP = 64, with
 // one score buffer each, 2 at DP = 128 with two) and fill each other's waits.
 //
 // Blocks that a row does not see whole go through a 64-bit mask a row (window, sinks, end of the keys, key mask); rows of V whose
@@ -22,12 +22,12 @@ namespace mf {
 namespace win {
 namespace {
 
-constexpr int kQ = 128, kK = 64, kThreads = 192;
+constexpr int kQ = 128, kK = 64, kThreads = 160;
 
 template <int DP> struct Cfg {
   static constexpr int NB = DP == 128 ? 2 : 1;                  // score buffers
-  static constexpr int NS = DP == 128 ? 2 : 3;                  // K and V stages
-  static constexpr int CTAS = DP == 128 ? 2 : 3;                // on an SM
+  static constexpr int NS = DP == 32 ? 3 : 2;                   // K and V stages
+  static constexpr int CTAS = DP == 128 ? 2 : 4;                // on an SM
   static constexpr uint32_t COLS = DP == 128 ? 256 : 128;       // TMEM
   static constexpr int QB = Geo<DP>::TILE(kQ), KB = Geo<DP>::TILE(kK);
   static constexpr size_t SMEM = 1024 + QB + 2 * NS * KB;
@@ -45,7 +45,7 @@ struct FwdP {
 };
 
 template <int NS, int NB> struct Bars {
-  uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_ready[NB], p_ready[NB], pv_done;
+  uint64_t q_full, k_full[NS], v_full[NS], s_ready[NB], p_ready[NB], pv_done;
 };
 
 template <int DP, typename T>
@@ -67,7 +67,7 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   if (tid == 0) {
     abort_s = 0;
     mbar_init(&bar.q_full, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
+    for (int i = 0; i < NS; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.v_full[i], 1); }
     for (int i = 0; i < NB; ++i) { mbar_init(&bar.s_ready[i], 1); mbar_init(&bar.p_ready[i], 128); }
     mbar_init(&bar.pv_done, 1);
     mbar_fence_init();
@@ -90,27 +90,33 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const int first = (int)((int64_t)tiles.count() * part / f.sp.splits), T_ = (int)((int64_t)tiles.count() * (part + 1) / f.sp.splits) - first;
 
   if (warp == 4) {
-    // ------------------------------------------------------------------------------------------------ copies
-    if (elect_one() && T_ > 0) {
-      mbar_expect_tx(&bar.q_full, f.q_bytes);
-      load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h0, i0, n * f.cq.n_mul, b * f.cq.b_mul);
-      int t = 0;
-      for (; t < T_; ++t) {
-        const int s = t % NS, j0 = tiles.at(first + t) * kK;
-        if (t >= NS) { wait_or_flag(&bar.k_empty[s], (t / NS - 1) & 1, abort_flag); wait_or_flag(&bar.v_empty[s], (t / NS - 1) & 1, abort_flag); }
-        if (*abort_flag) break;
-        mbar_expect_tx(&bar.k_full[s], C::KB);
-        load_tile_tma<DP>(sK + s * C::KB, &mk, &bar.k_full[s], kK, hk, j0, n * f.ck.n_mul, b * f.ck.b_mul);
-        mbar_expect_tx(&bar.v_full[s], C::KB);
-        load_tile_tma<DP>(sV + s * C::KB, &mv, &bar.v_full[s], kK, hk, j0, n * f.cv.n_mul, b * f.cv.b_mul);
-      }
-      // none may land after this CTA has left
-      drain_ring(&bar.q_full, 1, 1); drain_ring(bar.k_full, t, NS); drain_ring(bar.v_full, t, NS);
-    }
-  } else if (warp == 5) {
-    // ------------------------------------------------------------------------------------------------ products
+    // ----------------------------------------------------------------------------------------- copies and products
+    // P(t) in TMEM says that S(t) is complete, so the stage of K(t) is free.  With one score buffer S(t) is issued behind P V (t - 1), so
+    // the stage of V(t - 1) is free, too; with two that product is waited for (it has long been complete).
     const uint32_t id_s = idesc_f16(128, kK, f.fmt, 0, 0), id_o = idesc_f16(128, DP, f.fmt, 0, 1);
     const uint32_t q_lo = desc_lo(smem_u32(sQ), 16);
+    const bool leader = elect_one();
+    int k_asked = 0, v_asked = 0;
+    auto ask_k = [&](int upto) {
+      for (; k_asked < upto && k_asked < T_; ++k_asked) {
+        uint64_t* full = &bar.k_full[k_asked % NS];
+        if (leader) {
+          mbar_expect_tx(full, C::KB);
+          load_tile_tma<DP>(sK + k_asked % NS * C::KB, &mk, full, kK, hk, tiles.at(first + k_asked) * kK, n * f.ck.n_mul, b * f.ck.b_mul);
+        }
+      }
+      __syncwarp();
+    };
+    auto ask_v = [&](int upto) {
+      for (; v_asked < upto && v_asked < T_; ++v_asked) {
+        uint64_t* full = &bar.v_full[v_asked % NS];
+        if (leader) {
+          mbar_expect_tx(full, C::KB);
+          load_tile_tma<DP>(sV + v_asked % NS * C::KB, &mv, full, kK, hk, tiles.at(first + v_asked) * kK, n * f.cv.n_mul, b * f.cv.b_mul);
+        }
+      }
+      __syncwarp();
+    };
     auto scores = [&](int t) {                    // false: given up
       const int s = t % NS;
       wait_or_flag(&bar.k_full[s], (t / NS) & 1, abort_flag);
@@ -119,11 +125,16 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16), d = t0 + (t % NB) * 64;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) mma_ss_el(d, q_lo + k_step<DP>(ks, kQ), G::HI, k_lo + k_step<DP>(ks, kK), G::HI, id_s, ks > 0);
-      tc_commit_el(&bar.k_empty[s]);
       tc_commit_el(&bar.s_ready[t % NB]);
       return true;
     };
     if (T_ > 0) {
+      if (leader) {
+        mbar_expect_tx(&bar.q_full, f.q_bytes);
+        load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h0, i0, n * f.cq.n_mul, b * f.cq.b_mul);
+      }
+      ask_k(NS);
+      ask_v(NS);
       wait_or_flag(&bar.q_full, 0, abort_flag);
       bool ok = true;
       for (int t = 0; ok && t < NB && t < T_; ++t) ok = scores(t);
@@ -131,21 +142,27 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         const int s = t % NS;
         wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);
         wait_or_flag(&bar.p_ready[t % NB], (t / NB) & 1, abort_flag);
+        if (NB > 1 && t > 0) wait_or_flag(&bar.pv_done, (t - 1) & 1, abort_flag);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
         tc_fence_after();
         const uint32_t v_lo = desc_lo(smem_u32(sV + s * C::KB), kK * G::ROWB), a = t0 + (t % NB) * 64;
 #pragma unroll
         for (int ks = 0; ks < kK / 16; ++ks) mma_ts_el(tO, a + ks * 8, v_lo + ks * (16 * G::ROWB / 16), G::HI, id_o, t > 0 || ks > 0);
-        tc_commit_el(&bar.v_empty[s]);
         tc_commit_el(&bar.pv_done);
+        if (NB > 1 && NS == NB) ask_k(t + 1 + NS);             // S(t + NB) needs the stage that S(t) has left
         if (t + NB < T_) ok = scores(t + NB);
+        ask_k(t + 1 + NS);
+        ask_v(t + NS);
       }
     }
+    // none may land after this CTA has left
+    if (leader && T_ > 0) { drain_ring(&bar.q_full, 1, 1); drain_ring(bar.k_full, k_asked, NS); drain_ring(bar.v_full, v_asked, NS); }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const int r = warp * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
-    const bool live = l_ < nq && i < p.Lq;
+    const bool live = l_ < nq && i < p.Lq, any_live = __any_sync(0xffffffffu, live);       // a warp without rows (a few queries) only takes part
     const uint8_t* mask = p.mask ? p.mask + b * p.ms[0] + n * p.ms[1] : nullptr;
     auto mask_bytes = [&](int t, uint32_t (&mb)[2]) {
       const int j = tiles.at(first + t) * kK + lane;
@@ -165,47 +182,56 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       if (__any_sync(0xffffffffu, *abort_flag)) break;
       tc_fence_after();
       const uint32_t tS = t0 + lanes + (t % NB) * 64;
-      uint32_t s0[32], s1[32];
-      tmem_ld32(tS, s0);
-      tmem_ld32(tS + 32, s1);
-      tmem_ld_wait(s0, s1);
-      if (!(all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + kK) && (keep[0] & keep[1]) == ~0u)) {
-        const uint32_t b0 = seen32(p, at, j0) & keep[0], b1 = seen32(p, at, j0 + 32) & keep[1];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          if (!(b0 >> e & 1)) s0[e] = 0xff800000u;
-          if (!(b1 >> e & 1)) s1[e] = 0xff800000u;
-        }
-      }
-      float mx = m;
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) mx = max3f(max3f(mx, __uint_as_float(s0[e]), __uint_as_float(s0[e + 1])), __uint_as_float(s1[e]), __uint_as_float(s1[e + 1]));
+      const bool whole = all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + kK) && (keep[0] & keep[1]) == ~0u;
       float corr = 1.f;
-      if ((mx - m) * f.c1 > 8.f) {                // also from -inf
-        corr = ex2f((m - mx) * f.c1);
-        m = mx;
-        l *= corr;
-      }
-      const float off = m == -INFINITY ? 0.f : -m * f.c1;       // nothing seen so far: every logit is -inf
-      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      if (any_live) {
+        const uint32_t bits[2] = {whole ? ~0u : seen32(p, at, j0) & keep[0], whole ? ~0u : seen32(p, at, j0 + 32) & keep[1]};
+        auto hide = [&](uint32_t (&s)[32], uint32_t b) {
+          if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        const float2 x = fma2(make_float2(__uint_as_float(s0[e]), __uint_as_float(s0[e + 1])), c2, o2);
-        const float2 y = fma2(make_float2(__uint_as_float(s1[e]), __uint_as_float(s1[e + 1])), c2, o2);
-        const float2 px = make_float2(ex2f(x.x), ex2f(x.y)), py = make_float2(ex2f(y.x), ex2f(y.y));
-        sum[0] = add2(sum[0], px); sum[1] = add2(sum[1], py);
-        s0[e / 2] = Pack2<T>::pack(px.x, px.y);
-        s1[e / 2] = Pack2<T>::pack(py.x, py.y);
+            for (int e = 0; e < 32; ++e)
+              if (!(b >> e & 1)) s[e] = 0xff800000u;
+          }
+        };
+        uint32_t s[32];
+        float m4[4] = {m, m, m, m};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {             // the scores are read twice: 64 of them do not fit beside the rest
+          tmem_ld32(tS + c * 32, s);
+          tmem_ld_wait();
+          pin32(s);
+          hide(s, bits[c]);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) m4[e / 2 % 4] = max3f(m4[e / 2 % 4], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        }
+        const float mx = fmaxf(max3f(m4[0], m4[1], m4[2]), m4[3]);
+        if ((mx - m) * f.c1 > 8.f) {              // also from -inf
+          corr = ex2f((m - mx) * f.c1);
+          m = mx;
+          l *= corr;
+        }
+        const float off = m == -INFINITY ? 0.f : -m * f.c1;     // nothing seen so far: every logit is -inf
+        const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tmem_ld32(tS + c * 32, s);
+          tmem_ld_wait();
+          pin32(s);
+          hide(s, bits[c]);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
+            const float2 pr = make_float2(ex2f(x.x), ex2f(x.y));
+            sum[e / 2 % 2] = add2(sum[e / 2 % 2], pr);
+            w[e / 2] = Pack2<T>::pack(pr.x, pr.y);
+          }
+          tmem_st16(tS + c * 16, w);              // over scores that have been read twice
+        }
+        const float2 s2 = add2(sum[0], sum[1]);
+        l += s2.x + s2.y;
       }
-      {
-        uint32_t (&w0)[16] = *reinterpret_cast<uint32_t (*)[16]>(s0);
-        uint32_t (&w1)[16] = *reinterpret_cast<uint32_t (*)[16]>(s1);
-        tmem_st16(tS, w0);
-        tmem_st16(tS + 16, w1);
-      }
-      const float2 s2 = add2(sum[0], sum[1]);
-      l += s2.x + s2.y;
       // P V of the block before: O may be changed, and has to be complete to be
       if (t > 0) {
         wait_or_flag(&bar.pv_done, (t - 1) & 1, abort_flag);
