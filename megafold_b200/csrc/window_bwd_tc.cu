@@ -12,14 +12,19 @@
 //
 // window_dq_tc_kernel   a CTA keeps 128 rows of queries and walks the blocks of 64 keys that they see, queries on the lanes:
 //                         S = Q K^T   dP = dO V^T   dS = P (dP - delta)   dQ += dS K
+//                       (a narrow window: a walk that sums P dP to delta before that one, instead of the sum of dO O)
 //
 // Scores are formed twice (7 products instead of 5): a single pass would add dQ or dK and dV atomically, in an order that changes, and
 // a window leaves few tiles to carry an accumulator over.  In both walking kernels eight compute warps take a block, two to a
-// set of lanes with 32 columns each; one warp copies, one issues products.  TMEM lets two CTAs share an SM and fill each other's waits
-// (dK and dV at DP = 128: one CTA, two score buffers).
+// set of lanes with 32 columns each; one warp copies, one issues products.  TMEM lets two CTAs share an SM and fill each other's
+// waits (dK and dV at DP = 128: one CTA, two score buffers).  In the dQ kernel S and dP have barriers of their own besides, so that
+// the next S is formed while the compute warps exponentiate (184 -> 168 us at 16384 tokens, 16 heads of 64, window 1024);
+// in the other one, where each barrier stands between two products, that cost more than it gave (199 -> 233).
 //
 // Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they are overwritten with zeros in shared memory.
 // P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  Waits are bounded as in the forward.
+#include <type_traits>
+
 #include "window_tc_common.cuh"
 
 namespace mf {
@@ -42,21 +47,23 @@ struct BwdP {
   int q_bytes, qt_bytes;    // bytes of the rows of a block / a tile of queries (copies leave the rest of it alone)
   float c1;
   uint32_t fmt;
+  int two_walks;            // dQ: a walk for delta first
+  float* delta;             // ... which it writes here
   const uint8_t* terms;     // [packs of heads][n_blocks][kXB]
   float* parts;
   int* status;
 };
 
 // ---------------------------------------------------------------------------------------------------------------- terms
-// blockIdx = (block of rows, pack of heads, b * N + n); four threads a row
-template <typename T>
+// blockIdx = (block of rows, pack of heads, b * N + n); four threads a row.  GIVEN: delta has been written by the dQ kernel.
+template <typename T, bool GIVEN>
 __global__ void __launch_bounds__(256) window_terms_kernel(const __grid_constant__ WinP p, float* __restrict__ delta, uint8_t* __restrict__ terms, float sqrt_d) {
   const int r = threadIdx.x >> 2, q = threadIdx.x & 3;
   const int l = r / p.pack, nq = queries_of<kQB>(p), i = blockIdx.x * nq + l, h = blockIdx.y * p.pack + r - l * p.pack;
   const bool live = l < nq && i < p.Lq;
   const int64_t bn = blockIdx.z, row = (bn * p.Lq + i) * p.H + h;
   float s = 0.f;
-  if (live) {
+  if (!GIVEN && live) {
     const T *po = static_cast<const T*>(p.o) + row * p.D, *pg = static_cast<const T*>(p.d_o) + row * p.D;
     for (int d = q * 8; d < p.D; d += 32) {
       const uint4 a = __ldg(reinterpret_cast<const uint4*>(po + d)), g = __ldg(reinterpret_cast<const uint4*>(pg + d));
@@ -75,7 +82,7 @@ __global__ void __launch_bounds__(256) window_terms_kernel(const __grid_constant
   if (live) {
     const int64_t at = (bn * p.H + h) * p.Lq + i;
     lse = p.lse[at];
-    delta[at] = s;
+    if (GIVEN) s = delta[at]; else delta[at] = s;
   }
   // a row that sees nothing, or is none, gets probability 0 from a finite term
   __nv_bfloat16 a[3], d[3];
@@ -316,7 +323,7 @@ template <int DP> struct QCfg {
   static constexpr size_t SMEM = 1024 + 2 * QB + 2 * NS * KB;
 };
 template <int NS> struct QBars {
-  uint64_t q_full, kv_full[NS], kv_empty[NS], sd_ready, ds_ready, done;
+  uint64_t q_full, kv_full[NS], kv_empty[NS], s_ready, d_ready, s_read, ds_written, summed, done;
 };
 
 template <int DP, typename T>
@@ -331,6 +338,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *sQ = smem, *sG = sQ + C::QB, *sK = sG + C::QB, *sV = sK + NS * C::KB;
   __shared__ QBars<NS> bar;
+  __shared__ float sums[2][kRows];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
 
@@ -339,7 +347,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
     abort_s = 0;
     mbar_init(&bar.q_full, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
-    mbar_init(&bar.sd_ready, 1); mbar_init(&bar.ds_ready, kCompute); mbar_init(&bar.done, 1);
+    mbar_init(&bar.s_ready, 1); mbar_init(&bar.d_ready, 1); mbar_init(&bar.s_read, kCompute); mbar_init(&bar.ds_written, kCompute); mbar_init(&bar.summed, kCompute); mbar_init(&bar.done, 1);
     mbar_fence_init();
     prefetch_tmap(&mq); prefetch_tmap(&mg); prefetch_tmap(&mk); prefetch_tmap(&mv);
   }
@@ -353,7 +361,9 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
   const int bn = group / head_groups(p), h0 = (group - bn * head_groups(p)) * p.pack, n = bn % p.N, b = bn / p.N, hk = h0 / p.G;
   const int nq = queries_of<kRows>(p), i0 = qt * nq, i1 = i0 + nq < p.Lq ? i0 + nq : p.Lq;
   const KeyTiles tiles = key_tiles<kKB>(p, i0, i1);
-  const int T_ = tiles.count();
+  // steps: the blocks of keys, or (f.two_walks) all of them for delta and then all of them for dQ
+  const int blocks = tiles.count(), delta_steps = f.two_walks ? blocks : 0, T_ = delta_steps + blocks;
+  auto key_block = [&](int t) { return tiles.at(t < blocks ? t : t - blocks) * kKB; };
 
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------------ copies
@@ -363,7 +373,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       load_tile_tma<DP>(sG, &mg, &bar.q_full, kRows, h0, i0, n, b);
       int t = 0;
       for (; t < T_; ++t) {
-        const int s = t % NS, j0 = tiles.at(t) * kKB;
+        const int s = t % NS, j0 = key_block(t);
         if (t >= NS) wait_or_flag(&bar.kv_empty[s], (t / NS - 1) & 1, abort_flag);
         if (*abort_flag) break;
         mbar_expect_tx(&bar.kv_full[s], 2 * C::KB);
@@ -376,33 +386,47 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
     // ------------------------------------------------------------------------------------------------ products
     const uint32_t id_s = idesc_f16(128, kKB, f.fmt, 0, 0), id_q = idesc_f16(128, DP, f.fmt, 0, 1);
     const uint32_t q_lo = desc_lo(smem_u32(sQ), 16), g_lo = desc_lo(smem_u32(sG), 16);
-    auto scores = [&](int t) {
+    auto s_scores = [&](int t) {                  // S(t); false: given up
       const int s = t % NS;
       wait_or_flag(&bar.kv_full[s], (t / NS) & 1, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag)) return false;
       tc_fence_after();
-      const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16), v_lo = desc_lo(smem_u32(sV + s * C::KB), 16);
+      const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16);
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) mma_ss_el(t0, q_lo + k_step<DP>(ks, kRows), G::HI, k_lo + k_step<DP>(ks, kKB), G::HI, id_s, ks > 0);
+      tc_commit_el(&bar.s_ready);
+      return true;
+    };
+    auto d_scores = [&](int t) {                  // dP(t), of the stage that S(t) waited for
+      const uint32_t v_lo = desc_lo(smem_u32(sV + t % NS * C::KB), 16);
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) mma_ss_el(t0 + 64, g_lo + k_step<DP>(ks, kRows), G::HI, v_lo + k_step<DP>(ks, kKB), G::HI, id_s, ks > 0);
-      tc_commit_el(&bar.sd_ready);
-      return true;
+      tc_commit_el(&bar.d_ready);
     };
     if (T_ > 0) {
       wait_or_flag(&bar.q_full, 0, abort_flag);
-      bool ok = scores(0);
+      bool ok = s_scores(0);
+      if (ok) d_scores(0);
       for (int t = 0; ok && t < T_; ++t) {
         const int s = t % NS;
-        wait_or_flag(&bar.ds_ready, t & 1, abort_flag);
-        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        // S has been read: the next one, while the compute warps exponentiate (with one stage its keys are not there yet)
+        wait_or_flag(&bar.s_read, t & 1, abort_flag);
+        if (NS > 1 && t + 1 < T_) ok = s_scores(t + 1);
+        wait_or_flag(&bar.ds_written, t & 1, abort_flag);
+        if (!ok || __any_sync(0xffffffffu, *abort_flag)) break;
         tc_fence_after();
-        const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), kKB * G::ROWB);
+        if (t >= delta_steps) {
+          const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), kKB * G::ROWB);
 #pragma unroll
-        for (int ks = 0; ks < kKB / 16; ++ks) mma_ts_el(tQ, t0 + (ks / 2) * 32 + (ks % 2) * 8, k_lo + ks * (16 * G::ROWB / 16), G::HI, id_q, t > 0 || ks > 0);
+          for (int ks = 0; ks < kKB / 16; ++ks)
+            mma_ts_el(tQ, t0 + 64 + (ks / 2) * 32 + (ks % 2) * 8, k_lo + ks * (16 * G::ROWB / 16), G::HI, id_q, t > delta_steps || ks > 0);
+        }
         tc_commit_el(&bar.kv_empty[s]);
         if (t + 1 == T_) tc_commit_el(&bar.done);
-        else ok = scores(t + 1);
+        else {
+          if (NS == 1) ok = s_scores(t + 1);
+          if (ok) d_scores(t + 1);
+        }
       }
     }
   } else {
@@ -411,47 +435,86 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const bool live = l_ < nq && i < p.Lq;
     float lse = -INFINITY, delta = 0.f;
+    const int64_t stat = ((int64_t)bn * p.H + h) * p.Lq + i;
     if (live) {
-      const int64_t row = ((int64_t)bn * p.H + h) * p.Lq + i;
-      lse = p.lse[row]; delta = p.delta[row];
+      lse = p.lse[stat];
+      if (!f.two_walks) delta = p.delta[stat];
     }
+    float sum = 0.f;                              // of P dP over this thread's columns
     const float off = lse == -INFINITY ? -INFINITY : -lse * kLog2e;       // a row that sees nothing: probability 0
     const uint8_t* mask = p.mask ? p.mask + b * p.ms[0] + n * p.ms[1] : nullptr;
     auto mask_byte = [&](int t, int hf) -> uint32_t {
-      const int j = tiles.at(t) * kKB + hf * 32 + lane;
+      const int j = key_block(t) + hf * 32 + lane;
       return j < p.Lk && mask[(int64_t)j * p.ms[2]];
     };
     uint32_t mb = 1;
     if (mask && T_ > 0) mb = mask_byte(0, half);
     for (int t = 0; t < T_; ++t) {
-      const int j0 = tiles.at(t) * kKB + half * 32;
+      const int j0 = key_block(t) + half * 32;
       uint32_t keep = ~0u;
       if (mask) {
         keep = __ballot_sync(0xffffffffu, mb);
         if (t + 1 < T_) mb = mask_byte(t + 1, half);
       }
-      wait_or_flag(&bar.sd_ready, t & 1, abort_flag);
+      if (f.two_walks && t == delta_steps) {      // the two halves' sums make delta
+        sums[half][r] = sum;
+        mbar_arrive(&bar.summed);
+        wait_or_flag(&bar.summed, 0, abort_flag);
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        delta = sum + sums[half ^ 1][r];
+        if (half == 0 && live) f.delta[stat] = delta;
+      }
+      wait_or_flag(&bar.s_ready, t & 1, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag)) break;
       tc_fence_after();
-      const uint32_t tS = t0 + lanes + half * 32;
+      const uint32_t tS = t0 + lanes + half * 32, tD = tS + 64;
       uint32_t s[32], d[32];
       tmem_ld32(tS, s);
-      tmem_ld32(tS + 64, d);
-      tmem_ld_wait(s, d);
+      tmem_ld_wait();
+      pin32(s);
+      tc_fence_before();
+      mbar_arrive(&bar.s_read);
       const bool whole = all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + 32) && keep == ~0u;
       const uint32_t bits = whole ? ~0u : seen32(p, at, j0) & keep;
       const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off), d2 = make_float2(delta, delta);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
-        float2 ds = mul2(make_float2(ex2f(x.x), ex2f(x.y)), sub2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), d2));
+        s[e] = __float_as_uint(ex2f(x.x)); s[e + 1] = __float_as_uint(ex2f(x.y));
+      }
+      wait_or_flag(&bar.d_ready, t & 1, abort_flag);
+      if (__any_sync(0xffffffffu, *abort_flag)) break;
+      tc_fence_after();
+      tmem_ld32(tD, d);
+      tmem_ld_wait();
+      pin32(d);
+      if (t < delta_steps) {
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float2 x = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])));
+          if (!whole) {
+            if (!(bits >> e & 1)) x.x = 0.f;
+            if (!(bits >> (e + 1) & 1)) x.y = 0.f;
+          }
+          acc = add2(acc, x);
+        }
+        sum += acc.x + acc.y;
+        tc_fence_before();
+        mbar_arrive(&bar.ds_written);
+        continue;
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        float2 ds = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sub2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), d2));
         if (!whole) {
           if (!(bits >> e & 1)) ds.x = 0.f;
           if (!(bits >> (e + 1) & 1)) ds.y = 0.f;
         }
-        s[e / 2] = Pack2<T>::pack(ds.x, ds.y);
+        w[e / 2] = Pack2<T>::pack(ds.x, ds.y);
       }
-      tmem_st16(tS, *reinterpret_cast<uint32_t (*)[16]>(s));
+      tmem_st16(tD, w);
       if (mask) {
         // rows of masked keys of K, this warp set's 32 keys of the block (the keys beyond Lk are zeros already): S has been formed
         const uint32_t z = ~keep & ones32(p.Lk - j0);
@@ -469,7 +532,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&bar.ds_ready);
+      mbar_arrive(&bar.ds_written);
     }
     if (T_ > 0) wait_or_flag(&bar.done, 0, abort_flag);
     tc_fence_after();
@@ -482,6 +545,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
             store_rows_at<T>(tQ + lanes + c * 32, p.scale, live ? out + c * 32 : nullptr, p.D - c * 32);
       } else if (live && half == 0) {
         for (int e = 0; e < p.D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0u, 0u, 0u, 0u);
+        if (f.two_walks) f.delta[stat] = 0.f;
       }
     }
   }
@@ -513,7 +577,11 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   f.fmt = a.dtype == MF_BF16 ? 1u : 0u;
   float* delta = static_cast<float*>(a.workspace);
   uint8_t* terms = static_cast<uint8_t*>(a.workspace) + delta_bytes(p);
-  p.delta = delta; f.terms = terms;
+  // delta of a row is the sum of o d_o, o rounded to 16 bits, and dS = P (dP - delta) gets P times its error: with few keys a row, where P
+  // is large, that is as much as dS's own rounding (3 keys: dQ off by 3.2e-3 of its norm in bf16, instead of 2.4e-3; 129 keys: 2.6e-3).
+  // Up to 512 keys the dQ kernel forms it as the sum of P dP instead, in a walk of its own, which is short there.
+  f.two_walks = (int64_t)p.left + p.right + 1 + p.sinks <= 512 || p.Lk <= 512;
+  p.delta = f.delta = delta; f.terms = terms;
   f.parts = reinterpret_cast<float*>(terms + term_bytes(p));
   f.status = status_word();
   MF_REQUIRE(f.status, MF_ERR_CUDA, "could not allocate the device status word");
@@ -534,16 +602,29 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   if ((r = operand_map(&mk64, &f.ck, a.k, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.k_strides, G::COLS, 1, kKB))) return r;
   if ((r = operand_map(&mv64, &f.cv, a.v, a.dtype, a.B, a.N, a.Lk, a.Hk, a.D, a.v_strides, G::COLS, 1, kKB))) return r;
 
-  window_terms_kernel<T><<<dim3(f.n_blocks, head_groups(p), a.B * a.N), 256, 0, st>>>(p, delta, terms, sqrtf((float)a.D));
-  MF_LAUNCHED("window_terms_kernel");
+  const auto terms_kernel = [&](auto given) -> int {
+    window_terms_kernel<T, decltype(given)::value><<<dim3(f.n_blocks, head_groups(p), a.B * a.N), 256, 0, st>>>(p, delta, terms, sqrtf((float)a.D));
+    MF_LAUNCHED("window_terms_kernel");
+    return MF_OK;
+  };
   constexpr auto dkv = window_dkv_tc_kernel<DP, T>;
+  constexpr auto dq = window_dq_tc_kernel<DP, T>;
   if ((r = opt_in_smem<dkv>(KvCfg<DP>::SMEM))) return r;
+  if ((r = opt_in_smem<dq>(QCfg<DP>::SMEM))) return r;
+  const auto dq_kernel = [&]() -> int {
+    dq<<<(unsigned)grid_q, kThreads, QCfg<DP>::SMEM, st>>>(mq, mg, mk64, mv64, f);
+    MF_LAUNCHED("window_dq_tc_kernel");
+    return MF_OK;
+  };
+  if (f.two_walks) {
+    if ((r = dq_kernel())) return r;
+    if ((r = terms_kernel(std::true_type{}))) return r;
+  } else {
+    if ((r = terms_kernel(std::false_type{}))) return r;
+    if ((r = dq_kernel())) return r;
+  }
   dkv<<<(unsigned)grid_kv, kThreads, KvCfg<DP>::SMEM, st>>>(mk, mv, mq64, mg64, f);
   MF_LAUNCHED("window_dkv_tc_kernel");
-  constexpr auto dq = window_dq_tc_kernel<DP, T>;
-  if ((r = opt_in_smem<dq>(QCfg<DP>::SMEM))) return r;
-  dq<<<(unsigned)grid_q, kThreads, QCfg<DP>::SMEM, st>>>(mq, mg, mk64, mv64, f);
-  MF_LAUNCHED("window_dq_tc_kernel");
   return window_join<T, kKeys, kQB>(p, f.plan, f.parts, st);
 }
 template <typename T>
