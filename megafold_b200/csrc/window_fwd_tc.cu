@@ -1,15 +1,19 @@
 // Sliding-window attention with sinks, forward, on the tensor cores (tcgen05 + TMEM + TMA): 16-bit tensors, head sizes that are
 // multiples of 8 up to 128.
 //
-// A CTA takes 128 rows of queries (of the heads that share a key head) and walks the blocks of 64 keys that they see.  Warps 0-3: a thread owns a query row
-// (a TMEM lane): running maximum and sum, P over the scores in TMEM.  Warp 4 fetches Q, K and V by TMA and issues the products
+// A CTA takes 128 rows of queries (of the heads that share a key head) and walks the blocks of 64 keys that they see.  Warps 0-7: two
+// threads share a query row (a TMEM lane), 32 columns each; running maximum (the two exchange theirs) and sum, P over the
+// scores in TMEM.  Warp 8 fetches Q, K and V by TMA, warp 9 issues the products
 //
-//   S(t) = Q K(t)^T  -> one of NB buffers of 64 columns        O += P(t) V(t)   (P as TMEM A operand, V MN-major)
+//   S(t) = Q K(t)^T into one of two buffers          O += P(t) V(t)   (P as TMEM A operand, V MN-major)
 //
-// in the order S(0) [S(1)] PV(0) S(NB) PV(1) ..., so that a score buffer's P has been read when the next scores go into it.  O stays in
-// TMEM and is brought to a new maximum only when that grew by more than 2^8 in the exponent.  A window makes short walks
-// (5 blocks at 64 + 64 keys), so nothing is pipelined across items: several CTAs share an SM instead (4 up to DP = 64, with
-// one score buffer each, 2 at DP = 128 with two) and fill each other's waits.
+// in the order S(0) S(1) PV(0) S(2) PV(1) ..., so that a buffer's P has been read when the next scores go over it, and the next scores are
+// there while this block's are exponentiated.  O stays in TMEM and is brought to a new maximum only when that grew by more than
+// 2^8 in the exponent.  A window makes short walks (5 blocks at 64 + 64 keys), so nothing is pipelined across items: two CTAs share
+// an SM instead.  Tried at [1, 1, 16384, 16 on 4 heads, 64], window 1024 / [2, 1, 2048 of 6001, 16 on 4, 128], window 2047 / one token of 64
+// sequences, 32 on 8 heads of 128: this 160 / 94 / 69 us; one thread a row, one score buffer, four CTAs (two at 128 columns) 145 / 103 / 96;
+// one score buffer, two threads a row 159 / 127 / 87; blocks of 128 keys 168 / 102 / 77.
+// Bound: the exponentials, half of the time at 64 columns (16 a clock and SM), and the waits between a block's steps.
 //
 // Blocks that a row does not see whole go through a 64-bit mask a row (window, sinks, end of the keys, key mask); rows of V whose
 // key is masked are overwritten with zeros in shared memory, since 0 * NaN would reach the sum.  P is rounded to the
@@ -22,13 +26,13 @@ namespace mf {
 namespace win {
 namespace {
 
-constexpr int kQ = 128, kK = 64, kThreads = 160;
+constexpr int kQ = 128, kK = 64;
+constexpr int NB = 2;                                           // score buffers of 64 columns
+constexpr int kSoft = 256, kThreads = kSoft + 64;
+constexpr uint32_t kCols = 256;                                 // TMEM: scores at 0 and 64, O at 128
 
 template <int DP> struct Cfg {
-  static constexpr int NB = DP == 128 ? 2 : 1;                  // score buffers
-  static constexpr int NS = DP == 32 ? 3 : 2;                   // K and V stages
-  static constexpr int CTAS = DP == 128 ? 2 : 4;                // on an SM
-  static constexpr uint32_t COLS = DP == 128 ? 256 : 128;       // TMEM
+  static constexpr int NS = DP == 128 ? 2 : 3;                  // K and V stages
   static constexpr int QB = Geo<DP>::TILE(kQ), KB = Geo<DP>::TILE(kK);
   static constexpr size_t SMEM = 1024 + QB + 2 * NS * KB;
 };
@@ -44,36 +48,37 @@ struct FwdP {
   int* status;
 };
 
-template <int NS, int NB> struct Bars {
-  uint64_t q_full, k_full[NS], v_full[NS], s_ready[NB], p_ready[NB], pv_done;
+template <int NS> struct Bars {
+  uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_ready[NB], p_ready[NB], pv_done;
 };
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(kThreads, Cfg<DP>::CTAS)
+__global__ void __launch_bounds__(kThreads, 2)
 window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                      const __grid_constant__ FwdP f) {
   using C = Cfg<DP>;
   using G = Geo<DP>;
-  constexpr int NS = C::NS, NB = C::NB;
+  constexpr int NS = C::NS;
   const WinP& p = f.w;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *sQ = smem, *sK = sQ + C::QB, *sV = sK + NS * C::KB;
-  __shared__ Bars<NS, NB> bar;
+  __shared__ Bars<NS> bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
+  __shared__ float other[2][2][kQ];               // [parity of the block][half of the columns][row]: maxima, at the end sums
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   if (tid == 0) {
     abort_s = 0;
     mbar_init(&bar.q_full, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.v_full[i], 1); }
-    for (int i = 0; i < NB; ++i) { mbar_init(&bar.s_ready[i], 1); mbar_init(&bar.p_ready[i], 128); }
+    for (int i = 0; i < NS; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
+    for (int i = 0; i < NB; ++i) { mbar_init(&bar.s_ready[i], 1); mbar_init(&bar.p_ready[i], kSoft); }
     mbar_init(&bar.pv_done, 1);
     mbar_fence_init();
     prefetch_tmap(&mq); prefetch_tmap(&mk); prefetch_tmap(&mv);
   }
-  if (warp == 0) { tmem_alloc(&tmem_base_s, C::COLS); tmem_relinquish(); }
+  if (warp == 0) { tmem_alloc(&tmem_base_s, kCols); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -89,52 +94,53 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const KeyTiles tiles = key_tiles<kK>(p, i0, i1);
   const int first = (int)((int64_t)tiles.count() * part / f.sp.splits), T_ = (int)((int64_t)tiles.count() * (part + 1) / f.sp.splits) - first;
 
-  if (warp == 4) {
-    // ----------------------------------------------------------------------------------------- copies and products
-    // P(t) in TMEM says that S(t) is complete, so the stage of K(t) is free.  With one score buffer S(t) is issued behind P V (t - 1), so
-    // the stage of V(t - 1) is free, too; with two that product is waited for (it has long been complete).
+  if (warp == 8) {
+    // ------------------------------------------------------------------------------------------------ copies
+    // A copy a panel, each from a lane of its own: one instruction for two copies costs the warp little more than one copy.  K goes ahead of V:
+    // S(t) has left the stage of K(t) one product before V(t) is done with.
+    const bool leader = elect_one();
+    auto ask = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* full, int t, const Coords& c) {
+      if (leader) mbar_expect_tx(full, C::KB);
+      __syncwarp();
+      if (lane < G::PANELS) tma_load_5d(dst + lane * kK * G::ROWB, m, full, lane * G::COLS, hk, tiles.at(first + t) * kK, n * c.n_mul, b * c.b_mul);
+      __syncwarp();
+    };
+    int k_asked = 0, v_asked = 0;
+    if (T_ > 0) {
+      if (leader) mbar_expect_tx(&bar.q_full, f.q_bytes);
+      __syncwarp();
+      if (lane < G::PANELS) tma_load_5d(sQ + lane * kQ * G::ROWB, &mq, &bar.q_full, lane * G::COLS, h0, i0, n * f.cq.n_mul, b * f.cq.b_mul);
+      __syncwarp();
+      for (; v_asked < T_; ++v_asked) {
+        const int t = v_asked, s = t % NS;
+        if (t >= NS) wait_or_flag(&bar.k_empty[s], (t / NS - 1) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        ask(sK + s * C::KB, &mk, &bar.k_full[s], t, f.ck);
+        ++k_asked;
+        if (t >= NS) wait_or_flag(&bar.v_empty[s], (t / NS - 1) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        ask(sV + s * C::KB, &mv, &bar.v_full[s], t, f.cv);
+      }
+      // none may land after this CTA has left
+      drain_ring(&bar.q_full, 1, 1); drain_ring(bar.k_full, k_asked, NS); drain_ring(bar.v_full, v_asked, NS);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------------------------------------ products
     const uint32_t id_s = idesc_f16(128, kK, f.fmt, 0, 0), id_o = idesc_f16(128, DP, f.fmt, 0, 1);
     const uint32_t q_lo = desc_lo(smem_u32(sQ), 16);
-    const bool leader = elect_one();
-    int k_asked = 0, v_asked = 0;
-    auto ask_k = [&](int upto) {
-      for (; k_asked < upto && k_asked < T_; ++k_asked) {
-        uint64_t* full = &bar.k_full[k_asked % NS];
-        if (leader) {
-          mbar_expect_tx(full, C::KB);
-          load_tile_tma<DP>(sK + k_asked % NS * C::KB, &mk, full, kK, hk, tiles.at(first + k_asked) * kK, n * f.ck.n_mul, b * f.ck.b_mul);
-        }
-      }
-      __syncwarp();
-    };
-    auto ask_v = [&](int upto) {
-      for (; v_asked < upto && v_asked < T_; ++v_asked) {
-        uint64_t* full = &bar.v_full[v_asked % NS];
-        if (leader) {
-          mbar_expect_tx(full, C::KB);
-          load_tile_tma<DP>(sV + v_asked % NS * C::KB, &mv, full, kK, hk, tiles.at(first + v_asked) * kK, n * f.cv.n_mul, b * f.cv.b_mul);
-        }
-      }
-      __syncwarp();
-    };
     auto scores = [&](int t) {                    // false: given up
       const int s = t % NS;
       wait_or_flag(&bar.k_full[s], (t / NS) & 1, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag)) return false;
       tc_fence_after();
-      const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16), d = t0 + (t % NB) * 64;
+      const uint32_t k_lo = desc_lo(smem_u32(sK + s * C::KB), 16), d = t0 + t % NB * 64;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) mma_ss_el(d, q_lo + k_step<DP>(ks, kQ), G::HI, k_lo + k_step<DP>(ks, kK), G::HI, id_s, ks > 0);
       tc_commit_el(&bar.s_ready[t % NB]);
+      tc_commit_el(&bar.k_empty[s]);
       return true;
     };
     if (T_ > 0) {
-      if (leader) {
-        mbar_expect_tx(&bar.q_full, f.q_bytes);
-        load_tile_tma<DP>(sQ, &mq, &bar.q_full, kQ, h0, i0, n * f.cq.n_mul, b * f.cq.b_mul);
-      }
-      ask_k(NS);
-      ask_v(NS);
       wait_or_flag(&bar.q_full, 0, abort_flag);
       bool ok = true;
       for (int t = 0; ok && t < NB && t < T_; ++t) ok = scores(t);
@@ -142,26 +148,21 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         const int s = t % NS;
         wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);
         wait_or_flag(&bar.p_ready[t % NB], (t / NB) & 1, abort_flag);
-        if (NB > 1 && t > 0) wait_or_flag(&bar.pv_done, (t - 1) & 1, abort_flag);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
         tc_fence_after();
-        const uint32_t v_lo = desc_lo(smem_u32(sV + s * C::KB), kK * G::ROWB), a = t0 + (t % NB) * 64;
+        const uint32_t v_lo = desc_lo(smem_u32(sV + s * C::KB), kK * G::ROWB), a = t0 + t % NB * 64;
 #pragma unroll
-        for (int ks = 0; ks < kK / 16; ++ks) mma_ts_el(tO, a + ks * 8, v_lo + ks * (16 * G::ROWB / 16), G::HI, id_o, t > 0 || ks > 0);
+        for (int ks = 0; ks < kK / 16; ++ks)      // each half of the columns keeps its P where its scores were
+          mma_ts_el(tO, a + ks / 2 * 32 + ks % 2 * 8, v_lo + ks * (16 * G::ROWB / 16), G::HI, id_o, t > 0 || ks > 0);
         tc_commit_el(&bar.pv_done);
-        if (NB > 1 && NS == NB) ask_k(t + 1 + NS);             // S(t + NB) needs the stage that S(t) has left
+        tc_commit_el(&bar.v_empty[s]);
         if (t + NB < T_) ok = scores(t + NB);
-        ask_k(t + 1 + NS);
-        ask_v(t + NS);
       }
     }
-    // none may land after this CTA has left
-    if (leader && T_ > 0) { drain_ring(&bar.q_full, 1, 1); drain_ring(bar.k_full, k_asked, NS); drain_ring(bar.v_full, v_asked, NS); }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const int r = warp * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
     const bool live = l_ < nq && i < p.Lq, any_live = __any_sync(0xffffffffu, live);       // a warp without rows (a few queries) only takes part
     const uint8_t* mask = p.mask ? p.mask + b * p.ms[0] + n * p.ms[1] : nullptr;
     auto mask_bytes = [&](int t, uint32_t (&mb)[2]) {
@@ -179,32 +180,30 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         if (t + 1 < T_) mask_bytes(t + 1, mb);
       }
       wait_or_flag(&bar.s_ready[t % NB], (t / NB) & 1, abort_flag);
-      if (__any_sync(0xffffffffu, *abort_flag)) break;
       tc_fence_after();
-      const uint32_t tS = t0 + lanes + (t % NB) * 64;
+      const uint32_t tS = t0 + lanes + t % NB * 64 + half * 32;
       const bool whole = all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + kK) && (keep[0] & keep[1]) == ~0u;
-      float corr = 1.f;
+      uint32_t s[32];
+      tmem_ld32(tS, s);
+      tmem_ld_wait();
+      pin32(s);
+      float corr = 1.f, mx = m;
       if (any_live) {
-        const uint32_t bits[2] = {whole ? ~0u : seen32(p, at, j0) & keep[0], whole ? ~0u : seen32(p, at, j0 + 32) & keep[1]};
-        auto hide = [&](uint32_t (&s)[32], uint32_t b) {
-          if (!whole) {
+        if (!whole) {
+          const uint32_t bits = seen32(p, at, j0 + half * 32) & (half ? keep[1] : keep[0]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(b >> e & 1)) s[e] = 0xff800000u;
-          }
-        };
-        uint32_t s[32];
+          for (int e = 0; e < 32; ++e)
+            if (!(bits >> e & 1)) s[e] = 0xff800000u;
+        }
         float m4[4] = {m, m, m, m};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {             // the scores are read twice: 64 of them do not fit beside the rest
-          tmem_ld32(tS + c * 32, s);
-          tmem_ld_wait();
-          pin32(s);
-          hide(s, bits[c]);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) m4[e / 2 % 4] = max3f(m4[e / 2 % 4], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-        }
-        const float mx = fmaxf(max3f(m4[0], m4[1], m4[2]), m4[3]);
+        for (int e = 0; e < 32; e += 2) m4[e / 2 % 4] = max3f(m4[e / 2 % 4], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        mx = fmaxf(max3f(m4[0], m4[1], m4[2]), m4[3]);
+      }
+      other[t & 1][half][r] = mx;
+      if (named_sync_or(1 + (warp & 3), 64, *abort_flag)) break;          // the two warps of these rows, which leave together
+      if (any_live) {
+        mx = fmaxf(mx, other[t & 1][half ^ 1][r]);
         if ((mx - m) * f.c1 > 8.f) {              // also from -inf
           corr = ex2f((m - mx) * f.c1);
           m = mx;
@@ -213,22 +212,15 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         const float off = m == -INFINITY ? 0.f : -m * f.c1;     // nothing seen so far: every logit is -inf
         const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tmem_ld32(tS + c * 32, s);
-          tmem_ld_wait();
-          pin32(s);
-          hide(s, bits[c]);
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
-            const float2 pr = make_float2(ex2f(x.x), ex2f(x.y));
-            sum[e / 2 % 2] = add2(sum[e / 2 % 2], pr);
-            w[e / 2] = Pack2<T>::pack(pr.x, pr.y);
-          }
-          tmem_st16(tS + c * 16, w);              // over scores that have been read twice
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
+          const float2 pr = make_float2(ex2f(x.x), ex2f(x.y));
+          sum[e / 2 % 2] = add2(sum[e / 2 % 2], pr);
+          w[e / 2] = Pack2<T>::pack(pr.x, pr.y);
         }
+        tmem_st16(tS, w);
         const float2 s2 = add2(sum[0], sum[1]);
         l += s2.x + s2.y;
       }
@@ -238,7 +230,8 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         if (__any_sync(0xffffffffu, corr != 1.f)) {
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
+          for (int c = 0; c < DP / 32; ++c) {     // warps that share rows take alternate columns
+            if (c % 2 != half) continue;
             uint32_t o32[32];
             tmem_ld32(tO + lanes + c * 32, o32);
             tmem_ld_wait();
@@ -256,13 +249,13 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         if (z0 | z1) {
           const int s = t % NS;
           wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);
-          const int row = r >> 1;                 // two threads a row
+          const int row = tid / 4;                // four threads a row
           if ((row < 32 ? z0 >> row : z1 >> (row - 32)) & 1) {
-            uint8_t* at_row = sV + s * C::KB + row * G::ROWB + (r & 1) * (G::ROWB / 2);
+            uint8_t* at_row = sV + s * C::KB + row * G::ROWB + tid % 4 * (G::ROWB / 4);
 #pragma unroll
             for (int pn = 0; pn < G::PANELS; ++pn)
 #pragma unroll
-              for (int x = 0; x < G::ROWB / 32; ++x) *reinterpret_cast<uint4*>(at_row + pn * kK * G::ROWB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int x = 0; x < G::ROWB / 64; ++x) *reinterpret_cast<uint4*>(at_row + pn * kK * G::ROWB + x * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_async_smem();
         }
@@ -273,7 +266,9 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
     }
     if (T_ > 0) wait_or_flag(&bar.pv_done, (T_ - 1) & 1, abort_flag);
     tc_fence_after();
-    if (!__any_sync(0xffffffffu, *abort_flag)) {
+    other[T_ & 1][half][r] = l;                   // the last maxima were of the other parity
+    if (!named_sync_or(1 + (warp & 3), 64, *abort_flag)) {
+      l += other[T_ & 1][half ^ 1][r];
       const int64_t row = ((int64_t)bn * p.Lq + i) * p.H + h;
       const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m * f.c1 + lg2f(l)) * kLn2;
       if (f.sp.splits > 1) {
@@ -281,30 +276,31 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           if (c * 32 >= p.D) break;
+          if (c % 2 != half) continue;
           uint32_t o32[32];
           if (T_ > 0) { tmem_ld32(tO + lanes + c * 32, o32); tmem_ld_wait(); pin32(o32); }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (live && c * 32 + e < p.D) out[c * 32 + e] = T_ > 0 ? __uint_as_float(o32[e]) * inv : 0.f;
         }
-        if (live) f.sp.lse(part, row, p.D) = lse;
+        if (live && half == 0) f.sp.lse(part, row, p.D) = lse;
       } else {
         T* out = static_cast<T*>(p.o) + row * p.D;
         if (T_ > 0) {
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c)
-            if (c * 32 < p.D) store_rows_at<T>(tO + lanes + c * 32, inv, live ? out + c * 32 : nullptr, p.D - c * 32);
-        } else if (live) {
+            if (c % 2 == half && c * 32 < p.D) store_rows_at<T>(tO + lanes + c * 32, inv, live ? out + c * 32 : nullptr, p.D - c * 32);
+        } else if (live && half == 0) {
           for (int d = 0; d < p.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
         }
-        if (p.lse && live) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = lse;
+        if (p.lse && live && half == 0) p.lse[((int64_t)bn * p.H + h) * p.Lq + i] = lse;
       }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && abort_s) *reinterpret_cast<volatile int*>(f.status) = 1;
-  if (warp == 0) tmem_dealloc(t0, C::COLS);
+  if (warp == 0) tmem_dealloc(t0, kCols);
 }
 
 int tc_splits(const WinP& p) { return split_count<kQ, kK>(p, 2 * sm_count()); }
