@@ -10,10 +10,11 @@
 // in shared memory, a second kernel over the blocks.
 //
 // Bound: HBM; for single tokens latency.
-#include "common.cuh"
+#include "evo_tc_common.cuh"
 
 namespace mf {
 namespace {
+using tcx::add2; using tcx::fma2; using tcx::mul2; using tcx::sub2;
 
 constexpr int kThreads = 256;
 
@@ -72,52 +73,60 @@ __device__ __forceinline__ void load_unit(const T* row, int64_t sd, const Unit<V
     if (u.has_b) r.q = *reinterpret_cast<const Piece<T, V>*>(row + u.b);
   }
 }
-// x[0..V) and x[V..2V) hold the first and second elements of the V pairs (or the two pieces of an unturned unit)
+// The first and the second elements of a unit's V pairs (or the two pieces of an unturned unit), two to a register pair: packed fp32
+// arithmetic takes half the issue slots, which bound these kernels (V = 1: the second of each two is 0).
+template <int V> struct Vec {
+  static constexpr int P = (V + 1) / 2;
+  float2 a[P], b[P];
+};
+template <int V> __device__ __forceinline__ float get(const float2 (&x)[(V + 1) / 2], int e) { return e % 2 ? x[e / 2].y : x[e / 2].x; }
+template <int V> __device__ __forceinline__ void put(float2 (&x)[(V + 1) / 2], int e, float v) { if (e % 2) x[e / 2].y = v; else x[e / 2].x = v; }
 template <typename T, int V, bool IL>
-__device__ __forceinline__ void unpack_unit(const Raw<T, V>& r, float (&x)[2 * V]) {
+__device__ __forceinline__ void unpack_unit(const Raw<T, V>& r, Vec<V>& x) {
+  if constexpr (V == 1) x.a[0].y = x.b[0].y = 0.f;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     if constexpr (IL && V > 1) {
-      x[e] = to_f(2 * e < V ? r.p.v[2 * e] : r.q.v[2 * e - V]);
-      x[V + e] = to_f(2 * e + 1 < V ? r.p.v[2 * e + 1] : r.q.v[2 * e + 1 - V]);
+      put<V>(x.a, e, to_f(2 * e < V ? r.p.v[2 * e] : r.q.v[2 * e - V]));
+      put<V>(x.b, e, to_f(2 * e + 1 < V ? r.p.v[2 * e + 1] : r.q.v[2 * e + 1 - V]));
     } else {
-      x[e] = to_f(r.p.v[e]); x[V + e] = to_f(r.q.v[e]);
+      put<V>(x.a, e, to_f(r.p.v[e])); put<V>(x.b, e, to_f(r.q.v[e]));
     }
   }
 }
 template <typename T, int V, bool IL>
-__device__ __forceinline__ void store_unit(T* row, const Unit<V, IL>& u, const float (&x)[2 * V]) {
+__device__ __forceinline__ void store_unit(T* row, const Unit<V, IL>& u, const Vec<V>& x) {
   Piece<T, V> p, q;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     if constexpr (IL && V > 1) {
-      (2 * e < V ? p.v[2 * e] : q.v[2 * e - V]) = from_f<T>(x[e]);
-      (2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]) = from_f<T>(x[V + e]);
+      (2 * e < V ? p.v[2 * e] : q.v[2 * e - V]) = from_f<T>(get<V>(x.a, e));
+      (2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]) = from_f<T>(get<V>(x.b, e));
     } else {
-      p.v[e] = from_f<T>(x[e]); q.v[e] = from_f<T>(x[V + e]);
+      p.v[e] = from_f<T>(get<V>(x.a, e)); q.v[e] = from_f<T>(get<V>(x.b, e));
     }
   }
   if (u.has_a) *reinterpret_cast<Piece<T, V>*>(row + u.a) = p;
   if (u.has_b) *reinterpret_cast<Piece<T, V>*>(row + u.b) = q;
 }
-// index in a row of D elements of x[e] / of x[V + e]
+// index in a row of D elements of the e-th of the first / second elements
 template <int V, bool IL>
 __device__ __forceinline__ int element(const Unit<V, IL>& u, int e) {
   if constexpr (IL) { const int i = e < V ? 2 * e : 2 * (e - V) + 1; return u.a + i; }      // the pieces are adjacent
   else return e < V ? u.a + e : u.b + e - V;
 }
-
-// the weights of a unit from a row of fp32 in shared memory
+// the weights of a unit from a row of fp32 in shared memory (any number where there is no element: x is 0 there)
 template <int V, bool IL>
-__device__ __forceinline__ void load_weight(const float* w, const Unit<V, IL>& u, float (&out)[2 * V]) {
+__device__ __forceinline__ void load_weight(const float* w, const Unit<V, IL>& u, Vec<V>& out) {
+  const int a = u.has_a ? u.a : 0, b = u.has_b ? u.b : 0;
+  if constexpr (V == 1) out.a[0].y = out.b[0].y = 0.f;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int a = u.has_a ? u.a : 0, b = u.has_b ? u.b : 0;                          // where there is nothing x is 0
     if constexpr (IL && V > 1) {
-      out[e] = 2 * e < V ? w[a + 2 * e] : w[b + 2 * e - V];
-      out[V + e] = 2 * e + 1 < V ? w[a + 2 * e + 1] : w[b + 2 * e + 1 - V];
+      put<V>(out.a, e, 2 * e < V ? w[a + 2 * e] : w[b + 2 * e - V]);
+      put<V>(out.b, e, 2 * e + 1 < V ? w[a + 2 * e + 1] : w[b + 2 * e + 1 - V]);
     } else {
-      out[e] = w[a + e]; out[V + e] = w[b + e];
+      put<V>(out.a, e, w[a + e]); put<V>(out.b, e, w[b + e]);
     }
   }
 }
@@ -148,7 +157,8 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
     }
   }
   __syncthreads();
-  float dwq[BWD ? UPL : 1][2 * V] = {}, dwk[BWD ? UPL : 1][2 * V] = {};
+  constexpr int P = Vec<V>::P;
+  Vec<V> dwq[BWD ? UPL : 1] = {}, dwk[BWD ? UPL : 1] = {};
   const int64_t stride = (int64_t)gridDim.x * slots;
   for (int64_t t0 = (int64_t)blockIdx.x * slots; t0 < p.tokens; t0 += stride) {
     const int64_t tok = t0 + slot;
@@ -180,15 +190,17 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
       const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
       pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
     }
-    float cs[UPL][V], sn[UPL][V];
+    Vec<V> turn[UPL];                                          // a: cosines, b: sines
 #pragma unroll
     for (int k = 0; k < UPL; ++k) {
       const int u = lane + k * lpr;
       const bool turned = u < p.R / 2 / V;
 #pragma unroll
+      for (int e = 0; e < P; ++e) { turn[k].a[e] = make_float2(1.f, 1.f); turn[k].b[e] = make_float2(0.f, 0.f); }
+#pragma unroll
       for (int e = 0; e < V; ++e) {
-        cs[k][e] = 1.f; sn[k][e] = 0.f;
-        if (turned && live) turn_of(pos, p.inv_freq[u * V + e], sn[k][e], cs[k][e]);
+        float sn, cs;
+        if (turned && live) { turn_of(pos, p.inv_freq[u * V + e], sn, cs); put<V>(turn[k].a, e, cs); put<V>(turn[k].b, e, sn); }
       }
     }
     for (int g = g0; g < g1; ++g) {
@@ -196,58 +208,61 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
       const int h = is_q ? g : g - p.H;
       const int64_t out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
       const float* w = ws + (!p.qw ? 0 : !p.w_head ? (is_q ? 0 : p.D) : (g - g0) * p.D);
-      float x[UPL][2 * V], d[BWD ? UPL : 1][2 * V], ss = 0.f;
+      Vec<V> x[UPL], d[BWD ? UPL : 1];
+      float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < UPL; ++k) {
         unpack_unit<T, V, IL>(xr[k], x[k]);
         if constexpr (BWD) unpack_unit<T, V, IL>(dr[k], d[k]);
 #pragma unroll
-        for (int e = 0; e < 2 * V; ++e) ss = fmaf(x[k][e], x[k][e], ss);
+        for (int e = 0; e < P; ++e) ss2 = fma2(x[k].b[e], x[k].b[e], fma2(x[k].a[e], x[k].a[e], ss2));
       }
       if (g + 1 < g1) fetch(g + 1, xr, dr);
-      const float rstd = rsqrtf(fmaf(row_sum(ss, lpr), inv_d, p.eps));
+      const float rstd = rsqrtf(fmaf(row_sum(ss2.x + ss2.y, lpr), inv_d, p.eps));
+      const float2 rstd2 = make_float2(rstd, rstd);
       if constexpr (!BWD) {
         T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + out_at;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
           const Unit<V, IL> u = unit(k);
-          float wt[2 * V];
+          Vec<V> wt;
           load_weight<V, IL>(w, u, wt);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float y1 = x[k][e] * rstd * wt[e], y2 = x[k][V + e] * rstd * wt[V + e];
-            x[k][e] = y1 * cs[k][e] - y2 * sn[k][e];           // by 1 and 0 where nothing turns
-            x[k][V + e] = y2 * cs[k][e] + y1 * sn[k][e];
+          for (int e = 0; e < P; ++e) {
+            const float2 ya = mul2(mul2(x[k].a[e], rstd2), wt.a[e]), yb = mul2(mul2(x[k].b[e], rstd2), wt.b[e]), c = turn[k].a[e], s = turn[k].b[e];
+            x[k].a[e] = sub2(mul2(ya, c), mul2(yb, s));        // by 1 and 0 where nothing turns
+            x[k].b[e] = fma2(ya, s, mul2(yb, c));
           }
           store_unit<T, V, IL>(out, u, x[k]);
         }
       } else {
-        float dot = 0.f;
+        float2 dot2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          float wt[2 * V];
+          Vec<V> wt;
           load_weight<V, IL>(w, unit(k), wt);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float d1 = d[k][e], d2 = d[k][V + e];
-            d[k][e] = d1 * cs[k][e] + d2 * sn[k][e];
-            d[k][V + e] = d2 * cs[k][e] - d1 * sn[k][e];
-          }
-#pragma unroll
-          for (int e = 0; e < 2 * V; ++e) {
-            x[k][e] *= rstd;                                   // hat
-            const float t = d[k][e] * x[k][e];
-            if (is_q) dwq[k][e] += t; else dwk[k][e] += t;
-            d[k][e] *= wt[e];
-            dot = fmaf(d[k][e], x[k][e], dot);
+          for (int e = 0; e < P; ++e) {
+            const float2 c = turn[k].a[e], s = turn[k].b[e], da = d[k].a[e], db = d[k].b[e];
+            const float2 ga = fma2(db, s, mul2(da, c)), gb = sub2(mul2(db, c), mul2(da, s));
+            x[k].a[e] = mul2(x[k].a[e], rstd2); x[k].b[e] = mul2(x[k].b[e], rstd2);        // hat
+            const float2 ta = mul2(ga, x[k].a[e]), tb = mul2(gb, x[k].b[e]);
+            if (is_q) { dwq[k].a[e] = add2(dwq[k].a[e], ta); dwq[k].b[e] = add2(dwq[k].b[e], tb); }
+            else { dwk[k].a[e] = add2(dwk[k].a[e], ta); dwk[k].b[e] = add2(dwk[k].b[e], tb); }
+            dot2 = fma2(tb, wt.b[e], fma2(ta, wt.a[e], dot2));
+            d[k].a[e] = mul2(ga, wt.a[e]); d[k].b[e] = mul2(gb, wt.b[e]);
           }
         }
-        dot = row_sum(dot, lpr) * inv_d;
+        const float dot = row_sum(dot2.x + dot2.y, lpr) * -inv_d;
+        const float2 minus = make_float2(dot, dot);
         T* out = static_cast<T*>(is_q ? p.dq : p.dk) + out_at;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
 #pragma unroll
-          for (int e = 0; e < 2 * V; ++e) x[k][e] = rstd * fmaf(-x[k][e], dot, d[k][e]);
+          for (int e = 0; e < P; ++e) {
+            x[k].a[e] = mul2(rstd2, fma2(x[k].a[e], minus, d[k].a[e]));
+            x[k].b[e] = mul2(rstd2, fma2(x[k].b[e], minus, d[k].b[e]));
+          }
           store_unit<T, V, IL>(out, unit(k), x[k]);
         }
       }
@@ -266,7 +281,8 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) {
           const int i = element<V, IL>(u, e);
-          if (i < p.D && (u.turned || i >= p.R)) sum[slot * p.D + i] = which ? dwk[k][e] : dwq[k][e];
+          const Vec<V>& dw = which ? dwk[k] : dwq[k];
+          if (i < p.D && (u.turned || i >= p.R)) sum[slot * p.D + i] = e < V ? get<V>(dw.a, e) : get<V>(dw.b, e - V);
         }
       }
       __syncthreads();
