@@ -393,7 +393,9 @@ int mf_relpos_fwd(const mf_relpos_args* args, void* stream) {
   int r = check_relpos(*args); if (r) return r;
   MF_REQUIRE(args->weight && args->bias, MF_ERR_BAD_ARG, "weight and bias must not be NULL");
   r = check_device(); if (r) return r;
-  return relpos_fwd(*args, static_cast<cudaStream_t>(stream));
+  r = relpos_fwd(*args, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
 }
 
 size_t mf_relpos_bwd_workspace_bytes(const mf_relpos_args* args) { return args && check_relpos(*args) == MF_OK ? relpos_bwd_workspace(*args) : 0; }
@@ -405,7 +407,9 @@ int mf_relpos_bwd(const mf_relpos_args* args, void* stream) {
   MF_REQUIRE(args->d_bias && args->d_weight && float_dtype(args->dw_dtype), MF_ERR_BAD_ARG, "d_bias and d_weight must not be NULL, d_weight of a floating type");
   r = check_device(); if (r) return r;
   r = check_workspace(args->workspace, args->workspace_bytes, relpos_bwd_workspace(*args)); if (r) return r;
-  return relpos_bwd(*args, static_cast<cudaStream_t>(stream));
+  r = relpos_bwd(*args, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
 }
 
 int mf_qk_rotary_fwd(const mf_qk_rotary_args* args, void* stream) {
@@ -414,7 +418,9 @@ int mf_qk_rotary_fwd(const mf_qk_rotary_args* args, void* stream) {
   int r = check_qk_rotary(*args); if (r) return r;
   MF_REQUIRE(args->q_out && args->k_out, MF_ERR_BAD_ARG, "q_out and k_out must not be NULL");
   r = check_device(); if (r) return r;
-  return qk_rotary_fwd(*args, static_cast<cudaStream_t>(stream));
+  r = qk_rotary_fwd(*args, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
 }
 
 size_t mf_qk_rotary_bwd_workspace_bytes(const mf_qk_rotary_args* args) { return args && check_qk_rotary(*args) == MF_OK ? qk_rotary_bwd_workspace(*args) : 0; }
@@ -427,7 +433,9 @@ int mf_qk_rotary_bwd(const mf_qk_rotary_args* args, void* stream) {
   MF_REQUIRE(!args->q_weight == !args->dq_weight && !args->k_weight == !args->dk_weight, MF_ERR_BAD_ARG, "the weights' gradients are given with the weights");
   r = check_device(); if (r) return r;
   r = check_workspace(args->workspace, args->workspace_bytes, qk_rotary_bwd_workspace(*args)); if (r) return r;
-  return qk_rotary_bwd(*args, static_cast<cudaStream_t>(stream));
+  r = qk_rotary_bwd(*args, static_cast<cudaStream_t>(stream));
+  if (r == MF_OK) set_last_path("simt");
+  return r;
 }
 
 size_t mf_window_fwd_workspace_bytes(const mf_window_args* args) {

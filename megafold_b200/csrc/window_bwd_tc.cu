@@ -21,7 +21,8 @@
 // the next S is formed while the compute warps exponentiate (184 -> 168 us at 16384 tokens, 16 heads of 64, window 1024);
 // in the other one, where each barrier stands between two products, that cost more than it gave (199 -> 233).
 //
-// Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they are overwritten with zeros in shared memory.
+// Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they, and those that no query of the tile sees, are overwritten
+// with zeros in shared memory.
 // P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  Waits are bounded as in the forward.
 #include <type_traits>
 
@@ -361,6 +362,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
   const int bn = group / head_groups(p), h0 = (group - bn * head_groups(p)) * p.pack, n = bn % p.N, b = bn / p.N, hk = h0 / p.G;
   const int nq = queries_of<kRows>(p), i0 = qt * nq, i1 = i0 + nq < p.Lq ? i0 + nq : p.Lq;
   const KeyTiles tiles = key_tiles<kKB>(p, i0, i1);
+  const KeyRange range = key_range(p, i0, i1);
   // steps: the blocks of keys, or (f.two_walks) all of them for delta and then all of them for dQ
   const int blocks = tiles.count(), delta_steps = f.two_walks ? blocks : 0, T_ = delta_steps + blocks;
   auto key_block = [&](int t) { return tiles.at(t < blocks ? t : t - blocks) * kKB; };
@@ -515,9 +517,10 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
         w[e / 2] = Pack2<T>::pack(ds.x, ds.y);
       }
       tmem_st16(tD, w);
-      if (mask) {
-        // rows of masked keys of K, this warp set's 32 keys of the block (the keys beyond Lk are zeros already): S has been formed
-        const uint32_t z = ~keep & ones32(p.Lk - j0);
+      if (!whole) {
+        // rows of K of keys that are masked or that no query of the tile sees, this warp set's 32 keys of the block (the keys beyond Lk are
+        // zeros already): S has been formed
+        const uint32_t z = ~(keep & range32(range, j0)) & ones32(p.Lk - j0);
         if (z) {
           const int row = r >> 2;                 // four threads a row
           if (z >> row & 1) {

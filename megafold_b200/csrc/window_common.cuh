@@ -57,6 +57,17 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(const WinP& p, int i0, in
   if (t.front > t.w0) t.front = t.w0;
   return t;
 }
+// Keys that some query of [i0, i1) may see: [lo, hi) and [0, front).  The others in a tile are read as zeros: a cache may hold anything
+// where the window has passed.
+struct KeyRange { int lo, hi, front; };
+__host__ __device__ __forceinline__ KeyRange key_range(const WinP& p, int i0, int i1) {
+  KeyRange r;
+  r.hi = clamp_i(i1 + p.off + p.right, 0, p.Lk);
+  r.lo = clamp_i(i0 + p.off - p.left, 0, r.hi);
+  r.front = p.sinks < r.hi ? p.sinks : r.hi;
+  return r;
+}
+__device__ __forceinline__ bool in_range(const KeyRange& r, int j) { return j < r.hi && (j >= r.lo || j < r.front); }
 // Queries [lo, hi) that see a key of [j0, j1)
 __host__ __device__ __forceinline__ void query_range(const WinP& p, int j0, int j1, int& lo, int& hi) {
   lo = clamp_i(j0 - p.right - p.off, 0, p.Lq);

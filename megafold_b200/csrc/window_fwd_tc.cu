@@ -16,7 +16,7 @@
 // Bound: the exponentials, half of the time at 64 columns (16 a clock and SM), and the waits between a block's steps.
 //
 // Blocks that a row does not see whole go through a 64-bit mask a row (window, sinks, end of the keys, key mask); rows of V whose
-// key is masked are overwritten with zeros in shared memory, since 0 * NaN would reach the sum.  P is rounded to the
+// key is masked, or seen by no query of the tile, are overwritten with zeros in shared memory, since 0 * NaN would reach the sum.  P is rounded to the
 // operands' type (the matrix instruction's), its sum is of the unrounded fp32 values.
 //
 // All waits are bounded; on expiry the CTA leaves without touching its outputs and the host sees mf_async_status() != 0.
@@ -92,6 +92,7 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const int bn = group / head_groups(p), h0 = (group - bn * head_groups(p)) * p.pack, n = bn % p.N, b = bn / p.N, hk = h0 / p.G;
   const int nq = queries_of<kQ>(p), i0 = qt * nq, i1 = i0 + nq < p.Lq ? i0 + nq : p.Lq;
   const KeyTiles tiles = key_tiles<kK>(p, i0, i1);
+  const KeyRange range = key_range(p, i0, i1);
   const int first = (int)((int64_t)tiles.count() * part / f.sp.splits), T_ = (int)((int64_t)tiles.count() * (part + 1) / f.sp.splits) - first;
 
   if (warp == 8) {
@@ -100,7 +101,6 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
     // S(t) has left the stage of K(t) one product before V(t) is done with.
     const bool leader = elect_one();
     auto ask = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* full, int t, const Coords& c) {
-      if (leader) mbar_expect_tx(full, C::KB);
       __syncwarp();
       if (lane < G::PANELS) tma_load_5d(dst + lane * kK * G::ROWB, m, full, lane * G::COLS, hk, tiles.at(first + t) * kK, n * c.n_mul, b * c.b_mul);
       __syncwarp();
@@ -115,10 +115,12 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         const int t = v_asked, s = t % NS;
         if (t >= NS) wait_or_flag(&bar.k_empty[s], (t / NS - 1) & 1, abort_flag);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
+        if (leader) mbar_expect_tx(&bar.k_full[s], C::KB);
         ask(sK + s * C::KB, &mk, &bar.k_full[s], t, f.ck);
         ++k_asked;
         if (t >= NS) wait_or_flag(&bar.v_empty[s], (t / NS - 1) & 1, abort_flag);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
+        if (leader) mbar_expect_tx(&bar.v_full[s], C::KB);
         ask(sV + s * C::KB, &mv, &bar.v_full[s], t, f.cv);
       }
       // none may land after this CTA has left
@@ -242,10 +244,10 @@ window_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           }
         }
       }
-      if (mask) {
-        // masked keys' rows of V (the keys beyond Lk are zeros already)
+      if (!whole) {
+        // rows of V of keys that are masked or that no query of the tile sees (the keys beyond Lk are zeros already)
         const int left = p.Lk - j0;
-        const uint32_t z0 = ~keep[0] & ones32(left), z1 = ~keep[1] & ones32(left - 32);
+        const uint32_t z0 = ~(keep[0] & range32(range, j0)) & ones32(left), z1 = ~(keep[1] & range32(range, j0 + 32)) & ones32(left - 32);
         if (z0 | z1) {
           const int s = t % NS;
           wait_or_flag(&bar.v_full[s], (t / NS) & 1, abort_flag);

@@ -6,7 +6,7 @@
 // dQ per 64 rows of queries, and dK / dV per 64 keys and chunk of their list of query blocks.  Nothing is added atomically: every
 // result is a sum in a fixed order.  Bound: FP32 issue (66 % of it goes to the multiply-adds).
 //
-// Masked keys are read as zeros: whatever their rows hold (NaN, too) reaches nothing.  A row that sees no key gives 0, and a
+// Masked keys, and those of a tile that none of its queries sees, are read as zeros: whatever their rows hold (NaN, too) reaches nothing.  A row that sees no key gives 0, and a
 // log-sum-exp of -inf, and passes no gradient.
 #include "simt_tiles.cuh"
 #include "window_common.cuh"
@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
   const int part = blockIdx.x % sp.splits, i0 = blockIdx.x / sp.splits * queries_of<kTile>(p);
   const int i1 = i0 + queries_of<kTile>(p) < p.Lq ? i0 + queries_of<kTile>(p) : p.Lq;
   load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
-  const auto keep = [&](int j) { return kept(p, b, n, j); };
+  const KeyRange range = key_range(p, i0, i1);
+  const auto keep = [&](int j) { return in_range(range, j) && kept(p, b, n, j); };
   float acc[4][DP / 16], m[4], l[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
@@ -246,7 +247,8 @@ __device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h
   load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
   const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
   load_queries<T, DP>(Gs, p.d_o, gs, p.g_vec, p, b, n, i0, h0);
-  const auto keep = [&](int j) { return kept(p, b, n, j); };
+  const KeyRange range = key_range(p, i0, i1);
+  const auto keep = [&](int j) { return in_range(range, j) && kept(p, b, n, j); };
   float dq[4][DP / 16] = {}, lse[4], dl[4];
   int at[4];
 #pragma unroll

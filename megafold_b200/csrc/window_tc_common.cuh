@@ -58,6 +58,8 @@ __device__ __forceinline__ uint32_t seen32(const WinP& p, int at, int j0) {
   if (hi > p.Lk - j0) hi = p.Lk - j0;
   return ones32(hi) & (~ones32(at - p.left - j0) | ones32(p.sinks - j0));
 }
+// Bits of the 32 keys from j0 that are in a range
+__device__ __forceinline__ uint32_t range32(const KeyRange& r, int j0) { return ones32(r.hi - j0) & (~ones32(r.lo - j0) | ones32(r.front - j0)); }
 // Does every query of positions [at0, at1] see every key of [j0, j1)?  (the mask aside)
 __device__ __forceinline__ bool all_seen(const WinP& p, int at0, int at1, int j0, int j1) {
   return j1 <= p.Lk && j1 - 1 <= at0 + p.right && (j0 >= at1 - p.left || j1 <= p.sinks);

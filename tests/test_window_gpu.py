@@ -212,3 +212,38 @@ def test_refusals():
         mfb.window_attention_backward(o[:, :, :2], q, k, k, o, lse, 2)
     with pytest.raises(ValueError):
         mfb.window_attention_backward(o, q, k, k, o, lse[..., :2], 2)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [FP, BF, HF])
+@pytest.mark.parametrize("Lq,Lk,left,sinks", [(1, 700, 100, 4), (90, 1000, 70, 5), (3, 300, 31, 0), (64, 700, 1, 1)])
+def test_keys_that_the_window_has_passed_may_hold_anything(Lq, Lk, left, sinks, dt):
+    q, k, v, m, d_o = _inputs(1, 2, Lq, Lk, 4, 2, 64, "drop", dt)
+    gone = slice(sinks, Lk - Lq - left)
+    ref = orc.window(q, k, v, left, 0, sinks, m, d_o, u=torch.finfo(dt).eps / 2)
+    k[:, :, gone], v[:, :, gone] = float("nan"), float("inf")
+    c = [t.cuda() for t in (q, k, v, m, d_o)]
+    o, lse = mfb.window_attention_forward(*c[:3], left, 0, sinks, c[3])
+    _check(o, ref, "o")
+    _check(lse, ref, "lse")
+    for name, x in zip(("dq", "dk", "dv"), mfb.window_attention_backward(c[4], *c[:3], o, lse, left, 0, sinks, c[3])):
+        _check(x, ref, name)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^31 elements, of which the last query sees the end and the first keys."""
+    Lk, Hk, D, left, sinks = 2_200_003, 8, 128, 300, 5
+    if torch.cuda.mem_get_info()[0] < 14e9:
+        pytest.skip("needs 14 GB")
+    q, k, v, _, d_o = _inputs(1, 1, 2, left + 2 + sinks, 16, Hk, D, "none", BF)
+    ref = orc.window(q, k, v, left, 0, sinks, None, u=2.0 ** -8)
+    big = [torch.full((1, 1, Lk, Hk, D), float("nan"), dtype=BF, device="cuda") for _ in range(2)]
+    for b, t in zip(big, (k, v)):
+        b[:, :, :sinks], b[:, :, sinks - t.shape[2]:] = t[:, :, :sinks].cuda(), t[:, :, sinks:].cuda()
+    o, lse = mfb.window_attention_forward(q.cuda(), *big, left, 0, sinks)
+    _check(o, ref, "o")
+    _check(lse, ref, "lse")
+    small = mfb.window_attention_forward(q.cuda(), k.cuda(), v.cuda(), left, 0, sinks)
+    # the same keys in other tiles: both within the bounds of the definition
+    _check(small[0], ref, "o")
