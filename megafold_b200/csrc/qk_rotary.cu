@@ -5,9 +5,9 @@
 //
 // A head's row is a few threads, each with V pairs: two pieces of V elements that turn together (R / 2 apart, or adjacent where
 // pairs are interleaved), so that nothing but the sum of squares crosses threads.  Angles are formed and
-// reduced in 64 bits (a position of a million times a frequency in 32 bits is off by 0.06); a thread computes its V angles once for all heads of its token that it goes through.  Sums and norms are
-// fp32, the outputs are rounded once.  The weights' gradients are summed in a fixed order: a thread over its tokens, a block over its threads
-// in shared memory, a second kernel over the blocks.
+// reduced in 64 bits (a position of a million times a frequency in 32 bits is off by 0.06), once a token and block.  Sums and norms are
+// fp32, the outputs are rounded once.  The weights' gradients are summed in a fixed order: a thread over its tokens, a block over its
+// threads in shared memory, a second kernel over the blocks.
 //
 // Bound: HBM; for single tokens latency.
 #include "evo_tc_common.cuh"
@@ -26,11 +26,11 @@ struct RotP {
   const float* inv_freq;
   const void* pos; int64_t ps[3]; bool pos64;            // NULL: the index along L
   float eps;
-  int heads_per;                            // heads that a thread goes through
+  int hb, tb, mt;                           // a block's heads, its tokens at a time and its tokens in a chunk
   int log_lpr;                              // threads of a row
   void *q_out, *k_out;                      // contiguous
   const void *dq_out, *dk_out; void *dq, *dk;
-  float* parts;                             // [gridDim.y][gridDim.x][2][D]
+  float* parts;                             // sums of the blocks, for the weights' gradients
 };
 
 // Sine and cosine of pos * f, in half turns: the whole quarters are taken off in 64 bits, exactly but for the one rounding of the
@@ -45,8 +45,6 @@ __device__ __forceinline__ void turn_of(double pos, float f, float& s, float& c)
   c = quarter == 1 || quarter == 2 ? -c1 : c1;
 }
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Piece { T v[V]; };
-
 // A thread's unit u of a row: V pairs, or, behind the rotated part, up to 2 V elements that are not turned.
 template <int V, bool IL>
 struct Unit {
@@ -59,22 +57,44 @@ struct Unit {
     else { a = R + 2 * V * (u - nr); b = a + V; has_a = a < D; has_b = b < D; }
   }
 };
-// the two pieces of a unit as they are in memory
-template <typename T, int V> struct Raw { Piece<T, V> p, q; };
+// The two pieces of a unit as they are in memory, in 32-bit words (arrays of 16-bit elements went through local memory).
+template <typename T, int V> struct Raw {
+  static constexpr int B = sizeof(T) * V, W = (B + 3) / 4;
+  uint32_t p[W], q[W];
+};
+template <int B>
+__device__ __forceinline__ void load_words(const void* at, uint32_t (&w)[(B + 3) / 4]) {
+  if constexpr (B == 16) { const uint4 v = *static_cast<const uint4*>(at); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+  else if constexpr (B == 8) { const uint2 v = *static_cast<const uint2*>(at); w[0] = v.x; w[1] = v.y; }
+  else if constexpr (B == 4) w[0] = *static_cast<const uint32_t*>(at);
+  else w[0] = *static_cast<const uint16_t*>(at);
+}
+template <int B>
+__device__ __forceinline__ void store_words(void* at, const uint32_t (&w)[(B + 3) / 4]) {
+  if constexpr (B == 16) *static_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (B == 8) *static_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+  else if constexpr (B == 4) *static_cast<uint32_t*>(at) = w[0];
+  else *static_cast<uint16_t*>(at) = (uint16_t)w[0];
+}
 template <typename T, int V, bool IL>
 __device__ __forceinline__ void load_unit(const T* row, int64_t sd, const Unit<V, IL>& u, Raw<T, V>& r) {
-  if constexpr (V == 1) {
-    r.p.v[0] = u.has_a ? row[u.a * sd] : from_f<T>(0.f);
-    r.q.v[0] = u.has_b ? row[u.b * sd] : from_f<T>(0.f);
-  } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) r.p.v[e] = r.q.v[e] = from_f<T>(0.f);
-    if (u.has_a) r.p = *reinterpret_cast<const Piece<T, V>*>(row + u.a);
-    if (u.has_b) r.q = *reinterpret_cast<const Piece<T, V>*>(row + u.b);
-  }
+  for (int e = 0; e < Raw<T, V>::W; ++e) r.p[e] = r.q[e] = 0u;
+  if (u.has_a) load_words<Raw<T, V>::B>(row + (V == 1 ? u.a * sd : u.a), r.p);
+  if (u.has_b) load_words<Raw<T, V>::B>(row + (V == 1 ? u.b * sd : u.b), r.q);
 }
+// element pair k (elements 2 k and 2 k + 1; of a single element the first) of a piece
+template <typename T, int V> __device__ __forceinline__ float2 pair_of(const uint32_t (&w)[Raw<T, V>::W], int k) {
+  if constexpr (sizeof(T) == 2) { const float2 v = tcx::Pack2<T>::unpack(w[k]); return V == 1 ? make_float2(v.x, 0.f) : v; }
+  else return make_float2(__uint_as_float(w[2 * k]), V == 1 ? 0.f : __uint_as_float(w[(2 * k + 1) % Raw<T, V>::W]));
+}
+template <typename T, int V> __device__ __forceinline__ void set_pair(uint32_t (&w)[Raw<T, V>::W], int k, float2 v) {
+  if constexpr (sizeof(T) == 2) w[k] = tcx::Pack2<T>::pack(v.x, v.y);
+  else { w[2 * k] = __float_as_uint(v.x); if (V > 1) w[(2 * k + 1) % Raw<T, V>::W] = __float_as_uint(v.y); }
+}
+
 // The first and the second elements of a unit's V pairs (or the two pieces of an unturned unit), two to a register pair: packed fp32
-// arithmetic takes half the issue slots, which bound these kernels (V = 1: the second of each two is 0).
+// arithmetic takes half the issue slots (V = 1: the second of each two is 0).
 template <int V> struct Vec {
   static constexpr int P = (V + 1) / 2;
   float2 a[P], b[P];
@@ -83,31 +103,33 @@ template <int V> __device__ __forceinline__ float get(const float2 (&x)[(V + 1) 
 template <int V> __device__ __forceinline__ void put(float2 (&x)[(V + 1) / 2], int e, float v) { if (e % 2) x[e / 2].y = v; else x[e / 2].x = v; }
 template <typename T, int V, bool IL>
 __device__ __forceinline__ void unpack_unit(const Raw<T, V>& r, Vec<V>& x) {
-  if constexpr (V == 1) x.a[0].y = x.b[0].y = 0.f;
+  constexpr int P = Vec<V>::P;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if constexpr (IL && V > 1) {
-      put<V>(x.a, e, to_f(2 * e < V ? r.p.v[2 * e] : r.q.v[2 * e - V]));
-      put<V>(x.b, e, to_f(2 * e + 1 < V ? r.p.v[2 * e + 1] : r.q.v[2 * e + 1 - V]));
+  for (int k = 0; k < P; ++k) {
+    const float2 p = pair_of<T, V>(r.p, k), q = pair_of<T, V>(r.q, k);
+    if constexpr (IL && V > 1) {                 // a pair of memory is a first and a second element
+      put<V>(x.a, k, p.x); put<V>(x.b, k, p.y);
+      put<V>(x.a, P + k, q.x); put<V>(x.b, P + k, q.y);
     } else {
-      put<V>(x.a, e, to_f(r.p.v[e])); put<V>(x.b, e, to_f(r.q.v[e]));
+      x.a[k] = p; x.b[k] = q;
     }
   }
 }
 template <typename T, int V, bool IL>
 __device__ __forceinline__ void store_unit(T* row, const Unit<V, IL>& u, const Vec<V>& x) {
-  Piece<T, V> p, q;
+  constexpr int P = Vec<V>::P;
+  Raw<T, V> r;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
+  for (int k = 0; k < P; ++k) {
     if constexpr (IL && V > 1) {
-      (2 * e < V ? p.v[2 * e] : q.v[2 * e - V]) = from_f<T>(get<V>(x.a, e));
-      (2 * e + 1 < V ? p.v[2 * e + 1] : q.v[2 * e + 1 - V]) = from_f<T>(get<V>(x.b, e));
+      set_pair<T, V>(r.p, k, make_float2(get<V>(x.a, k), get<V>(x.b, k)));
+      set_pair<T, V>(r.q, k, make_float2(get<V>(x.a, P + k), get<V>(x.b, P + k)));
     } else {
-      p.v[e] = from_f<T>(get<V>(x.a, e)); q.v[e] = from_f<T>(get<V>(x.b, e));
+      set_pair<T, V>(r.p, k, x.a[k]); set_pair<T, V>(r.q, k, x.b[k]);
     }
   }
-  if (u.has_a) *reinterpret_cast<Piece<T, V>*>(row + u.a) = p;
-  if (u.has_b) *reinterpret_cast<Piece<T, V>*>(row + u.b) = q;
+  if (u.has_a) store_words<Raw<T, V>::B>(row + u.a, r.p);
+  if (u.has_b) store_words<Raw<T, V>::B>(row + u.b, r.q);
 }
 // index in a row of D elements of the e-th of the first / second elements
 template <int V, bool IL>
@@ -115,99 +137,101 @@ __device__ __forceinline__ int element(const Unit<V, IL>& u, int e) {
   if constexpr (IL) { const int i = e < V ? 2 * e : 2 * (e - V) + 1; return u.a + i; }      // the pieces are adjacent
   else return e < V ? u.a + e : u.b + e - V;
 }
-// the weights of a unit from a row of fp32 in shared memory (any number where there is no element: x is 0 there)
-template <int V, bool IL>
-__device__ __forceinline__ void load_weight(const float* w, const Unit<V, IL>& u, Vec<V>& out) {
-  const int a = u.has_a ? u.a : 0, b = u.has_b ? u.b : 0;
-  if constexpr (V == 1) out.a[0].y = out.b[0].y = 0.f;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if constexpr (IL && V > 1) {
-      put<V>(out.a, e, 2 * e < V ? w[a + 2 * e] : w[b + 2 * e - V]);
-      put<V>(out.b, e, 2 * e + 1 < V ? w[a + 2 * e + 1] : w[b + 2 * e + 1 - V]);
-    } else {
-      put<V>(out.a, e, w[a + e]); put<V>(out.b, e, w[b + e]);
-    }
-  }
-}
 __device__ __forceinline__ float row_sum(float v, int lpr) {
   for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// blockIdx.y = group of heads_per heads (of the H + Hk of queries and keys); threads of a block walk tokens.
-// UPL: units of a thread.  (Every thread of a warp takes part in each sum: rows that do not exist are zeros.)
-// The weights of the block's heads wait in shared memory as fp32: read from global memory for each row, converted from a type known
-// at run time, they were most of the instructions (4 + 4 heads of 32, 147456 tokens: 96 us forward, 220 backward).
+// A block takes `hb` heads (blockIdx.y; of the H + Hk of queries and keys) of `tb` tokens at a time and walks the tokens: the threads of a token's
+// heads are neighbours, so that a warp reads and writes whole lines, and a thread keeps to its head, whose weights and whose sums of
+// the weights' gradients stay in registers.  The angles of the next tokens are formed by all threads together, `mt` tokens (a
+// multiple of tb) ahead, in shared memory.  (With a thread going through all heads of its token instead, each load touched as many
+// lines as the warp had tokens: 4 + 4 heads of 32, 147456 tokens: 48 us forward, 108 backward.)
+// UPL: units of a thread.  Every thread of a warp takes part in each sum over a row: rows that do not exist are zeros.
 template <typename T, int V, int UPL, bool IL, bool BWD>
 __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary_kernel(const __grid_constant__ RotP p) {
-  const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr, slots = kThreads >> p.log_lpr;
-  const int heads = p.H + p.Hk, g0 = blockIdx.y * p.heads_per, g1 = g0 + p.heads_per < heads ? g0 + p.heads_per : heads;
+  constexpr int P = Vec<V>::P;
+  const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr;
+  const int heads = p.H + p.Hk, tslot = slot / p.hb, g = blockIdx.y * p.hb + slot - tslot * p.hb;
+  const bool head_ok = tslot < p.tb && g < heads, is_q = g < p.H;
+  const int h = is_q ? g : g - p.H, pairs = p.R / 2;
   const float inv_d = 1.f / p.D;
   extern __shared__ __align__(16) float shared[];
-  float* const ws = shared;                                    // [1 (no weights), 2 (shared: q, k) or heads of the group][D]
-  if (!p.qw) {
-    for (int x = threadIdx.x; x < p.D; x += kThreads) ws[x] = 1.f;
-  } else if (!p.w_head) {
-    for (int x = threadIdx.x; x < 2 * p.D; x += kThreads) ws[x] = x < p.D ? load_rt(p.qw, x, p.w_dtype) : load_rt(p.kw, x - p.D, p.w_dtype);
-  } else {
-    for (int x = threadIdx.x; x < (g1 - g0) * p.D; x += kThreads) {
-      const int64_t at = (int64_t)g0 * p.D + x, nq = (int64_t)p.H * p.D;
-      ws[x] = at < nq ? load_rt(p.qw, at, p.w_dtype) : load_rt(p.kw, at - nq, p.w_dtype);
+  float2* const angles = reinterpret_cast<float2*>(shared);    // [mt][pairs]: cosine, sine
+
+  Vec<V> wt[UPL], dw[BWD ? UPL : 1] = {};
+#pragma unroll
+  for (int k = 0; k < UPL; ++k) {
+    const Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+    const void* w = is_q ? p.qw : p.kw;
+    if constexpr (V == 1) wt[k].a[0].y = wt[k].b[0].y = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e) {
+      const int i = element<V, IL>(u, e);
+      const float x = !head_ok || i >= p.D ? 0.f : w ? load_rt(w, h * p.w_head + i, p.w_dtype) : 1.f;
+      if (e < V) put<V>(wt[k].a, e, x); else put<V>(wt[k].b, e - V, x);
     }
   }
-  __syncthreads();
-  constexpr int P = Vec<V>::P;
-  Vec<V> dwq[BWD ? UPL : 1] = {}, dwk[BWD ? UPL : 1] = {};
-  const int64_t stride = (int64_t)gridDim.x * slots;
-  for (int64_t t0 = (int64_t)blockIdx.x * slots; t0 < p.tokens; t0 += stride) {
-    const int64_t tok = t0 + slot;
-    const bool live = tok < p.tokens;
-    const uint32_t bn = live ? (uint32_t)tok / (uint32_t)p.L : 0, l = live ? (uint32_t)tok - bn * p.L : 0, b = bn / (uint32_t)p.N, n = bn - b * p.N;
-    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1] + l * p.qs[2];
-    const T* kk = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1] + l * p.ks[2];
-    auto unit = [&](int k) {
-      Unit<V, IL> u(lane + k * lpr, p.R, p.D);
-      u.has_a = u.has_a && live; u.has_b = u.has_b && live;
-      return u;
-    };
-    auto fetch = [&](int g, Raw<T, V> (&x)[UPL], Raw<T, V> (&d)[BWD ? UPL : 1]) {
-      const bool is_q = g < p.H;
-      const int h = is_q ? g : g - p.H;
-      const T* row = is_q ? q + h * p.qs[3] : kk + h * p.ks[3];
+  const int64_t qs3 = is_q ? p.qs[3] : p.ks[3], sd = is_q ? p.qs[4] : p.ks[4];
+  const int64_t sb = is_q ? p.qs[0] : p.ks[0], sn = is_q ? p.qs[1] : p.ks[1], sl = is_q ? p.qs[2] : p.ks[2];
+  const T* const in = static_cast<const T*>(is_q ? p.q : p.k) + h * qs3;
+  const int own = is_q ? p.H : p.Hk;                           // heads of a token in the contiguous arrays
+  const T* const din = BWD ? static_cast<const T*>(is_q ? p.dq_out : p.dk_out) + (int64_t)h * p.D : nullptr;
+  T* const out = static_cast<T*>(BWD ? (is_q ? p.dq : p.dk) : (is_q ? p.q_out : p.k_out)) + (int64_t)h * p.D;
+  auto unit = [&](int k, bool live) {
+    Unit<V, IL> u(lane + k * lpr, p.R, p.D);
+    u.has_a = u.has_a && live; u.has_b = u.has_b && live;
+    return u;
+  };
+  // a thread's place among the tokens: stepped along, and found by divisions only where a sequence ends
+  struct Place {
+    int64_t tok;
+    uint32_t l;
+    const T* row;
+  };
+  auto place = [&](int64_t tok) {
+    Place c;
+    const uint32_t t = head_ok && tok < p.tokens ? (uint32_t)tok : 0, bn = t / (uint32_t)p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
+    c.tok = tok; c.l = t - bn * p.L;
+    c.row = in + b * sb + n * sn + c.l * sl;
+    return c;
+  };
+  const int64_t row_step = p.tb * sl, arr_step = (int64_t)p.tb * own * p.D;
+  auto fetch = [&](const Place& c, const T* dp, bool live, Raw<T, V> (&x)[UPL], Raw<T, V> (&d)[BWD ? UPL : 1]) {
 #pragma unroll
-      for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(row, is_q ? p.qs[4] : p.ks[4], unit(k), x[k]);
-      if constexpr (BWD) {
-        const T* dr = static_cast<const T*>(is_q ? p.dq_out : p.dk_out) + (tok * (is_q ? p.H : p.Hk) + h) * p.D;
+    for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(c.row, sd, unit(k, live), x[k]);
+    if constexpr (BWD) {
 #pragma unroll
-        for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(dr, 1, unit(k), d[k]);
-      }
-    };
+      for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(dp, 1, unit(k, live), d[k]);
+    }
+  };
+  // this block's tokens: chunks of mt, gridDim.x apart
+  for (int64_t c0 = (int64_t)blockIdx.x * p.mt; c0 < p.tokens; c0 += (int64_t)gridDim.x * p.mt) {
+    const int64_t c1 = c0 + p.mt < p.tokens ? c0 + p.mt : p.tokens;
+    Place at = place(c0 + tslot);
+    bool live = head_ok && at.tok < c1;
     Raw<T, V> xr[UPL], dr[BWD ? UPL : 1];
-    fetch(g0, xr, dr);                                         // on its way while the angles are formed
-    double pos = (double)l;
-    if (p.pos) {
-      const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
-      pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
-    }
-    Vec<V> turn[UPL];                                          // a: cosines, b: sines
-#pragma unroll
-    for (int k = 0; k < UPL; ++k) {
-      const int u = lane + k * lpr;
-      const bool turned = u < p.R / 2 / V;
-#pragma unroll
-      for (int e = 0; e < P; ++e) { turn[k].a[e] = make_float2(1.f, 1.f); turn[k].b[e] = make_float2(0.f, 0.f); }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float sn, cs;
-        if (turned && live) { turn_of(pos, p.inv_freq[u * V + e], sn, cs); put<V>(turn[k].a, e, cs); put<V>(turn[k].b, e, sn); }
+    const int64_t arr = (live ? at.tok : 0) * own * p.D;
+    const T* dp = BWD ? din + arr : nullptr;
+    T* to = out + arr;
+    const float2* turns = angles + (live ? tslot : 0) * pairs;
+    fetch(at, dp, live, xr, dr);                               // on its way while the angles are formed
+    __syncthreads();                                           // the last chunk's angles have been read
+    for (int x = threadIdx.x; x < (int)(c1 - c0) * pairs; x += kThreads) {
+      const int i = x / pairs, f = x - i * pairs;
+      const uint32_t t = (uint32_t)(c0 + i), bn = t / (uint32_t)p.L, l = t - bn * p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
+      double pos = (double)l;
+      if (p.pos) {
+        const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
+        pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
       }
+      float2 a;
+      turn_of(pos, p.inv_freq[f], a.y, a.x);
+      angles[x] = a;
     }
-    for (int g = g0; g < g1; ++g) {
-      const bool is_q = g < p.H;
-      const int h = is_q ? g : g - p.H;
-      const int64_t out_at = (tok * (is_q ? p.H : p.Hk) + h) * p.D;
-      const float* w = ws + (!p.qw ? 0 : !p.w_head ? (is_q ? 0 : p.D) : (g - g0) * p.D);
+    __syncthreads();
+    // as many steps for every thread: the sums over rows take whole warps
+    for (int64_t t0 = c0; t0 < c1; t0 += p.tb) {
       Vec<V> x[UPL], d[BWD ? UPL : 1];
       float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -217,45 +241,52 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
 #pragma unroll
         for (int e = 0; e < P; ++e) ss2 = fma2(x[k].b[e], x[k].b[e], fma2(x[k].a[e], x[k].a[e], ss2));
       }
-      if (g + 1 < g1) fetch(g + 1, xr, dr);
+      const bool now = live;
+      at.tok += p.tb; at.l += p.tb; at.row += row_step;
+      if (BWD) dp += arr_step;
+      live = head_ok && at.tok < c1;
+      if (live && at.l >= (uint32_t)p.L) at = place(at.tok);
+      fetch(at, dp, live, xr, dr);
       const float rstd = rsqrtf(fmaf(row_sum(ss2.x + ss2.y, lpr), inv_d, p.eps));
       const float2 rstd2 = make_float2(rstd, rstd);
-      if constexpr (!BWD) {
-        T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + out_at;
+      float2 dot2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < UPL; ++k) {
-          const Unit<V, IL> u = unit(k);
-          Vec<V> wt;
-          load_weight<V, IL>(w, u, wt);
+      for (int k = 0; k < UPL; ++k) {
+        const Unit<V, IL> u = unit(k, now);
+        Vec<V> turn;                                           // a: cosines, b: sines; 1 and 0 where nothing turns
+#pragma unroll
+        for (int e = 0; e < P; ++e) { turn.a[e] = make_float2(1.f, 1.f); turn.b[e] = make_float2(0.f, 0.f); }
+        if (u.turned && now) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float2 t = turns[(lane + k * lpr) * V + e];
+            put<V>(turn.a, e, t.x); put<V>(turn.b, e, t.y);
+          }
+        }
+        if constexpr (!BWD) {
 #pragma unroll
           for (int e = 0; e < P; ++e) {
-            const float2 ya = mul2(mul2(x[k].a[e], rstd2), wt.a[e]), yb = mul2(mul2(x[k].b[e], rstd2), wt.b[e]), c = turn[k].a[e], s = turn[k].b[e];
-            x[k].a[e] = sub2(mul2(ya, c), mul2(yb, s));        // by 1 and 0 where nothing turns
+            const float2 ya = mul2(mul2(x[k].a[e], rstd2), wt[k].a[e]), yb = mul2(mul2(x[k].b[e], rstd2), wt[k].b[e]), c = turn.a[e], s = turn.b[e];
+            x[k].a[e] = sub2(mul2(ya, c), mul2(yb, s));
             x[k].b[e] = fma2(ya, s, mul2(yb, c));
           }
-          store_unit<T, V, IL>(out, u, x[k]);
-        }
-      } else {
-        float2 dot2 = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < UPL; ++k) {
-          Vec<V> wt;
-          load_weight<V, IL>(w, unit(k), wt);
+          store_unit<T, V, IL>(to, u, x[k]);
+        } else {
 #pragma unroll
           for (int e = 0; e < P; ++e) {
-            const float2 c = turn[k].a[e], s = turn[k].b[e], da = d[k].a[e], db = d[k].b[e];
+            const float2 c = turn.a[e], s = turn.b[e], da = d[k].a[e], db = d[k].b[e];
             const float2 ga = fma2(db, s, mul2(da, c)), gb = sub2(mul2(db, c), mul2(da, s));
             x[k].a[e] = mul2(x[k].a[e], rstd2); x[k].b[e] = mul2(x[k].b[e], rstd2);        // hat
             const float2 ta = mul2(ga, x[k].a[e]), tb = mul2(gb, x[k].b[e]);
-            if (is_q) { dwq[k].a[e] = add2(dwq[k].a[e], ta); dwq[k].b[e] = add2(dwq[k].b[e], tb); }
-            else { dwk[k].a[e] = add2(dwk[k].a[e], ta); dwk[k].b[e] = add2(dwk[k].b[e], tb); }
-            dot2 = fma2(tb, wt.b[e], fma2(ta, wt.a[e], dot2));
-            d[k].a[e] = mul2(ga, wt.a[e]); d[k].b[e] = mul2(gb, wt.b[e]);
+            dw[k].a[e] = add2(dw[k].a[e], ta); dw[k].b[e] = add2(dw[k].b[e], tb);
+            dot2 = fma2(tb, wt[k].b[e], fma2(ta, wt[k].a[e], dot2));
+            d[k].a[e] = mul2(ga, wt[k].a[e]); d[k].b[e] = mul2(gb, wt[k].b[e]);
           }
         }
+      }
+      if constexpr (BWD) {
         const float dot = row_sum(dot2.x + dot2.y, lpr) * -inv_d;
         const float2 minus = make_float2(dot, dot);
-        T* out = static_cast<T*>(is_q ? p.dq : p.dk) + out_at;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
 #pragma unroll
@@ -263,56 +294,66 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
             x[k].a[e] = mul2(rstd2, fma2(x[k].a[e], minus, d[k].a[e]));
             x[k].b[e] = mul2(rstd2, fma2(x[k].b[e], minus, d[k].b[e]));
           }
-          store_unit<T, V, IL>(out, unit(k), x[k]);
+          store_unit<T, V, IL>(to, unit(k, now), x[k]);
         }
       }
+      to += arr_step;
+      turns += p.tb * pairs;
     }
   }
   if constexpr (BWD) {
     if (!p.parts) return;
-    float* const sum = shared;                                 // [slots][D]
-    float* out = p.parts + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
+    float* const sum = shared;                                 // [token][head of the block][D]
+    __syncthreads();
+    if (head_ok) {
 #pragma unroll
       for (int k = 0; k < UPL; ++k) {
         const Unit<V, IL> u(lane + k * lpr, p.R, p.D);
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) {
           const int i = element<V, IL>(u, e);
-          const Vec<V>& dw = which ? dwk[k] : dwq[k];
-          if (i < p.D && (u.turned || i >= p.R)) sum[slot * p.D + i] = e < V ? get<V>(dw.a, e) : get<V>(dw.b, e - V);
+          if (i < p.D && (u.turned || i >= p.R)) sum[slot * p.D + i] = e < V ? get<V>(dw[k].a, e) : get<V>(dw[k].b, e - V);
         }
       }
-      __syncthreads();
-      for (int i = threadIdx.x; i < p.D; i += kThreads) {
+    }
+    __syncthreads();
+    const int here = heads - (int)blockIdx.y * p.hb < p.hb ? heads - (int)blockIdx.y * p.hb : p.hb, q_here = p.H - (int)blockIdx.y * p.hb;
+    if (p.w_head) {                                            // a row a head: parts [gridDim.x][heads][D]
+      for (int x = threadIdx.x; x < here * p.D; x += kThreads) {
         float s = 0.f;
-        for (int k = 0; k < slots; ++k) s += sum[k * p.D + i];
-        out[which * p.D + i] = s;
+        for (int t = 0; t < p.tb; ++t) s += sum[t * p.hb * p.D + x];
+        p.parts[((int64_t)blockIdx.x * heads + blockIdx.y * p.hb) * p.D + x] = s;
+      }
+    } else {                                                   // queries and keys: parts [gridDim.y][gridDim.x][2][D]
+      for (int x = threadIdx.x; x < 2 * p.D; x += kThreads) {
+        const int which = x / p.D, i = x - which * p.D;
+        float s = 0.f;
+        for (int t = 0; t < p.tb; ++t)
+          for (int y = 0; y < here; ++y)
+            if ((y >= q_here) == which) s += sum[(t * p.hb + y) * p.D + i];
+        p.parts[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D + x] = s;
       }
     }
   }
 }
 
-// Weight gradients: blockIdx = (32 elements, row of [H or 1 + Hk or 1]); a row is the sum of its blocks' rows, 32 of them at a time.
-__global__ void __launch_bounds__(1024) qk_rotary_join_kernel(const float* __restrict__ parts, int gx, int gy, int D, int H, int Hk, bool per_head, void* __restrict__ dqw,
-                                                              void* __restrict__ dkw, int w_dtype) {
+// Weight gradients: blockIdx = (32 elements, row of [H or 1 + Hk or 1]); a row is the sum of `n` parts, `step` floats apart from `first`, 32
+// of them at a time.
+__global__ void __launch_bounds__(1024) qk_rotary_join_kernel(const float* __restrict__ parts, int n, int step, int D, int q_rows, void* __restrict__ dqw, void* __restrict__ dkw,
+                                                              int w_dtype) {
   __shared__ float sums[32][33];
-  const int q_rows = per_head ? H : 1, row = blockIdx.y, i = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-  const bool is_k = row >= q_rows;
-  const int64_t k0 = per_head ? (int64_t)row * gx : 0, k1 = per_head ? k0 + gx : (int64_t)gy * gx;        // per head: a group of blocks each, queries' heads first
+  const int row = blockIdx.y, i = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
   float s = 0.f;
   if (i < D) {
 #pragma unroll 8
-    for (int64_t k = k0 + warp; k < k1; k += 32) s += parts[(k * 2 + is_k) * D + i];
+    for (int k = warp; k < n; k += 32) s += parts[(int64_t)k * step + row * D + i];
   }
   sums[warp][threadIdx.x & 31] = s;
   __syncthreads();
   if (warp || i >= D) return;
   s = 0.f;
   for (int k = 0; k < 32; ++k) s += sums[k][threadIdx.x];
-  if (is_k) store_rt(dkw, (int64_t)(row - q_rows) * D + i, w_dtype, s);
+  if (row >= q_rows) store_rt(dkw, (int64_t)(row - q_rows) * D + i, w_dtype, s);
   else store_rt(dqw, (int64_t)row * D + i, w_dtype, s);
 }
 
@@ -329,13 +370,12 @@ RotP rot_params(const mf_qk_rotary_args& a) {
   return p;
 }
 
-// Elements of a piece: the widest load that sizes, strides and addresses allow, 16 bytes on the forward and 8 on the backward, where a
-// thread holds twice as much and the sums of the weights' gradients besides (with 16 bytes 176 registers, one block of
-// 256 threads on an SM).
-int piece_limit(int dtype, bool bwd) { return (bwd ? 8 : 16) / (int)dtype_size(dtype); }
+// Elements of a piece: the widest load that sizes, strides and addresses allow, 8 bytes at most (with 16 a thread holds twice as much, and
+// an SM half as many threads).
+int piece_limit(int dtype) { return 8 / (int)dtype_size(dtype); }
 int piece(const mf_qk_rotary_args& a, bool bwd) {
   const int es = (int)dtype_size(a.dtype);
-  for (int v = piece_limit(a.dtype, bwd); v > 1; v /= 2) {
+  for (int v = piece_limit(a.dtype); v > 1; v /= 2) {
     bool ok = a.R / 2 % v == 0 && (a.D - a.R) % v == 0 && a.q_strides[4] == 1 && a.k_strides[4] == 1;
     for (int i = 0; i < 4; ++i) ok = ok && a.q_strides[i] % v == 0 && a.k_strides[i] % v == 0;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (bwd ? (uintptr_t)a.dq_out | (uintptr_t)a.dk_out | (uintptr_t)a.dq | (uintptr_t)a.dk
@@ -346,63 +386,63 @@ int piece(const mf_qk_rotary_args& a, bool bwd) {
 }
 int units_per(int V) { return V >= 4 ? 1 : V == 2 ? 2 : 4; }
 
-struct Plan { int log_lpr, heads_per, gx, gy; };
+struct Plan { int log_lpr, hb, tb, mt, gx, gy; size_t smem; };
 Plan plan(const mf_qk_rotary_args& a, int V, bool bwd) {
   Plan c;
-  const int units = a.R / 2 / V + (a.D - a.R + 2 * V - 1) / (2 * V), lanes = (units + units_per(V) - 1) / units_per(V);
+  const int units = a.R / 2 / V + (a.D - a.R + 2 * V - 1) / (2 * V), lanes = (units + units_per(V) - 1) / units_per(V), heads = a.H + a.Hk;
   c.log_lpr = 0;
   while ((1 << c.log_lpr) < lanes) ++c.log_lpr;
-  const int slots = kThreads >> c.log_lpr, heads = a.H + a.Hk;
-  const int64_t tokens = (int64_t)a.B * a.N * a.L, blocks = (tokens + slots - 1) / slots, want = 8 * (int64_t)tcx::sm_count();
-  // every head of a token in one thread, which computes the angles once; fewer where that leaves processors idle, and one where
-  // each head has a weight of its own whose gradient a block sums
-  c.heads_per = heads;
-  if (bwd && a.per_head && a.dq_weight) c.heads_per = 1;
-  if (a.per_head && a.q_weight)
-    while (c.heads_per > 1 && (size_t)c.heads_per * a.D * sizeof(float) > 24 * 1024) c.heads_per = (c.heads_per + 1) / 2;
-  while (c.heads_per > 1 && blocks * ((heads + c.heads_per - 1) / c.heads_per) < want) c.heads_per = (c.heads_per + 1) / 2;
-  c.gy = (heads + c.heads_per - 1) / c.heads_per;
-  int64_t gx = blocks;
+  const int slots = kThreads >> c.log_lpr, pairs = a.R / 2;
+  const int64_t tokens = (int64_t)a.B * a.N * a.L, want = (bwd ? 3 : 8) * (int64_t)tcx::sm_count();
+  c.hb = heads < slots ? heads : slots;
+  c.gy = (heads + c.hb - 1) / c.hb;
+  c.hb = (heads + c.gy - 1) / c.gy;
+  c.tb = slots / c.hb;
+  // a chunk: some four angles a thread, less where that leaves processors idle, 16 KB of them at most
+  int steps = 4 * kThreads / (c.tb * (pairs > 0 ? pairs : 1));
+  if (steps < 1) steps = 1;
+  while (steps > 1 && (tokens + (int64_t)c.tb * steps - 1) / ((int64_t)c.tb * steps) * c.gy < want) steps /= 2;
+  while (steps * c.tb * pairs * 8 > 16 * 1024 && steps > 1) steps /= 2;
+  while (c.tb > 1 && c.tb * pairs * 8 > 32 * 1024) c.tb /= 2;
+  c.mt = c.tb * steps;
+  int64_t gx = (tokens + c.mt - 1) / c.mt;
   if (bwd) { const int64_t most = (want + c.gy - 1) / c.gy; if (gx > most) gx = most; }
-  if (gx > 0x7fffffff) gx = 0x7fffffff;
   c.gx = (int)gx;
+  c.smem = sizeof(float2) * (size_t)c.mt * pairs;
+  const size_t sums = bwd && a.dq_weight ? sizeof(float) * (size_t)c.tb * c.hb * a.D : 0;
+  if (sums > c.smem) c.smem = sums;
   return c;
 }
+size_t part_floats(const mf_qk_rotary_args& a, const Plan& c) { return (size_t)c.gx * a.D * (a.per_head ? a.H + a.Hk : 2 * c.gy); }
 
 template <typename T, int V, bool BWD>
 int run(const mf_qk_rotary_args& a, cudaStream_t st) {
   constexpr int UPL = V >= 4 ? 1 : V == 2 ? 2 : 4;
   RotP p = rot_params(a);
   const Plan c = plan(a, V, BWD);
-  p.log_lpr = c.log_lpr; p.heads_per = c.heads_per;
-  size_t smem = sizeof(float) * a.D * (!a.q_weight ? 1 : !a.per_head ? 2 : c.heads_per);
-  if (BWD && a.dq_weight) {
-    p.parts = static_cast<float*>(a.workspace);
-    const size_t sums = sizeof(float) * (kThreads >> c.log_lpr) * a.D;
-    if (sums > smem) smem = sums;
-  }
+  p.log_lpr = c.log_lpr; p.hb = c.hb; p.tb = c.tb; p.mt = c.mt;
+  const bool sums = BWD && a.dq_weight;
+  if (sums) p.parts = static_cast<float*>(a.workspace);
   const auto go = [&](auto il) -> int {
     constexpr auto kern = qk_rotary_kernel<T, V, UPL, decltype(il)::value, BWD>;
-    if (int e = opt_in_smem<kern>(smem)) return e;
-    kern<<<dim3(c.gx, c.gy), kThreads, smem, st>>>(p);
+    if (int e = opt_in_smem<kern>(c.smem)) return e;
+    kern<<<dim3(c.gx, c.gy), kThreads, c.smem, st>>>(p);
     MF_LAUNCHED("qk_rotary_kernel");
     return MF_OK;
   };
   if (int e = a.interleaved ? go(std::true_type{}) : go(std::false_type{})) return e;
-  if (BWD && a.dq_weight) {
+  if (sums) {
     const int rows = a.per_head ? a.H + a.Hk : 2;
-    qk_rotary_join_kernel<<<dim3((a.D + 31) / 32, rows), 1024, 0, st>>>(p.parts, c.gx, c.gy, a.D, a.H, a.Hk, a.per_head != 0, a.dq_weight, a.dk_weight,
-                                                                                                a.w_dtype);
+    qk_rotary_join_kernel<<<dim3((a.D + 31) / 32, rows), 1024, 0, st>>>(p.parts, a.per_head ? c.gx : c.gx * c.gy, rows * a.D, a.D, a.per_head ? a.H : 1, a.dq_weight, a.dk_weight,
+                                                                      a.w_dtype);
     MF_LAUNCHED("qk_rotary_join_kernel");
   }
   return MF_OK;
 }
 template <typename T, bool BWD>
 int dispatch(const mf_qk_rotary_args& a, cudaStream_t st) {
-  constexpr int kMost = (BWD ? 8 : 16) / (int)sizeof(T);
   const int v = piece(a, BWD);
-  if constexpr (kMost >= 8) if (v == 8) return run<T, 8, BWD>(a, st);
-  if constexpr (kMost >= 4) if (v == 4) return run<T, 4, BWD>(a, st);
+  if constexpr (sizeof(T) == 2) if (v == 4) return run<T, 4, BWD>(a, st);
   return v == 2 ? run<T, 2, BWD>(a, st) : run<T, 1, BWD>(a, st);
 }
 }  // namespace
@@ -415,10 +455,9 @@ int qk_rotary_fwd(const mf_qk_rotary_args& a, cudaStream_t st) {
 size_t qk_rotary_bwd_workspace(const mf_qk_rotary_args& a) {
   if (!a.dq_weight) return 0;
   size_t most = 0;
-  for (int v = 1; v <= piece_limit(a.dtype, true); v *= 2) {       // whichever width the alignment allows
+  for (int v = 1; v <= piece_limit(a.dtype); v *= 2) {       // whichever width the alignment allows
     if (a.R / 2 % v || (a.D - a.R) % v) break;
-    const Plan c = plan(a, v, true);
-    const size_t n = sizeof(float) * 2 * a.D * (size_t)c.gx * c.gy;
+    const size_t n = sizeof(float) * part_floats(a, plan(a, v, true));
     if (n > most) most = n;
   }
   return most;
