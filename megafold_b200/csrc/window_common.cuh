@@ -107,12 +107,11 @@ KeyPlan key_plan(const WinP& p, int blocks_wanted) {
     int& m = t < c.n_sink ? most_sink : most_rest;
     if (n > m) m = n;
   }
-  // the longest list of a tile without sinks, unless that leaves processors idle; never below a few entries, which would
-  // not pay for the partial sums
-  const int64_t heads = (int64_t)p.B * p.N * p.Hk;
-  int64_t chunk = most_rest > 0 ? most_rest : most_sink;
-  const int64_t even = (all * heads + blocks_wanted - 1) / blocks_wanted;
-  if (chunk > even) chunk = even;
+  // an even share of all entries for each block that the processors hold, as long as that cuts no list needlessly; never below a few
+  // entries, which would not pay for the partial sums
+  const int64_t heads = (int64_t)p.B * p.N * p.Hk, most = most_sink > most_rest ? most_sink : most_rest;
+  int64_t chunk = (all * heads + blocks_wanted - 1) / blocks_wanted;
+  if (chunk > most) chunk = most;
   if (chunk < 6) chunk = 6;
   c.chunk = (int)chunk;
   auto chunks = [&](int n) { const int k = (n + c.chunk - 1) / c.chunk; return k > 1 ? k : 1; };
@@ -134,19 +133,19 @@ __device__ __forceinline__ float* part_of(float* parts, const KeyPlan& c, const 
   return parts + (size_t)2 * KT * p.D * (head * c.split_x + x);
 }
 
-// Adds the parts of the tiles that were split, a thread an element: blockIdx = (piece of 256 elements, tile, head of all sequences).
+// Adds the parts of the tiles that were split, a thread an element; blockIdx.x enumerates (head of all sequences, tile, piece of 256 elements).
 // (With a block a tile a long sequence's tile of sinks, 28 parts of it, took 163 us.)
 template <typename T, int KT, int QB>
-__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinP p, const KeyPlan c, const float* __restrict__ parts) {
-  const int tile = blockIdx.y, nc = tile < c.n_sink ? c.nc_sink : c.nc_rest;
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinP p, const KeyPlan c, const float* __restrict__ parts, int tiles, int pieces) {
+  const int unit = blockIdx.x / pieces, tile = unit % tiles, nc = tile < c.n_sink ? c.nc_sink : c.nc_rest;
   const int x0 = tile < c.n_sink ? tile * c.nc_sink : c.n_sink * c.nc_sink + (tile - c.n_sink) * c.nc_rest;
-  const int e = blockIdx.x * 256 + threadIdx.x;
+  const int e = (blockIdx.x - unit * pieces) * 256 + threadIdx.x;
   if (x0 >= c.split_x || nc == 1 || e >= 2 * KT * p.D) return;
   const int which = e / (KT * p.D), r = e - which * KT * p.D, row = r / p.D, d = r - row * p.D, j = tile * KT + row;
   if (j >= p.Lk) return;
   int used = (list_length<KT, QB>(p, tile) + c.chunk - 1) / c.chunk;
   if (used < 1) used = 1;
-  const int64_t head = blockIdx.z, bn = head / p.Hk;
+  const int64_t head = unit / tiles, bn = head / p.Hk;
   const float* src = part_of<KT>(const_cast<float*>(parts), c, p, head, x0) + e;
   const size_t step = (size_t)2 * KT * p.D;
   float s = 0.f;
@@ -158,10 +157,10 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 template <typename T, int KT, int QB>
 int window_join(const WinP& p, const KeyPlan& c, const float* parts, cudaStream_t st) {
   if (!c.split_x) return MF_OK;
-  const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink;
-  const int64_t heads = (int64_t)p.B * p.N * p.Hk;
-  MF_REQUIRE(tiles <= 65535 && heads <= 65535, MF_ERR_UNSUPPORTED, "%d tiles of %lld heads in parts are more than one launch takes", tiles, (long long)heads);
-  window_join_kernel<T, KT, QB><<<dim3((2 * KT * p.D + 255) / 256, tiles, (unsigned)heads), 256, 0, st>>>(p, c, parts);
+  const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink, pieces = (2 * KT * p.D + 255) / 256;
+  const int64_t blocks = (int64_t)p.B * p.N * p.Hk * tiles * pieces;
+  MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%d tiles of keys in parts are more than one launch takes", tiles);
+  window_join_kernel<T, KT, QB><<<(unsigned)blocks, 256, 0, st>>>(p, c, parts, tiles, pieces);
   MF_LAUNCHED("window_join_kernel");
   return MF_OK;
 }

@@ -69,6 +69,11 @@ CASES = [  # B, N, Lq, Lk, H, Hk, D, left, right, sinks, mask
     (1, 2, 140, 140, 2, 2, 48, 10, 3, 9, "front"),        # rows and sinks whose keys are all masked
     (1, 1, 64, 64, 2, 2, 32, 3, 0, 1000, "none"),         # more sinks than keys
     (1, 1, 1100, 1100, 1, 1, 32, 200, 0, 4, "none"),
+    (1, 1, 150, 150, 6, 2, 64, 30, 0, 4, "drop"),         # three heads share a key head: tiles of 126 and 63 rows
+    (1, 2, 90, 130, 14, 2, 32, 50, 7, 3, "pad"),          # seven
+    (1, 1, 40, 40, 48, 1, 16, 20, 0, 2, "none"),          # 48: two queries a tile
+    (1, 1, 70, 70, 72, 1, 32, 20, 5, 2, "drop"),          # more heads than a tile has rows: one at a time
+    (1, 1, 70, 300, 5, 1, 128, 100, 0, 2, "drop"),
 ]
 
 
@@ -247,3 +252,9 @@ def test_offsets_beyond_32_bits():
     small = mfb.window_attention_forward(q.cuda(), k.cuda(), v.cuda(), left, 0, sinks)
     # the same keys in other tiles: both within the bounds of the definition
     _check(small[0], ref, "o")
+
+
+@gpu
+@pytest.mark.parametrize("dt", [FP, BF])
+def test_more_heads_of_sequences_than_a_grid_has_rows(dt):
+    _run(*_inputs(1, 17000, 17, 17, 4, 4, 16, "drop", dt), 5, 0, 2)
