@@ -26,6 +26,7 @@ struct RotP {
   const float* inv_freq;
   const void* pos; int64_t ps[3]; bool pos64;            // NULL: the index along L
   float eps;
+  uint32_t pair_magic;                      // 2^20 / (R / 2), rounded up
   int hb, tb, mt;                           // a block's heads, its tokens at a time and its tokens in a chunk
   int log_lpr;                              // threads of a row
   void *q_out, *k_out;                      // contiguous
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
   const float inv_d = 1.f / p.D;
   extern __shared__ __align__(16) float shared[];
   float2* const angles = reinterpret_cast<float2*>(shared);    // [mt][pairs]: cosine, sine
+  double* const positions = reinterpret_cast<double*>(angles + p.mt * pairs);
 
   Vec<V> wt[UPL], dw[BWD ? UPL : 1] = {};
 #pragma unroll
@@ -183,15 +185,15 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
     u.has_a = u.has_a && live; u.has_b = u.has_b && live;
     return u;
   };
+  const uint32_t tokens = (uint32_t)p.tokens;
   // a thread's place among the tokens: stepped along, and found by divisions only where a sequence ends
   struct Place {
-    int64_t tok;
-    uint32_t l;
+    uint32_t tok, l;
     const T* row;
   };
-  auto place = [&](int64_t tok) {
+  auto place = [&](uint32_t tok) {
     Place c;
-    const uint32_t t = head_ok && tok < p.tokens ? (uint32_t)tok : 0, bn = t / (uint32_t)p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
+    const uint32_t t = head_ok && tok < tokens ? tok : 0, bn = t / (uint32_t)p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
     c.tok = tok; c.l = t - bn * p.L;
     c.row = in + b * sb + n * sn + c.l * sl;
     return c;
@@ -206,32 +208,35 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
     }
   };
   // this block's tokens: chunks of mt, gridDim.x apart
-  for (int64_t c0 = (int64_t)blockIdx.x * p.mt; c0 < p.tokens; c0 += (int64_t)gridDim.x * p.mt) {
-    const int64_t c1 = c0 + p.mt < p.tokens ? c0 + p.mt : p.tokens;
+  for (uint32_t c0 = blockIdx.x * p.mt; c0 < tokens; c0 += gridDim.x * p.mt) {
+    const uint32_t c1 = c0 + p.mt < tokens ? c0 + p.mt : tokens;
     Place at = place(c0 + tslot);
     bool live = head_ok && at.tok < c1;
     Raw<T, V> xr[UPL], dr[BWD ? UPL : 1];
-    const int64_t arr = (live ? at.tok : 0) * own * p.D;
+    const int64_t arr = (int64_t)(live ? at.tok : 0) * own * p.D;
     const T* dp = BWD ? din + arr : nullptr;
     T* to = out + arr;
     const float2* turns = angles + (live ? tslot : 0) * pairs;
     fetch(at, dp, live, xr, dr);                               // on its way while the angles are formed
-    __syncthreads();                                           // the last chunk's angles have been read
-    for (int x = threadIdx.x; x < (int)(c1 - c0) * pairs; x += kThreads) {
-      const int i = x / pairs, f = x - i * pairs;
-      const uint32_t t = (uint32_t)(c0 + i), bn = t / (uint32_t)p.L, l = t - bn * p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
+    for (uint32_t i = threadIdx.x; i < c1 - c0; i += kThreads) {
+      const uint32_t t = c0 + i, bn = t / (uint32_t)p.L, l = t - bn * p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
       double pos = (double)l;
       if (p.pos) {
-        const int64_t at = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
-        pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
+        const int64_t x = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
+        pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[x] : (double)static_cast<const int32_t*>(p.pos)[x];
       }
+      positions[i] = pos;
+    }
+    __syncthreads();                                           // besides: the last chunk's angles have been read
+    for (uint32_t x = threadIdx.x; x < (c1 - c0) * pairs; x += kThreads) {
+      const uint32_t i = x * p.pair_magic >> 20, f = x - i * pairs;          // x / pairs, for the few thousand angles of a chunk
       float2 a;
-      turn_of(pos, p.inv_freq[f], a.y, a.x);
+      turn_of(positions[i], p.inv_freq[f], a.y, a.x);
       angles[x] = a;
     }
     __syncthreads();
     // as many steps for every thread: the sums over rows take whole warps
-    for (int64_t t0 = c0; t0 < c1; t0 += p.tb) {
+    for (uint32_t t0 = c0; t0 < c1; t0 += p.tb) {
       Vec<V> x[UPL], d[BWD ? UPL : 1];
       float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -254,14 +259,20 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
       for (int k = 0; k < UPL; ++k) {
         const Unit<V, IL> u = unit(k, now);
         Vec<V> turn;                                           // a: cosines, b: sines; 1 and 0 where nothing turns
+        if (u.turned) {                                        // (a dead thread's row is zeros: any angle will do)
+          const float2* at_turn = turns + (lane + k * lpr) * V;
+          if constexpr (V == 1) {
+            turn.a[0] = make_float2(at_turn->x, 0.f); turn.b[0] = make_float2(at_turn->y, 0.f);
+          } else {
 #pragma unroll
-        for (int e = 0; e < P; ++e) { turn.a[e] = make_float2(1.f, 1.f); turn.b[e] = make_float2(0.f, 0.f); }
-        if (u.turned && now) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float2 t = turns[(lane + k * lpr) * V + e];
-            put<V>(turn.a, e, t.x); put<V>(turn.b, e, t.y);
+            for (int e = 0; e < P; ++e) {
+              const float4 t = reinterpret_cast<const float4*>(at_turn)[e];
+              turn.a[e] = make_float2(t.x, t.z); turn.b[e] = make_float2(t.y, t.w);
+            }
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < P; ++e) { turn.a[e] = make_float2(1.f, 1.f); turn.b[e] = make_float2(0.f, 0.f); }
         }
         if constexpr (!BWD) {
 #pragma unroll
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
         }
       }
       to += arr_step;
-      turns += p.tb * pairs;
+      if (live) turns += p.tb * pairs;
     }
   }
   if constexpr (BWD) {
@@ -408,7 +419,7 @@ Plan plan(const mf_qk_rotary_args& a, int V, bool bwd) {
   int64_t gx = (tokens + c.mt - 1) / c.mt;
   if (bwd) { const int64_t most = (want + c.gy - 1) / c.gy; if (gx > most) gx = most; }
   c.gx = (int)gx;
-  c.smem = sizeof(float2) * (size_t)c.mt * pairs;
+  c.smem = sizeof(float2) * (size_t)c.mt * pairs + sizeof(double) * c.mt;
   const size_t sums = bwd && a.dq_weight ? sizeof(float) * (size_t)c.tb * c.hb * a.D : 0;
   if (sums > c.smem) c.smem = sums;
   return c;
@@ -421,6 +432,7 @@ int run(const mf_qk_rotary_args& a, cudaStream_t st) {
   RotP p = rot_params(a);
   const Plan c = plan(a, V, BWD);
   p.log_lpr = c.log_lpr; p.hb = c.hb; p.tb = c.tb; p.mt = c.mt;
+  p.pair_magic = a.R > 1 ? ((1u << 20) + a.R / 2 - 1) / (a.R / 2) : 1u << 20;
   const bool sums = BWD && a.dq_weight;
   if (sums) p.parts = static_cast<float*>(a.workspace);
   const auto go = [&](auto il) -> int {
