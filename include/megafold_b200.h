@@ -305,7 +305,7 @@ MF_API int mf_relpos_bwd(const mf_relpos_args* args, void* stream);
  * RMS norm of every head of queries and keys and their rotation by position:
  *   y = x * (mean_d x^2 + eps)^-1/2 * weight;  of y's first R elements, pair k (elements k and k + R/2, or 2k and 2k + 1 with
  *   `interleaved`) is turned by the angle position * inv_freq[k], formed in 64 bits; the others stay.
- * q [B,N,L,H,D] and k [B,N,L,Hk,D] with arbitrary element strides; D <= 256, R even, R <= D.
+ * q [B,N,L,H,D] and k [B,N,L,Hk,D] with arbitrary element strides; D <= 256, R even, R <= D, B*N*L < 2^31.
  * q_weight, k_weight: [D], or with per_head [H,D] and [Hk,D], contiguous in w_dtype; both NULL: ones.  inv_freq: fp32 [R/2].
  * positions: pos_bytes (4 or 8) wide integers with element strides (b, n, l); NULL: the index along L.
  * q_out, k_out, dq_out, dk_out, dq, dk: contiguous, in `dtype`.  dq_weight, dk_weight: as the weights (NULL without), fully
@@ -334,7 +334,7 @@ MF_API int mf_qk_rotary_bwd(const mf_qk_rotary_args* args, void* stream);
  *
  * q [B,N,Lq,H,D], k and v [B,N,Lk,Hk,D] with arbitrary element strides; D <= 128, H a multiple of Hk, Lq and Lk <= 2^29.
  * left, right, sinks >= 0 (INT32_MAX: no bound).  mask: MF_U8 keep-mask with element strides (b, n, l), NULL: every key is
- * kept.  What masked keys hold (NaN, too) reaches nothing.
+ * kept.  What keys hold that are masked or that no query sees (NaN, too) reaches nothing; the others have to hold numbers.
  * o, d_o, dq [B,N,Lq,H,D], dk, dv [B,N,Lk,Hk,D]: contiguous in `dtype`; lse: fp32 [B,N,H,Lq], may be NULL on the forward.
  * Every result is summed in a fixed order (bit-reproducible).  workspace: mf_window_fwd_workspace_bytes() /
  * mf_window_bwd_workspace_bytes() bytes (0: none needed), 256-byte aligned.

@@ -11,7 +11,7 @@
 // there while this block's are exponentiated.  O stays in TMEM and is brought to a new maximum only when that grew by more than
 // 2^8 in the exponent.  A window makes short walks (5 blocks at 64 + 64 keys), so nothing is pipelined across items: two CTAs share
 // an SM instead.  Tried at [1, 1, 16384, 16 on 4 heads, 64], window 1024 / [2, 1, 2048 of 6001, 16 on 4, 128], window 2047 / one token of 64
-// sequences, 32 on 8 heads of 128: this 160 / 94 / 69 us; one thread a row, one score buffer, four CTAs (two at 128 columns) 145 / 103 / 96;
+// sequences, 32 on 8 heads of 128: this 160 / 88 / 68 us; one thread a row, one score buffer, four CTAs (two at 128 columns) 145 / 103 / 96;
 // one score buffer, two threads a row 159 / 127 / 87; blocks of 128 keys 168 / 102 / 77.
 // Bound: the exponentials, half of the time at 64 columns (16 a clock and SM), and the waits between a block's steps.
 //

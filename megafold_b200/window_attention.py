@@ -23,8 +23,8 @@ def window_attention(Q, K, V, left, right=0, sinks: int = 0, mask=None):
 
     Query i stands at position ``p = i + Lk - Lq`` (the queries are the last of the keys) and sees key j where ``j <= p + right`` and
     ``j >= p - left`` or ``j < sinks``.  ``left`` or ``right`` None: no bound on that side; ``right=0`` is causal.
-    mask: a bool (or uint8) keep-mask ``[B, N, 1, 1, Lk]``; what masked keys hold, even NaN, reaches nothing.  A query that sees no key
-    gives zeros and passes no gradient."""
+    mask: a bool (or uint8) keep-mask ``[B, N, 1, 1, Lk]``.  What keys hold that are masked or that no query sees, even NaN, reaches
+    nothing.  A query that sees no key gives zeros and passes no gradient."""
     return _lib.native().window_attention(Q, K, V, mask, *_span(left, right, sinks))
 
 

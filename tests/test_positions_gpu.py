@@ -193,6 +193,37 @@ def test_no_forward_mode_and_no_transforms():
                 call(torch.autograd.forward_ad.make_dual(arg, arg))
 
 
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(4)
+    # the table: the result is linear in it, so that a difference is the gradient's product up to the rounding of sums of 900 terms
+    w, d = torch.randn(16, 2, generator=g), torch.randn(1, 1, 2, 30, 30, generator=g)
+    step = torch.randn(16, 2, generator=g)
+    leaf = w.cuda().requires_grad_(True)
+    grad, = torch.autograd.grad(mfb.relative_position_bias(leaf, 30, 30, max_distance=20), leaf, d.cuda())
+    pos = torch.arange(30)[None]
+    f = lambda t: float((orc.relpos(t, orc.buckets(pos, pos, 16, 20, "log", True))[0] * d.double()).sum())        # noqa: E731
+    want = f(w.double() + step.double()) - f(w.double())
+    assert abs(float((grad.cpu().double() * step.double()).sum()) - want) <= 1e-5 * float((grad.cpu().double() * step.double()).abs().sum())
+    # norm and rotation: central differences of a function whose values are sums of some 1000 terms of size one
+    q, k = torch.randn(1, 1, 9, 3, 24, generator=g), torch.randn(1, 1, 9, 1, 24, generator=g)
+    qw, kw = 1 + 0.2 * torch.randn(24, generator=g), 1 + 0.2 * torch.randn(24, generator=g)
+    freq, pos = torch.rand(8, generator=g), torch.arange(9)
+    dq, dk = torch.randn(q.shape, generator=g), torch.randn(k.shape, generator=g)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, qw, kw)]
+    outs = mfb.qk_norm_rotary(*leaves, freq.cuda(), pos.cuda(), 1e-6, True)
+    grads = torch.autograd.grad(outs, leaves, [dq.cuda(), dk.cuda()])
+    for i in range(4):
+        step = torch.randn(leaves[i].shape, generator=g).double()
+
+        def value(h):
+            a = [t.double() + (h * step if j == i else 0) for j, t in enumerate((q, k, qw, kw))]
+            return float((orc.rotary(a[0], a[2], freq, pos, 1e-6, True) * dq.double()).sum() + (orc.rotary(a[1], a[3], freq, pos, 1e-6, True) * dk.double()).sum())
+
+        want = (value(1e-5) - value(-1e-5)) / 2e-5
+        prod = grads[i].cpu().double() * step
+        assert abs(float(prod.sum()) - want) <= 1e-5 * float(prod.abs().sum()) + 1e-6, i
+
+
 def test_evo_oracle_is_the_plain_softmax():
     """The attention oracle of the older tests and the one above agree (so that the layer's test rests on both)."""
     g = torch.Generator().manual_seed(0)
