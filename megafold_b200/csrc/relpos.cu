@@ -136,9 +136,11 @@ __global__ void __launch_bounds__(kThreads, 4) relpos_fwd_kernel(const __grid_co
 // where positions run on.  It sums in registers and adds a sum to a column of its own of the block's table in shared memory when the row
 // changes (no atomics: the sums' order is fixed); walking down columns instead, a warp met such a change in most of its
 // steps and [2, 8, 1531, 1531] took 173 us.  The block's table goes to `parts` [gridDim.y * gridDim.x][H][rows].
-constexpr int kBwdCols = 8;
+// Two rows of a thread are in registers, two more on their way into L2, and 512 threads of an SM have 128 registers each: [2, 8, 1531, 1531]
+// fp32 and 64 rows of the table 102 us, six rows ahead instead of four 103; three blocks of 80 registers 112, without the way into L2 120.
+constexpr int kBwdCols = 8, kBwdAhead = 4, kBwdResident = 512;
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
+__global__ void __launch_bounds__(kThreads, kBwdResident / kThreads) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
   constexpr int kC = kBwdCols;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
@@ -209,16 +211,24 @@ __global__ void __launch_bounds__(kThreads, 3) relpos_bwd_kernel(const __grid_co
     for (int e = 0; e < kC; ++e) acc[e] += to_f(x[e]);             // zeros for columns that are not there
     next(c);
   };
+  auto ahead = [&](int i) {
+    for (int x = lane * 128; x < width * (int)sizeof(T); x += tpr * 128)
+      if (i < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(in + (int64_t)i * p.Lk) + x));
+  };
+#pragma unroll
+  for (int k = 2; k < kBwdAhead; ++k) ahead(i0 + slot + k * slots);
   Cursor in_at = start(), sum_at = start();
   T x0[kC], x1[kC];                                // two rows under way
   load(in_at, x0);
   load(in_at, x1);
   while (sum_at.i < end) {
-    T y[kC];
-#pragma unroll
-    for (int e = 0; e < kC; ++e) { y[e] = x0[e]; x0[e] = x1[e]; }
+    add(sum_at, x0);
+    ahead(in_at.i + (kBwdAhead - 2) * slots);
+    load(in_at, x0);
+    if (sum_at.i >= end) break;
+    add(sum_at, x1);
+    ahead(in_at.i + (kBwdAhead - 2) * slots);
     load(in_at, x1);
-    add(sum_at, y);
   }
 #pragma unroll
   for (int e = 0; e < kC; ++e) mine[cur[e] * nt] += acc[e];
@@ -275,7 +285,7 @@ BwdPlan bwd_plan(RelP& p) {
   b.tiles = (p.Lk + tpr * kBwdCols - 1) / (tpr * kBwdCols);
   // as many blocks as fit the processors at once, each with two steps of its rows at least
   int fit = (int)(220 * 1024 / (b.smem + 4096));
-  if (fit > 1024 / b.threads) fit = 1024 / b.threads;
+  if (fit > kBwdResident / b.threads) fit = kBwdResident / b.threads;
   const int64_t want = (int64_t)tcx::sm_count() * (fit < 1 ? 1 : fit), others = (int64_t)p.H * b.tiles * p.B;
   int64_t strips = want / others;
   const int64_t most = (p.Lq + 2 * slots - 1) / (2 * slots);
