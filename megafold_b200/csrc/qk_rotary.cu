@@ -9,7 +9,7 @@
 // fp32, the outputs are rounded once.  The weights' gradients are summed in a fixed order: a thread over its tokens, a block over its
 // threads in shared memory, a second kernel over the blocks.
 //
-// Bound: HBM; for single tokens latency.
+// Bound: issue slots and the latency of the instructions (0.57 of the copy rate); for single tokens the latency of a launch.
 #include "evo_tc_common.cuh"
 
 namespace mf {
@@ -28,6 +28,7 @@ struct RotP {
   float eps;
   uint32_t pair_magic;                      // 2^20 / (R / 2), rounded up
   int hb, tb, mt;                           // a block's heads, its tokens at a time and its tokens in a chunk
+  int spans;                                // chunks of a sequence where all sequences have the same positions, else 0
   int log_lpr;                              // threads of a row
   void *q_out, *k_out;                      // contiguous
   const void *dq_out, *dk_out; void *dq, *dk;
@@ -139,18 +140,25 @@ __device__ __forceinline__ int element(const Unit<V, IL>& u, int e) {
   else return e < V ? u.a + e : u.b + e - V;
 }
 __device__ __forceinline__ float row_sum(float v, int lpr) {
-  for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lpr) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 // A block takes `hb` heads (blockIdx.y; of the H + Hk of queries and keys) of `tb` tokens at a time and walks the tokens: the threads of a token's
 // heads are neighbours, so that a warp reads and writes whole lines, and a thread keeps to its head, whose weights and whose sums of
-// the weights' gradients stay in registers.  The angles of the next tokens are formed by all threads together, `mt` tokens (a
-// multiple of tb) ahead, in shared memory.  (With a thread going through all heads of its token instead, each load touched as many
-// lines as the warp had tokens: 4 + 4 heads of 32, 147456 tokens: 48 us forward, 108 backward.)
+// the weights' gradients stay in registers.  The angles of a chunk of tokens are formed by all threads together in shared memory.  A step's
+// loads leave one step ahead (asynchronous copies three to six steps ahead were no faster: registers and warps bound it, not the way to memory).
+// 4 + 4 heads of 32, 147456 tokens, forward and backward: a thread through all heads of its token 48 and 108 us; a thread a head in
+// pieces of 8 bytes 50 and 71; pieces of 16 bytes, as many blocks as stay resident 42 and 63, with the same positions in all 384 sequences 39 and 58.
 // UPL: units of a thread.  Every thread of a warp takes part in each sum over a row: rows that do not exist are zeros.
+constexpr int units_per(int V) { return V >= 4 ? 1 : V == 2 ? 2 : 4; }
+// blocks of an SM ([1, 32768, 16 + 4, 128] bf16 in pieces of 16 bytes: forward 2 blocks 113 us, 3 99, 4 110; backward 1 186, 2 133, 3 233.
+// [1, 147456, 4 + 4, 32] fp32: forward 3 blocks 68, 4 60; backward 2 91, 3 93)
+constexpr int resident(int V, int es, bool bwd) { return units_per(V) > 1 ? 2 : V * es < 16 ? (bwd ? 3 : 4) : bwd ? 2 : es == 4 ? 4 : 3; }
 template <typename T, int V, int UPL, bool IL, bool BWD>
-__global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary_kernel(const __grid_constant__ RotP p) {
+__global__ void __launch_bounds__(kThreads, resident(V, sizeof(T), BWD)) qk_rotary_kernel(const __grid_constant__ RotP p) {
   constexpr int P = Vec<V>::P;
   const int lpr = 1 << p.log_lpr, lane = threadIdx.x & (lpr - 1), slot = threadIdx.x >> p.log_lpr;
   const int heads = p.H + p.Hk, tslot = slot / p.hb, g = blockIdx.y * p.hb + slot - tslot * p.hb;
@@ -158,8 +166,10 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
   const int h = is_q ? g : g - p.H, pairs = p.R / 2;
   const float inv_d = 1.f / p.D;
   extern __shared__ __align__(16) float shared[];
-  float2* const angles = reinterpret_cast<float2*>(shared);    // [mt][pairs]: cosine, sine
-  double* const positions = reinterpret_cast<double*>(angles + p.mt * pairs);
+  // [mt][pairs] cosines and sines (two pairs: both cosines, then both sines), then V pairs that turn nothing
+  float* const angles = reinterpret_cast<float*>(shared);
+  double* const positions = reinterpret_cast<double*>(angles + 2 * (p.mt * pairs + V));
+  if (threadIdx.x < 2 * V) angles[2 * p.mt * pairs + threadIdx.x] = V > 1 ? (threadIdx.x & 2 ? 0.f : 1.f) : (threadIdx.x ? 0.f : 1.f);
 
   Vec<V> wt[UPL], dw[BWD ? UPL : 1] = {};
 #pragma unroll
@@ -207,110 +217,148 @@ __global__ void __launch_bounds__(kThreads, UPL > 1 ? 2 : BWD ? 3 : 4) qk_rotary
       for (int k = 0; k < UPL; ++k) load_unit<T, V, IL>(dp, 1, unit(k, live), d[k]);
     }
   };
-  // this block's tokens: chunks of mt, gridDim.x apart
-  for (uint32_t c0 = blockIdx.x * p.mt; c0 < tokens; c0 += gridDim.x * p.mt) {
-    const uint32_t c1 = c0 + p.mt < tokens ? c0 + p.mt : tokens;
-    Place at = place(c0 + tslot);
-    bool live = head_ok && at.tok < c1;
-    Raw<T, V> xr[UPL], dr[BWD ? UPL : 1];
-    const int64_t arr = (int64_t)(live ? at.tok : 0) * own * p.D;
-    const T* dp = BWD ? din + arr : nullptr;
-    T* to = out + arr;
-    const float2* turns = angles + (live ? tslot : 0) * pairs;
-    fetch(at, dp, live, xr, dr);                               // on its way while the angles are formed
-    for (uint32_t i = threadIdx.x; i < c1 - c0; i += kThreads) {
-      const uint32_t t = c0 + i, bn = t / (uint32_t)p.L, l = t - bn * p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
-      double pos = (double)l;
-      if (p.pos) {
-        const int64_t x = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
-        pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[x] : (double)static_cast<const int32_t*>(p.pos)[x];
-      }
-      positions[i] = pos;
+  // This block's chunks, mt tokens at most each.  Where all sequences have the same positions, a block keeps to one span of them and
+  // walks the sequences, with one set of angles; else the chunks are gridDim.x apart.
+  const uint32_t span = p.spans ? blockIdx.x % p.spans : 0, leap = p.spans ? gridDim.x / p.spans : gridDim.x, n_rows = p.spans ? tokens / p.L : 0;
+  struct Chunk { uint32_t c0, c1; };                           // none left: c0 = c1
+  auto chunk = [&](uint32_t x) {
+    Chunk c;
+    uint32_t end = tokens;
+    if (p.spans) {
+      if (x >= n_rows) return Chunk{tokens, tokens};
+      end = (x + 1) * p.L;
+      c.c0 = x * p.L + span * p.mt;
+    } else {
+      if (x >= (tokens + p.mt - 1) / p.mt) return Chunk{tokens, tokens};
+      c.c0 = x * p.mt;
     }
-    __syncthreads();                                           // besides: the last chunk's angles have been read
-    for (uint32_t x = threadIdx.x; x < (c1 - c0) * pairs; x += kThreads) {
-      const uint32_t i = x * p.pair_magic >> 20, f = x - i * pairs;          // x / pairs, for the few thousand angles of a chunk
-      float2 a;
-      turn_of(positions[i], p.inv_freq[f], a.y, a.x);
-      angles[x] = a;
-    }
-    __syncthreads();
-    // as many steps for every thread: the sums over rows take whole warps
-    for (uint32_t t0 = c0; t0 < c1; t0 += p.tb) {
-      Vec<V> x[UPL], d[BWD ? UPL : 1];
-      float2 ss2 = make_float2(0.f, 0.f);
+    c.c1 = end - c.c0 < (uint32_t)p.mt ? end : c.c0 + p.mt;
+    return c;
+  };
+  uint32_t at_chunk = p.spans ? blockIdx.x / p.spans : blockIdx.x;
+  Chunk rest = chunk(at_chunk);                                // what is left of the chunk
+  Place at = place(rest.c0 + tslot);
+  bool live = head_ok && at.tok < rest.c1, fresh = true, angles_left = true;
+  Raw<T, V> xr[UPL], dr[BWD ? UPL : 1];
+  const T* dp = BWD ? din + (int64_t)(live ? at.tok : 0) * own * p.D : nullptr;
+  T* to = out + (int64_t)(live ? at.tok : 0) * own * p.D;
+  int first_turn[UPL], turn_step[UPL];
 #pragma unroll
-      for (int k = 0; k < UPL; ++k) {
-        unpack_unit<T, V, IL>(xr[k], x[k]);
-        if constexpr (BWD) unpack_unit<T, V, IL>(dr[k], d[k]);
-#pragma unroll
-        for (int e = 0; e < P; ++e) ss2 = fma2(x[k].b[e], x[k].b[e], fma2(x[k].a[e], x[k].a[e], ss2));
+  for (int k = 0; k < UPL; ++k) {
+    const bool turned = unit(k, true).turned;
+    first_turn[k] = 2 * (turned ? tslot * pairs + (lane + k * lpr) * V : p.mt * pairs);
+    turn_step[k] = turned ? 2 * p.tb * pairs : 0;
+  }
+  fetch(at, dp, live, xr, dr);                                 // on its way while the angles are formed
+  const float* turns[UPL];
+  while (rest.c0 < rest.c1) {
+    if (fresh && angles_left) {
+      for (uint32_t i = threadIdx.x; i < rest.c1 - rest.c0; i += kThreads) {
+        const uint32_t t = rest.c0 + i, bn = t / (uint32_t)p.L, l = t - bn * p.L, b = bn / (uint32_t)p.N, n = bn - b * p.N;
+        double pos = (double)l;
+        if (p.pos) {
+          const int64_t x = b * p.ps[0] + n * p.ps[1] + l * p.ps[2];
+          pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[x] : (double)static_cast<const int32_t*>(p.pos)[x];
+        }
+        positions[i] = pos;
       }
-      const bool now = live;
+      __syncthreads();                                         // besides: the last chunk's angles have been read
+      for (uint32_t x = threadIdx.x; x < (rest.c1 - rest.c0) * pairs; x += kThreads) {
+        const uint32_t i = x * p.pair_magic >> 20, f = x - i * pairs;          // x / pairs, for the few thousand angles of a chunk
+        float* const at_turn = angles + (V > 1 ? 4 * (x >> 1) + (x & 1) : 2 * x);
+        turn_of(positions[i], p.inv_freq[f], at_turn[V > 1 ? 2 : 1], at_turn[0]);
+      }
+      __syncthreads();
+      angles_left = !p.spans;
+    }
+    if (fresh) {
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) turns[k] = angles + (live ? first_turn[k] : 2 * p.mt * pairs);      // a dead thread's row is zeros and turns nothing
+    }
+    // every thread takes every step: the sums over rows take whole warps
+    Vec<V> x[UPL], d[BWD ? UPL : 1];
+    float2 ss2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < UPL; ++k) {
+      unpack_unit<T, V, IL>(xr[k], x[k]);
+      if constexpr (BWD) unpack_unit<T, V, IL>(dr[k], d[k]);
+#pragma unroll
+      for (int e = 0; e < P; ++e) ss2 = fma2(x[k].b[e], x[k].b[e], fma2(x[k].a[e], x[k].a[e], ss2));
+    }
+    const bool now = live;
+    T* const row_out = to;
+    rest.c0 += p.tb;
+    fresh = rest.c0 >= rest.c1;
+    if (!fresh) {
       at.tok += p.tb; at.l += p.tb; at.row += row_step;
+      live = head_ok && at.tok < rest.c1;
       if (BWD) dp += arr_step;
-      live = head_ok && at.tok < c1;
+      to += arr_step;
       if (live && at.l >= (uint32_t)p.L) at = place(at.tok);
-      fetch(at, dp, live, xr, dr);
-      const float rstd = rsqrtf(fmaf(row_sum(ss2.x + ss2.y, lpr), inv_d, p.eps));
-      const float2 rstd2 = make_float2(rstd, rstd);
-      float2 dot2 = make_float2(0.f, 0.f);
+    } else {                                                 // to the next chunk
+      at_chunk += leap;
+      rest = chunk(at_chunk);
+      at = place(rest.c0 + tslot);
+      live = head_ok && at.tok < rest.c1;
+      const int64_t arr = (int64_t)(live ? at.tok : 0) * own * p.D;
+      if (BWD) dp = din + arr;
+      to = out + arr;
+    }
+    fetch(at, dp, live, xr, dr);
+    const float rstd = rsqrtf(fmaf(row_sum(ss2.x + ss2.y, lpr), inv_d, p.eps));
+    const float2 rstd2 = make_float2(rstd, rstd);
+    float2 dot2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < UPL; ++k) {
+      const Unit<V, IL> u = unit(k, now);
+      Vec<V> turn;                                           // a: cosines, b: sines; 1 and 0 where nothing turns
+      if constexpr (V == 1) {
+        const float2 t = *reinterpret_cast<const float2*>(turns[k]);
+        turn.a[0] = make_float2(t.x, 0.f); turn.b[0] = make_float2(t.y, 0.f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float4 t = reinterpret_cast<const float4*>(turns[k])[e];
+          turn.a[e] = make_float2(t.x, t.y); turn.b[e] = make_float2(t.z, t.w);
+        }
+      }
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float2 ya = mul2(mul2(x[k].a[e], rstd2), wt[k].a[e]), yb = mul2(mul2(x[k].b[e], rstd2), wt[k].b[e]), c = turn.a[e], s = turn.b[e];
+          x[k].a[e] = sub2(mul2(ya, c), mul2(yb, s));
+          x[k].b[e] = fma2(ya, s, mul2(yb, c));
+        }
+        store_unit<T, V, IL>(row_out, u, x[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float2 c = turn.a[e], s = turn.b[e], da = d[k].a[e], db = d[k].b[e];
+          const float2 ga = fma2(db, s, mul2(da, c)), gb = sub2(mul2(db, c), mul2(da, s));
+          x[k].a[e] = mul2(x[k].a[e], rstd2); x[k].b[e] = mul2(x[k].b[e], rstd2);        // hat
+          const float2 ta = mul2(ga, x[k].a[e]), tb = mul2(gb, x[k].b[e]);
+          dw[k].a[e] = add2(dw[k].a[e], ta); dw[k].b[e] = add2(dw[k].b[e], tb);
+          dot2 = fma2(tb, wt[k].b[e], fma2(ta, wt[k].a[e], dot2));
+          d[k].a[e] = mul2(ga, wt[k].a[e]); d[k].b[e] = mul2(gb, wt[k].b[e]);
+        }
+      }
+    }
+    if constexpr (BWD) {
+      const float dot = row_sum(dot2.x + dot2.y, lpr) * -inv_d;
+      const float2 minus = make_float2(dot, dot);
 #pragma unroll
       for (int k = 0; k < UPL; ++k) {
-        const Unit<V, IL> u = unit(k, now);
-        Vec<V> turn;                                           // a: cosines, b: sines; 1 and 0 where nothing turns
-        if (u.turned) {                                        // (a dead thread's row is zeros: any angle will do)
-          const float2* at_turn = turns + (lane + k * lpr) * V;
-          if constexpr (V == 1) {
-            turn.a[0] = make_float2(at_turn->x, 0.f); turn.b[0] = make_float2(at_turn->y, 0.f);
-          } else {
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-              const float4 t = reinterpret_cast<const float4*>(at_turn)[e];
-              turn.a[e] = make_float2(t.x, t.z); turn.b[e] = make_float2(t.y, t.w);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < P; ++e) { turn.a[e] = make_float2(1.f, 1.f); turn.b[e] = make_float2(0.f, 0.f); }
+        for (int e = 0; e < P; ++e) {
+          x[k].a[e] = mul2(rstd2, fma2(x[k].a[e], minus, d[k].a[e]));
+          x[k].b[e] = mul2(rstd2, fma2(x[k].b[e], minus, d[k].b[e]));
         }
-        if constexpr (!BWD) {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const float2 ya = mul2(mul2(x[k].a[e], rstd2), wt[k].a[e]), yb = mul2(mul2(x[k].b[e], rstd2), wt[k].b[e]), c = turn.a[e], s = turn.b[e];
-            x[k].a[e] = sub2(mul2(ya, c), mul2(yb, s));
-            x[k].b[e] = fma2(ya, s, mul2(yb, c));
-          }
-          store_unit<T, V, IL>(to, u, x[k]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const float2 c = turn.a[e], s = turn.b[e], da = d[k].a[e], db = d[k].b[e];
-            const float2 ga = fma2(db, s, mul2(da, c)), gb = sub2(mul2(db, c), mul2(da, s));
-            x[k].a[e] = mul2(x[k].a[e], rstd2); x[k].b[e] = mul2(x[k].b[e], rstd2);        // hat
-            const float2 ta = mul2(ga, x[k].a[e]), tb = mul2(gb, x[k].b[e]);
-            dw[k].a[e] = add2(dw[k].a[e], ta); dw[k].b[e] = add2(dw[k].b[e], tb);
-            dot2 = fma2(tb, wt[k].b[e], fma2(ta, wt[k].a[e], dot2));
-            d[k].a[e] = mul2(ga, wt[k].a[e]); d[k].b[e] = mul2(gb, wt[k].b[e]);
-          }
-        }
+        store_unit<T, V, IL>(row_out, unit(k, now), x[k]);
       }
-      if constexpr (BWD) {
-        const float dot = row_sum(dot2.x + dot2.y, lpr) * -inv_d;
-        const float2 minus = make_float2(dot, dot);
-#pragma unroll
-        for (int k = 0; k < UPL; ++k) {
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            x[k].a[e] = mul2(rstd2, fma2(x[k].a[e], minus, d[k].a[e]));
-            x[k].b[e] = mul2(rstd2, fma2(x[k].b[e], minus, d[k].b[e]));
-          }
-          store_unit<T, V, IL>(to, unit(k, now), x[k]);
-        }
-      }
-      to += arr_step;
-      if (live) turns += p.tb * pairs;
     }
+#pragma unroll
+    for (int k = 0; k < UPL; ++k)
+      if (live) turns[k] += turn_step[k];
   }
   if constexpr (BWD) {
     if (!p.parts) return;
@@ -381,12 +429,16 @@ RotP rot_params(const mf_qk_rotary_args& a) {
   return p;
 }
 
-// Elements of a piece: the widest load that sizes, strides and addresses allow, 8 bytes at most (with 16 a thread holds twice as much, and
-// an SM half as many threads).
-int piece_limit(int dtype) { return 8 / (int)dtype_size(dtype); }
+// Elements of a piece: the widest load that sizes, strides and addresses allow, 16 bytes at most, and 8 where 16 would leave processors
+// without a block (32 tokens of 32 + 8 heads of 128: 4.0 us instead of 4.9; 32768 tokens of 16 + 4 heads 117 forward, 187 backward instead of 99 and 133).
+int piece_limit(const mf_qk_rotary_args& a) {
+  const int v = 16 / (int)dtype_size(a.dtype);
+  const int64_t elements = (int64_t)a.B * a.N * a.L * (a.H + a.Hk) * a.D;
+  return elements / (2 * v) < (int64_t)kThreads * tcx::sm_count() ? v / 2 : v;
+}
 int piece(const mf_qk_rotary_args& a, bool bwd) {
   const int es = (int)dtype_size(a.dtype);
-  for (int v = piece_limit(a.dtype); v > 1; v /= 2) {
+  for (int v = piece_limit(a); v > 1; v /= 2) {
     bool ok = a.R / 2 % v == 0 && (a.D - a.R) % v == 0 && a.q_strides[4] == 1 && a.k_strides[4] == 1;
     for (int i = 0; i < 4; ++i) ok = ok && a.q_strides[i] % v == 0 && a.k_strides[i] % v == 0;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (bwd ? (uintptr_t)a.dq_out | (uintptr_t)a.dk_out | (uintptr_t)a.dq | (uintptr_t)a.dk
@@ -395,31 +447,46 @@ int piece(const mf_qk_rotary_args& a, bool bwd) {
   }
   return 1;
 }
-int units_per(int V) { return V >= 4 ? 1 : V == 2 ? 2 : 4; }
 
-struct Plan { int log_lpr, hb, tb, mt, gx, gy; size_t smem; };
+struct Plan { int log_lpr, hb, tb, mt, spans, gx, gy; size_t smem; };
 Plan plan(const mf_qk_rotary_args& a, int V, bool bwd) {
   Plan c;
   const int units = a.R / 2 / V + (a.D - a.R + 2 * V - 1) / (2 * V), lanes = (units + units_per(V) - 1) / units_per(V), heads = a.H + a.Hk;
   c.log_lpr = 0;
   while ((1 << c.log_lpr) < lanes) ++c.log_lpr;
   const int slots = kThreads >> c.log_lpr, pairs = a.R / 2;
-  const int64_t tokens = (int64_t)a.B * a.N * a.L, want = (bwd ? 3 : 8) * (int64_t)tcx::sm_count();
-  c.hb = heads < slots ? heads : slots;
+  // as few groups of heads as leave few threads without a row (20 heads, 32 rows a block: two groups, three tokens at a time)
+  int used = 0;
+  for (int least = (heads + slots - 1) / slots, gy = least; gy <= 4 * least && gy <= heads; ++gy) {
+    const int hb = (heads + gy - 1) / gy, tb = slots / hb, of_all = (int)((int64_t)1000 * heads * tb / ((int64_t)(heads + hb - 1) / hb * slots));
+    if (of_all > used + used / 10) { used = of_all; c.hb = hb; c.tb = tb; }
+  }
   c.gy = (heads + c.hb - 1) / c.hb;
-  c.hb = (heads + c.gy - 1) / c.gy;
-  c.tb = slots / c.hb;
-  // a chunk: some four angles a thread, less where that leaves processors idle, 16 KB of them at most
-  int steps = 4 * kThreads / (c.tb * (pairs > 0 ? pairs : 1));
-  if (steps < 1) steps = 1;
-  while (steps > 1 && (tokens + (int64_t)c.tb * steps - 1) / ((int64_t)c.tb * steps) * c.gy < want) steps /= 2;
-  while (steps * c.tb * pairs * 8 > 16 * 1024 && steps > 1) steps /= 2;
   while (c.tb > 1 && c.tb * pairs * 8 > 32 * 1024) c.tb /= 2;
-  c.mt = c.tb * steps;
-  int64_t gx = (tokens + c.mt - 1) / c.mt;
-  if (bwd) { const int64_t most = (want + c.gy - 1) / c.gy; if (gx > most) gx = most; }
-  c.gx = (int)gx;
-  c.smem = sizeof(float2) * (size_t)c.mt * pairs + sizeof(double) * c.mt;
+  // Steps of a chunk, 16 KB of angles and positions at most: those that take the blocks of one wave the least time.  Where all sequences have the same positions (and
+  // are no shorter than eight ninths of their steps), a block forms the angles of one chunk of them once; else it waits for new ones at each chunk.
+  const int64_t tokens = (int64_t)a.B * a.N * a.L, rows = (int64_t)a.B * a.N;
+  int64_t places = (int64_t)resident(V, (int)dtype_size(a.dtype), bwd) * tcx::sm_count() / c.gy, best = 0;
+  if (places < 1) places = 1;
+  const int64_t steps = (a.L + c.tb - 1) / c.tb;
+  const bool same = rows > 1 && steps * c.tb * 8 <= (int64_t)9 * a.L &&
+                    (!a.positions || ((a.B == 1 || a.pos_strides[0] == 0) && (a.N == 1 || a.pos_strides[1] == 0)));
+  for (int n = 1; n <= 64 && (n == 1 || n * c.tb * (pairs + 1) * 8 <= 16 * 1024); ++n) {
+    const int mt = c.tb * n;
+    int64_t time, spans = same ? (steps + n - 1) / n : 0, gx;
+    if (spans > places) spans = 0;
+    if (spans) {
+      const int64_t leap = places / spans < rows ? places / spans : rows;
+      gx = spans * leap;
+      time = ((rows + leap - 1) / leap + 1) * n;
+    } else {
+      const int64_t chunks = (tokens + mt - 1) / mt;
+      gx = chunks < places ? chunks : places;
+      time = (chunks + gx - 1) / gx * (n + 1);
+    }
+    if (n == 1 || time < best) { best = time; c.mt = mt; c.spans = (int)spans; c.gx = (int)gx; }
+  }
+  c.smem = sizeof(float2) * ((size_t)c.mt * pairs + V) + sizeof(double) * c.mt;
   const size_t sums = bwd && a.dq_weight ? sizeof(float) * (size_t)c.tb * c.hb * a.D : 0;
   if (sums > c.smem) c.smem = sums;
   return c;
@@ -428,10 +495,10 @@ size_t part_floats(const mf_qk_rotary_args& a, const Plan& c) { return (size_t)c
 
 template <typename T, int V, bool BWD>
 int run(const mf_qk_rotary_args& a, cudaStream_t st) {
-  constexpr int UPL = V >= 4 ? 1 : V == 2 ? 2 : 4;
+  constexpr int UPL = units_per(V);
   RotP p = rot_params(a);
   const Plan c = plan(a, V, BWD);
-  p.log_lpr = c.log_lpr; p.hb = c.hb; p.tb = c.tb; p.mt = c.mt;
+  p.log_lpr = c.log_lpr; p.hb = c.hb; p.tb = c.tb; p.mt = c.mt; p.spans = c.spans;
   p.pair_magic = a.R > 1 ? ((1u << 20) + a.R / 2 - 1) / (a.R / 2) : 1u << 20;
   const bool sums = BWD && a.dq_weight;
   if (sums) p.parts = static_cast<float*>(a.workspace);
@@ -454,7 +521,8 @@ int run(const mf_qk_rotary_args& a, cudaStream_t st) {
 template <typename T, bool BWD>
 int dispatch(const mf_qk_rotary_args& a, cudaStream_t st) {
   const int v = piece(a, BWD);
-  if constexpr (sizeof(T) == 2) if (v == 4) return run<T, 4, BWD>(a, st);
+  if constexpr (sizeof(T) == 2) if (v == 8) return run<T, 8, BWD>(a, st);
+  if (v == 4) return run<T, 4, BWD>(a, st);
   return v == 2 ? run<T, 2, BWD>(a, st) : run<T, 1, BWD>(a, st);
 }
 }  // namespace
@@ -467,7 +535,7 @@ int qk_rotary_fwd(const mf_qk_rotary_args& a, cudaStream_t st) {
 size_t qk_rotary_bwd_workspace(const mf_qk_rotary_args& a) {
   if (!a.dq_weight) return 0;
   size_t most = 0;
-  for (int v = 1; v <= piece_limit(a.dtype); v *= 2) {       // whichever width the alignment allows
+  for (int v = 1; v <= piece_limit(a); v *= 2) {       // whichever width the alignment allows
     if (a.R / 2 % v || (a.D - a.R) % v) break;
     const size_t n = sizeof(float) * part_floats(a, plan(a, v, true));
     if (n > most) most = n;

@@ -72,6 +72,31 @@ def test_forward_and_backward(B, N, L, H, Hk, D, R, dt, per_head, interleaved):
 
 
 @gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("B,N,L,H,Hk,D,R", [(2, 20, 131, 4, 4, 32, 32), (3, 3, 450, 5, 1, 96, 32), (2, 1, 900, 16, 4, 128, 128), (1, 4, 1100, 3, 2, 24, 8), (5, 60, 17, 4, 4, 32, 16)])
+def test_positions_of_all_sequences(B, N, L, H, Hk, D, R, dt, interleaved):
+    """Enough rows for the widest loads; positions of each sequence, and one set for all of them, expanded in every way or left out:
+    the same numbers but for the order of the sums over tokens, which are all held to their bound."""
+    q, k, qw, kw, freq, _, dq, dk = _inputs(B, N, L, H, Hk, D, R, True, dt)
+    line = torch.arange(L)
+    kinds = [line.expand(B, N, L).contiguous().cuda(), line.cuda(), line.cuda().int().expand(N, L), line.cuda()[None, None].expand(B, N, L), None]
+    first = None
+    for pos in kinds:
+        leaves = [t.cuda().requires_grad_(True) for t in (q, k, qw, kw)]
+        outs = mfb.qk_norm_rotary(*leaves, freq.cuda(), pos, 1e-6, interleaved)
+        grads = torch.autograd.grad(outs, leaves, [dq.cuda(), dk.cuda()])
+        if first is None:
+            first = (*outs, *grads[:2])
+            _compare(q, k, qw, kw, freq, line.expand(B, N, L), dq, dk, 1e-6, interleaved, leaves, outs, grads)
+            size = [(2 * d.double().abs().amax(-1, keepdim=True) * x.double().abs() * (x.double() ** 2).mean(-1, keepdim=True).rsqrt()).sum((0, 1, 2)) for d, x in ((dq, q), (dk, k))]
+            sums = grads[2:]
+        assert all(torch.equal(a, b) for a, b in zip((*outs, *grads[:2]), first))
+        for a, b, s in zip(grads[2:], sums, size):
+            _check(a, b.double().cpu(), 2 * 2.0 ** -24 * 256 * s + 2.0 ** -23 * b.abs().double().cpu(), "dw")
+
+
+@gpu
 @pytest.mark.parametrize("tokens", [3000, 20011])
 def test_many_tokens(tokens):
     """More tokens than threads of the backward's grid: each walks several."""
