@@ -136,8 +136,10 @@ __global__ void __launch_bounds__(kThreads, 4) relpos_fwd_kernel(const __grid_co
 // where positions run on.  It sums in registers and adds a sum to a column of its own of the block's table in shared memory when the row
 // changes (no atomics: the sums' order is fixed); walking down columns instead, a warp met such a change in most of its
 // steps and [2, 8, 1531, 1531] took 173 us.  The block's table goes to `parts` [gridDim.y * gridDim.x][H][rows].
-// Two rows of a thread are in registers, two more on their way into L2, and 512 threads of an SM have 128 registers each: [2, 8, 1531, 1531]
-// fp32 and 64 rows of the table 102 us, six rows ahead instead of four 103; three blocks of 80 registers 112, without the way into L2 120.
+// Bound by issue slots (the look-ups).  Where a block's positions run on without a gap it looks up what comes around the tile's end only: [2, 8, 1531, 1531] fp32
+// 51 us instead of 75, [1, 16, 4096, 4096] bf16 248 instead of 432 (buckets = 32).
+// Two rows of a thread are in registers, two more on their way into L2, and 512 threads of an SM have 128 registers each: with gaps and 64 rows of the
+// table 78 us (before tiles were fitted to the rows 102), six rows ahead instead of four 103; three blocks of 80 registers 112, without the way into L2 120.
 constexpr int kBwdCols = 8, kBwdAhead = 4, kBwdResident = 512;
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBwdResident / kThreads) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
@@ -160,9 +162,20 @@ __global__ void __launch_bounds__(kThreads, kBwdResident / kThreads) relpos_bwd_
   }
   fill_rows(p, lut, tmp, tid, nt);
   for (int x = tid; x < p.rows * nt; x += nt) table[x] = 0.f;
-  near = __syncthreads_and(near);
-  float* mine = table + tid;                       // the only column that this thread touches before the last barrier
   const int i0 = (int)((int64_t)p.Lq * strip / p.strips), end = (int)((int64_t)p.Lq * (strip + 1) / p.strips);
+  // run_on: each position is the one before and one, of the tile's keys and of the strip's queries
+  bool run_on = !p.k_seg && width > slots;
+  for (int i = i0 + tid; i < end; i += nt) {
+    const int64_t x = q_position(p, b, i);
+    near_to(x, o.pos, near);
+    if (p.q_seg) near_to(load_int(p.q_seg, b * p.qs_b + i, p.seg64), o.seg, near);
+    if (i + 1 < end) run_on = run_on && q_position(p, b, i + 1) - x == 1;
+  }
+  near = __syncthreads_and(near);
+  for (int x = tid; x + 1 < width; x += nt) run_on = run_on && kpos[x + 1] - kpos[x] == 1;
+  run_on = __syncthreads_and(run_on && near);
+  bool begun = false;
+  float* mine = table + tid;                       // the only column that this thread touches before the last barrier
   const T* in = d_bias + (((int64_t)b * p.H + h) * p.Lq) * p.Lk + j0;
   // column e of this thread at query i is lane + e * tpr + (i - i0), around the width
   const int columns = (width - lane + tpr - 1) >> p.log_tpr;       // of the tile's width; at most kC
@@ -178,56 +191,81 @@ __global__ void __launch_bounds__(kThreads, kBwdResident / kThreads) relpos_bwd_
   auto next = [&](Cursor& c) { c.i += slots; c.first = wrap(c.first + step); c.row += (int64_t)slots * p.Lk; };
   auto load = [&](Cursor& c, T (&x)[kC]) {
 #pragma unroll
-    for (int e = 0; e < kC; ++e) x[e] = c.i < end && e < columns ? c.row[wrap(c.first + e * tpr)] : from_f<T>(0.f);
+    for (int e = 0; e < kC; ++e) {
+      const bool there = c.i < end && e < columns;
+      const T* at = c.row + wrap(c.first + e * tpr);
+      x[e] = there ? *at : from_f<T>(0.f);
+    }
     next(c);
   };
   auto add = [&](Cursor& c, const T (&x)[kC]) {
-    bool close = near;
-    const int qp = near_to(q_position(p, b, c.i), o.pos, close), qs = p.q_seg ? near_to(load_int(p.q_seg, b * p.qs_b + c.i, p.seg64), o.seg, close) : 0;
-    int row[kC];
-    if (close) {
+    const auto q_at = [&]() { return (int)q_position(p, b, c.i) - (int)o.pos; };
+    // where positions run on, only the columns that came around in this step have another distance: the first, and the one behind which
+    // the tile ends (a bit a column; two at most, as they lie further apart than a step but for the last and the first)
+    uint32_t around = 0;
+    if (run_on && begun) {
+      const int k = width - c.first, e = (k + tpr - 1) >> p.log_tpr;
+      around = (c.first < step ? 1u : 0u) | (e < columns && (e << p.log_tpr) - k < step ? 1u << e : 0u);
+    }
+    if (!(run_on && begun)) {
+      int row[kC];
+      if (near) {
+        const int qp = q_at(), qs = p.q_seg ? (int)load_int(p.q_seg, b * p.qs_b + c.i, p.seg64) - (int)o.seg : 0;
 #pragma unroll
-      for (int e = 0; e < kC; ++e) row[e] = kpos[wrap_in(c.first + e * tpr, e)];
+        for (int e = 0; e < kC; ++e) row[e] = kpos[wrap_in(c.first + e * tpr, e)];
 #pragma unroll
-      for (int e = 0; e < kC; ++e) row[e] = row_of(p, lut, row[e] - qp);
-      if (p.q_seg) {
+        for (int e = 0; e < kC; ++e) row[e] = row_of(p, lut, row[e] - qp);
+        if (p.q_seg) {
+#pragma unroll
+          for (int e = 0; e < kC; ++e)
+            if (kseg[wrap_in(c.first + e * tpr, e)] != qs) row[e] = p.rows - 1;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kC; ++e) row[e] = row_of_far(p, lut, b, c.i, j0 + wrap_in(c.first + e * tpr, e));
+      }
+      bool moved = false;
+#pragma unroll
+      for (int e = 0; e < kC; ++e) moved = moved || row[e] != cur[e];
+      if (__any_sync(0xffffffffu, moved)) {        // a warp is in one row of the bias: tpr is 32 at least
 #pragma unroll
         for (int e = 0; e < kC; ++e)
-          if (kseg[wrap_in(c.first + e * tpr, e)] != qs) row[e] = p.rows - 1;
+          if (row[e] != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row[e]; acc[e] = 0.f; }
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kC; ++e) row[e] = row_of_far(p, lut, b, c.i, j0 + wrap_in(c.first + e * tpr, e));
-    }
-    bool moved = false;
-#pragma unroll
-    for (int e = 0; e < kC; ++e) moved = moved || row[e] != cur[e];
-    if (__any_sync(0xffffffffu, moved)) {          // a warp is in one row of the bias: tpr is 32 at least
+      begun = true;
+    } else if (__any_sync(0xffffffffu, around != 0)) {
+      const int qp = q_at();
 #pragma unroll
       for (int e = 0; e < kC; ++e)
-        if (row[e] != cur[e]) { mine[cur[e] * nt] += acc[e]; cur[e] = row[e]; acc[e] = 0.f; }
+        if (around >> e & 1) {
+          mine[cur[e] * nt] += acc[e];
+          acc[e] = 0.f;
+          cur[e] = row_of(p, lut, kpos[wrap(c.first + e * tpr)] - qp);
+        }
     }
 #pragma unroll
     for (int e = 0; e < kC; ++e) acc[e] += to_f(x[e]);             // zeros for columns that are not there
     next(c);
   };
-  auto ahead = [&](int i) {
-    for (int x = lane * 128; x < width * (int)sizeof(T); x += tpr * 128)
-      if (i < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(in + (int64_t)i * p.Lk) + x));
+  // a row of the tile is no more than tpr lines of 128 bytes
+  const bool asks = lane * 128 < width * (int)sizeof(T);
+  auto ahead = [&](int i, const T* row) {
+    if (asks && i < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(row) + lane * 128));
   };
-#pragma unroll
-  for (int k = 2; k < kBwdAhead; ++k) ahead(i0 + slot + k * slots);
   Cursor in_at = start(), sum_at = start();
+  const int64_t row_step = (int64_t)slots * p.Lk;
+#pragma unroll
+  for (int k = 2; k < kBwdAhead; ++k) ahead(in_at.i + k * slots, in_at.row + k * row_step);
   T x0[kC], x1[kC];                                // two rows under way
   load(in_at, x0);
   load(in_at, x1);
   while (sum_at.i < end) {
     add(sum_at, x0);
-    ahead(in_at.i + (kBwdAhead - 2) * slots);
+    ahead(in_at.i + (kBwdAhead - 2) * slots, in_at.row + (kBwdAhead - 2) * row_step);
     load(in_at, x0);
     if (sum_at.i >= end) break;
     add(sum_at, x1);
-    ahead(in_at.i + (kBwdAhead - 2) * slots);
+    ahead(in_at.i + (kBwdAhead - 2) * slots, in_at.row + (kBwdAhead - 2) * row_step);
     load(in_at, x1);
   }
 #pragma unroll
@@ -279,7 +317,12 @@ BwdPlan bwd_plan(RelP& p) {
   BwdPlan b;
   b.threads = kThreads;
   while (b.threads > 32 && (size_t)p.rows * b.threads * 4 > 72 * 1024) b.threads /= 2;
-  p.log_tpr = log_threads(p.Lk, kBwdCols, 5, b.threads);
+  // threads of a row: those that leave the least of the columns' places empty, with a step more where a column wraps around (one a row)
+  int64_t least = 0;
+  for (int l = 5; (1 << l) <= b.threads; ++l) {
+    const int64_t wide = (int64_t)kBwdCols << l, cost = (p.Lk + wide - 1) / wide * wide * (320 + (64 >> (l - 5)));
+    if (l == 5 || cost < least) { least = cost; p.log_tpr = l; }
+  }
   const int tpr = 1 << p.log_tpr, slots = b.threads >> p.log_tpr;
   b.smem = lut_bytes(p) + (size_t)p.rows * b.threads * 4 + (size_t)tpr * kBwdCols * (p.k_seg ? 8 : 4);
   b.tiles = (p.Lk + tpr * kBwdCols - 1) / (tpr * kBwdCols);

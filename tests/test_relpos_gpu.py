@@ -51,6 +51,34 @@ def test_bias_and_gradient(B, H, Lq, Lk, count, reach, scheme, both, segments, w
     assert torch.equal(first, again)                                        # summed in a fixed order
 
 
+@pytest.mark.parametrize("positions", ["none", "far away", "a gap in the keys", "a gap in the queries", "backwards", "from far to near"])
+@pytest.mark.parametrize("Lk", [1, 2, 5, 9, 31, 33, 65, 70, 257, 263, 513, 1025, 1531, 2049, 2055])
+@pytest.mark.parametrize("Lq", [1, 7, 300])
+def test_positions_that_run_on(Lq, Lk, positions):
+    """Every width of a tile around the places where columns come around its end.  The gradient's elements are small integers: all sums are exact."""
+    g = torch.Generator().manual_seed(Lq + Lk)
+    k, q = torch.arange(Lk), torch.arange(Lq) + Lk - Lq
+    if positions == "far away":
+        k, q = k + (1 << 41), q + (1 << 41)
+    elif positions == "a gap in the keys":
+        k = k + (k >= Lk // 2) * 3
+    elif positions == "a gap in the queries":
+        q = q + (torch.arange(Lq) >= Lq - Lq // 3) * 2
+    elif positions == "backwards":
+        k, q = -k, -q
+    elif positions == "from far to near":
+        q = q - (torch.arange(Lq) < Lq // 2).long() * (1 << 33)
+    w = torch.zeros(24, 2, device="cuda", requires_grad=True)
+    d = torch.randint(-8, 9, (1, 1, 2, Lq, Lk), generator=g)
+    rows = orc.buckets(q[None], k[None], 24, 100, "log", True)
+    want = torch.stack([torch.bincount(rows.flatten(), d[0, 0, h].flatten().double(), minlength=24) for h in range(2)], 1)
+    args = (Lq, Lk) if positions == "none" else (q.cuda(), k.cuda())
+    for dt in (torch.bfloat16, torch.float32):
+        got = mfb.relative_position_bias(w, *args, max_distance=100, scheme="log", dtype=dt)
+        grad, = torch.autograd.grad(got, w, d.cuda().to(dt))
+        assert torch.equal(grad.cpu().double(), want)
+
+
 def test_lengths_instead_of_positions_and_one_row_of_positions_for_the_batch():
     w = torch.randn(32, 3, device="cuda")
     a = mfb.relative_position_bias(w, 5, 40, max_distance=128)
