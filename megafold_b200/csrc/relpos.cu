@@ -48,15 +48,18 @@ __device__ __forceinline__ int near_to(int64_t x, int64_t from, bool& near) {
 __device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int32_t* tmp, int tid, int nt) {
   for (int x = tid; x < p.n_edges; x += nt) tmp[x] = p.edges[x];
   __syncthreads();
-  for (int x = tid; x <= 2 * p.reach; x += nt) {
-    const int d = x - p.reach, n = d < 0 ? -d : d;
-    int lo = 0, hi = p.n_edges;                  // edges not above n
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (tmp[mid] <= n) lo = mid + 1; else hi = mid;
-    }
-    const int r = d > 0 ? p.base_pos + p.step_pos * lo : p.base_neg + p.step_neg * lo;
-    lut[x] = (uint16_t)(r < 0 ? 0 : r >= p.rows ? p.rows - 1 : r);
+  // a thread fills adjacent distances of both signs, with one search among the edges
+  const auto row = [&](int base, int by, int k) { const int r = base + by * k; return (uint16_t)(r < 0 ? 0 : r >= p.rows ? p.rows - 1 : r); };
+  const int run = (p.reach + nt) / nt, to = run * (tid + 1) <= p.reach ? run * (tid + 1) : p.reach + 1;
+  int n = run * tid, k = 0;                      // k edges are not above n
+  for (int hi = p.n_edges; n < to && k < hi;) {
+    const int mid = (k + hi) >> 1;
+    if (tmp[mid] <= n) k = mid + 1; else hi = mid;
+  }
+  for (; n < to; ++n) {
+    while (k < p.n_edges && tmp[k] <= n) ++k;
+    if (n) lut[p.reach + n] = row(p.base_pos, p.step_pos, k);
+    lut[p.reach - n] = row(p.base_neg, p.step_neg, k);
   }
 }
 __device__ __forceinline__ int row_of(const RelP& p, const uint16_t* lut, int d) { return lut[(d < -p.reach ? -p.reach : d > p.reach ? p.reach : d) + p.reach]; }
@@ -353,7 +356,10 @@ int run_fwd(const mf_relpos_args& a, cudaStream_t st) {
   const int64_t row_blocks = (p.Lq + slots - 1) / slots, want = 4 * (int64_t)tcx::sm_count();
   while (heads > 1 && row_blocks * tiles * p.B * ((p.H + heads - 1) / heads) < want) heads = (heads + 1) / 2;
   const int groups = (p.H + heads - 1) / heads;
-  int64_t strips = (2 * want + (int64_t)tiles * groups * p.B - 1) / ((int64_t)tiles * groups * p.B);
+  // one wave of blocks, or two where a block of one would write more than 384 KB: a wave begins with some 4 us of tables ([2, 8, 1531, 1531]
+  // bf16 28 us instead of 33), two end more evenly ([4, 8, 1536, 1536] fp32 55 us instead of 65)
+  const int64_t waves = (int64_t)p.B * p.H * p.Lq * p.Lk * (int)sizeof(T) > want * (384 << 10) ? 2 : 1;
+  int64_t strips = (waves * want + (int64_t)tiles * groups * p.B - 1) / ((int64_t)tiles * groups * p.B);
   if (strips > row_blocks) strips = row_blocks;
   if (strips > 65535 / p.B) strips = 65535 / p.B;
   p.strips = (int)(strips < 1 ? 1 : strips);
