@@ -12,9 +12,9 @@ constexpr int kThreads = 256;
 constexpr int kTile = 64;
 constexpr int kPPitch = kTile + 4;
 
-// Rows [row0, row0 + 64) x [0, DP) of a [.., L, H, D] operand as fp32, zero outside L and D and where ok(row) is false.
-template <typename T, int DP, typename Ok>
-__device__ __forceinline__ void load_tile_where(float* dst, const void* src, const int64_t* s, bool vec, int b, int n, int h, int row0, int L, int D, Ok ok) {
+// Rows [row0, row0 + 64) x [0, DP) of a [.., L, H, D] operand as fp32, zero outside L and D.
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const void* src, const int64_t* s, bool vec, int b, int n, int h, int row0, int L, int D) {
   constexpr int pitch = DP + 4;
   const T* base = static_cast<const T*>(src) + b * s[0] + n * s[1] + h * s[3];
 #pragma unroll
@@ -23,7 +23,7 @@ __device__ __forceinline__ void load_tile_where(float* dst, const void* src, con
     const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4;
     const int l = row0 + r;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (l < L && d < D && ok(l)) {
+    if (l < L && d < D) {
       const T* p = base + l * s[2];
       if (vec) {
         __align__(16) T e[4];
@@ -39,11 +39,6 @@ __device__ __forceinline__ void load_tile_where(float* dst, const void* src, con
     }
     *reinterpret_cast<float4*>(dst + r * pitch + d) = v;
   }
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(float* dst, const void* src, const int64_t* s, bool vec, int b, int n, int h, int row0, int L, int D) {
-  load_tile_where<T, DP>(dst, src, s, vec, b, n, h, row0, L, D, [](int) { return true; });
 }
 
 // acc[a][b] += sum_d A[ty + 16 a][d] B[tx + 16 b][d]
@@ -69,8 +64,11 @@ __device__ __forceinline__ void dot_tile(const float* A, const float* B, int ty,
   }
 }
 
-// acc[a][e] += sum_c P[ty + 16 a][c] V[c][d], the thread's DP / 16 head columns d = tx * DP / 16 + e
-template <int DP>
+// The DP / 16 head columns of a thread: adjacent ones, or (SPREAD) fours of them, 64 apart, so that eight threads read 128 adjacent bytes
+template <int DP> __device__ __forceinline__ int column(int tx, int e) { return DP <= 64 ? tx * (DP / 16) + e : e / 4 * 64 + tx * 4 + e % 4; }
+
+// acc[a][e] += sum_c P[ty + 16 a][c] V[c][d], d = tx * DP / 16 + e or (SPREAD) column(tx, e)
+template <int DP, bool SPREAD = false>
 __device__ __forceinline__ void sum_tile(const float* P, const float* V, int ty, int tx, float (&acc)[4][DP / 16]) {
   constexpr int pitch = DP + 4, E = DP / 16;
 #pragma unroll 4
@@ -81,12 +79,12 @@ __device__ __forceinline__ void sum_tile(const float* P, const float* V, int ty,
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       float v[E];
-      const float* row = V + (c + k) * pitch + tx * E;
+      const float* row = V + (c + k) * pitch + (SPREAD && E > 4 ? tx * 4 : tx * E);
       if constexpr (E == 2) { const float2 t = *reinterpret_cast<const float2*>(row); v[0] = t.x; v[1] = t.y; }
       else {
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(row + e);
+          const float4 t = *reinterpret_cast<const float4*>(row + (SPREAD ? e * 16 : e));
           v[e] = t.x; v[e + 1] = t.y; v[e + 2] = t.z; v[e + 3] = t.w;
         }
       }

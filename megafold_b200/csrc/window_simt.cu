@@ -4,7 +4,8 @@
 // Tiles and products are those of the dense attention's CUDA-core kernels.  Forward: a block per (b, n, 64 rows of queries) walks the
 // key tiles that its rows see, with the running maximum and sum of the softmax.  Backward, two kinds of blocks in one launch:
 // dQ per 64 rows of queries, and dK / dV per 64 keys and chunk of their list of query blocks.  Nothing is added atomically: every
-// result is a sum in a fixed order.  Bound: FP32 issue (66 % of it goes to the multiply-adds).
+// result is a sum in a fixed order.  Bound: issue slots (62 to 65 % at [1, 2000, 8, 64], window 300 both ways) and reads of shared memory (63 to 72 % of
+// the L1's rate), with the FP32 pipe busy 41 to 47 %.
 //
 // Masked keys, and those of a tile that none of its queries sees, are read as zeros: whatever their rows hold (NaN, too) reaches nothing.  A row that sees no key gives 0, and a
 // log-sum-exp of -inf, and passes no gradient.
@@ -23,32 +24,65 @@ __device__ __forceinline__ Row query_row(const WinP& p, int i0, int h0, int r) {
   const int l = r / p.pack;
   return Row{l < queries_of<kTile>(p) ? i0 + l : p.Lq, h0 + r - l * p.pack};
 }
-template <typename T, int DP>
-__device__ __forceinline__ void load_queries(float* dst, const void* src, const int64_t* s, bool vec, const WinP& p, int b, int n, int i0, int h0) {
-  constexpr int pitch = DP + 4;
-  const T* base = static_cast<const T*>(src) + b * s[0] + n * s[1];
+// kept, for any j; reads the mask without a branch on j
+__device__ __forceinline__ bool there(const WinP& p, int b, int n, int j) { return j < p.Lk & kept(p, b, n, j < p.Lk ? j : p.Lk - 1); }
+
+// 64 rows as fp32, zero outside D and where there is none: at(r) is row r's first element or NULL.  The addresses come first, then the loads, then
+// the stores: with a mask's byte awaited before each load, the forward of [1, 2720, 16 : 4, 128] took 3.4 ms instead of 2.8.
+template <typename T, int DP, typename At>
+__device__ __forceinline__ void load_rows(float* dst, bool vec, int64_t sd, int D, At at) {
+  constexpr int pitch = DP + 4, kAll = kTile * DP / 4 / kThreads, kOnce = kAll < 4 ? kAll : 4;
 #pragma unroll
-  for (int it = 0; it < kTile * DP / 4 / kThreads; ++it) {
-    const int idx = it * kThreads + threadIdx.x;
-    const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4;
-    const Row q = query_row(p, i0, h0, r);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (q.i < p.Lq && d < p.D) {
-      const T* at = base + q.i * s[2] + q.h * s[3];
+  for (int i0 = 0; i0 < kAll; i0 += kOnce) {
+    const T* from[kOnce];
+    float4 v[kOnce];
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) {
+      const int idx = (i0 + i) * kThreads + threadIdx.x, d = idx % (DP / 4) * 4;
+      const T* row = at(idx / (DP / 4));
+      from[i] = row && d < D ? row + d * sd : nullptr;
+    }
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) {
+      const int d = ((i0 + i) * kThreads + threadIdx.x) % (DP / 4) * 4;
+      const T* p = from[i];
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (vec) {
-        __align__(16) T e[4];
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(at + d));
-        else *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(at + d));
-        v = make_float4(to_f(e[0]), to_f(e[1]), to_f(e[2]), to_f(e[3]));
-      } else {
-        v.x = to_f(at[d * s[4]]);
-        if (d + 1 < p.D) v.y = to_f(at[(d + 1) * s[4]]);
-        if (d + 2 < p.D) v.z = to_f(at[(d + 2) * s[4]]);
-        if (d + 3 < p.D) v.w = to_f(at[(d + 3) * s[4]]);
+        if constexpr (sizeof(T) == 4) {
+          if (p) v[i] = __ldg(reinterpret_cast<const float4*>(p));
+        } else {
+          uint2 w = make_uint2(0u, 0u);
+          if (p) w = __ldg(reinterpret_cast<const uint2*>(p));
+          __align__(8) T e[4];
+          *reinterpret_cast<uint2*>(e) = w;
+          v[i] = make_float4(to_f(e[0]), to_f(e[1]), to_f(e[2]), to_f(e[3]));
+        }
+      } else if (p) {
+        v[i].x = to_f(p[0]);
+        if (d + 1 < D) v[i].y = to_f(p[sd]);
+        if (d + 2 < D) v[i].z = to_f(p[2 * sd]);
+        if (d + 3 < D) v[i].w = to_f(p[3 * sd]);
       }
     }
-    *reinterpret_cast<float4*>(dst + r * pitch + d) = v;
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) {
+      const int idx = (i0 + i) * kThreads + threadIdx.x;
+      *reinterpret_cast<float4*>(dst + idx / (DP / 4) * pitch + idx % (DP / 4) * 4) = v[i];
+    }
   }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void load_queries(float* dst, const void* src, const int64_t* s, bool vec, const WinP& p, int b, int n, int i0, int h0) {
+  const T* base = static_cast<const T*>(src) + b * s[0] + n * s[1];
+  load_rows<T, DP>(dst, vec, s[4], p.D, [&](int r) {
+    const Row q = query_row(p, i0, h0, r);
+    return q.i < p.Lq ? base + q.i * s[2] + q.h * s[3] : nullptr;
+  });
+}
+template <typename T, int DP, typename Keep>
+__device__ __forceinline__ void load_keys(float* dst, const void* src, const int64_t* s, bool vec, const WinP& p, int b, int n, int hk, int j0, Keep keep) {
+  const T* base = static_cast<const T*>(src) + b * s[0] + n * s[1] + hk * s[3];
+  load_rows<T, DP>(dst, vec, s[4], p.D, [&](int r) { return keep(j0 + r) ? base + (j0 + r) * s[2] : nullptr; });
 }
 
 template <typename T, int DP>
@@ -61,7 +95,7 @@ __device__ __forceinline__ void store_keys(void* out, const WinP& p, int64_t bn,
     T* row = static_cast<T*>(out) + ((bn * p.Lk + l) * p.Hk + h) * D;
 #pragma unroll
     for (int e = 0; e < DP / 16; ++e) {
-      const int d = tx * (DP / 16) + e;
+      const int d = column<DP>(tx, e);
       if (d < D) row[d] = from_f<T>(acc[a][e] * f);
     }
   }
@@ -76,24 +110,28 @@ __device__ __forceinline__ void store_queries(void* out, const WinP& p, int64_t 
     T* row = static_cast<T*>(out) + ((bn * p.Lq + q.i) * p.H + q.h) * D;
 #pragma unroll
     for (int e = 0; e < DP / 16; ++e) {
-      const int d = tx * (DP / 16) + e;
+      const int d = column<DP>(tx, e);
       if (d < D) row[d] = from_f<T>(acc[a][e] * f[a]);
     }
   }
 }
 
+// Heads of more than 64 have one buffer for a tile's keys and then its values, so that two blocks fit an SM
+// ([1, 2720, 16 : 4, 128], window 2043: 2.83 -> 2.55 ms)
+constexpr bool one_buffer(int DP) { return DP > 64; }
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_constant__ WinP p, const Split sp) {
+__global__ void __launch_bounds__(kThreads, 2) window_fwd_simt_kernel(const __grid_constant__ WinP p, const Split sp) {
   extern __shared__ __align__(16) float smem[];
   constexpr int kOp = kTile * (DP + 4);
-  float *Qs = smem, *Ks = Qs + kOp, *Vs = Ks + kOp, *Ps = Vs + kOp;
+  constexpr bool kOne = one_buffer(DP);
+  float *Qs = smem, *Ks = Qs + kOp, *Vs = kOne ? Ks : Ks + kOp, *Ps = Vs + kOp;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int h0 = blockIdx.y * p.pack, hk = h0 / p.G, bn = blockIdx.z, b = bn / p.N, n = bn - b * p.N;
   const int part = blockIdx.x % sp.splits, i0 = blockIdx.x / sp.splits * queries_of<kTile>(p);
   const int i1 = i0 + queries_of<kTile>(p) < p.Lq ? i0 + queries_of<kTile>(p) : p.Lq;
   load_queries<T, DP>(Qs, p.q, p.qs, p.q_vec, p, b, n, i0, h0);
   const KeyRange range = key_range(p, i0, i1);
-  const auto keep = [&](int j) { return in_range(range, j) && kept(p, b, n, j); };
+  const auto keep = [&](int j) { return in_range(range, j) & there(p, b, n, j); };
   float acc[4][DP / 16], m[4], l[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
@@ -109,11 +147,11 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
   for (int t = (int)((int64_t)tiles.count() * part / sp.splits); t < t_end; ++t) {
     const int j0 = tiles.at(t) * kTile;
     __syncthreads();
-    load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
-    load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    load_keys<T, DP>(Ks, p.k, p.ks, p.k_vec, p, b, n, hk, j0, keep);
+    if (!kOne) load_keys<T, DP>(Vs, p.v, p.vs, p.v_vec, p, b, n, hk, j0, keep);
     bool see[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) see[c] = j0 + tx + 16 * c < p.Lk && keep(j0 + tx + 16 * c);
+    for (int c = 0; c < 4; ++c) see[c] = keep(j0 + tx + 16 * c);
     __syncthreads();
     float s[4][4] = {};
     dot_tile<DP>(Qs, Ks, ty, tx, s);
@@ -136,8 +174,14 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
 #pragma unroll
       for (int e = 0; e < DP / 16; ++e) acc[a][e] *= corr;
     }
-    __syncwarp();                // a row's probabilities are written and read by the same half warp
-    sum_tile<DP>(Ps, Vs, ty, tx, acc);
+    if (kOne) {
+      __syncthreads();
+      load_keys<T, DP>(Vs, p.v, p.vs, p.v_vec, p, b, n, hk, j0, keep);
+      __syncthreads();
+    } else {
+      __syncwarp();              // a row's probabilities are written and read by the same half warp
+    }
+    sum_tile<DP, true>(Ps, Vs, ty, tx, acc);
   }
   float inv[4];
 #pragma unroll
@@ -151,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) window_fwd_simt_kernel(const __grid_
       float* row = sp.row(part, r, p.D);
 #pragma unroll
       for (int e = 0; e < DP / 16; ++e)
-        if (tx * (DP / 16) + e < p.D) row[tx * (DP / 16) + e] = acc[a][e] * inv[a];
+        if (column<DP>(tx, e) < p.D) row[column<DP>(tx, e)] = acc[a][e] * inv[a];
       if (tx == 0) sp.lse(part, r, p.D) = m[a] + logf(l[a]);
     }
     return;
@@ -171,6 +215,16 @@ __device__ __forceinline__ void p_ds(const WinP& p, bool see, float s, float dp,
   ds = see ? pr * (dp - dl) : 0.f;
 }
 
+template <int DP>
+__device__ __forceinline__ void add_tile(const float* P, const float* V, int ty, int tx, float (&acc)[4][DP / 16]) {
+  float sum[4][DP / 16] = {};
+  sum_tile<DP, true>(P, V, ty, tx, sum);
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) acc[a][e] += sum[a][e];
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* parts, float* smem, int bn, int hk, int x) {
   constexpr int kOp = kTile * (DP + 4);
@@ -180,16 +234,16 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
   plan_item(c, x, tile, part);
   const int j0 = tile * kTile, len = list_length<kTile, kTile>(p, tile), e0 = part * c.chunk;
   if (part > 0 && e0 >= len) return;
-  const auto keep = [&](int j) { return kept(p, b, n, j); };
-  load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
-  load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+  const auto keep = [&](int j) { return there(p, b, n, j); };
+  load_keys<T, DP>(Ks, p.k, p.ks, p.k_vec, p, b, n, hk, j0, keep);
+  load_keys<T, DP>(Vs, p.v, p.vs, p.v_vec, p, b, n, hk, j0, keep);
   int lo, hi;
   query_range(p, j0, j0 + kTile < p.Lk ? j0 + kTile : p.Lk, lo, hi);
   const int nq = queries_of<kTile>(p), first = lo / nq, per_head = hi > lo ? (hi + nq - 1) / nq - first : 1;
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   bool see[4];
 #pragma unroll
-  for (int a = 0; a < 4; ++a) see[a] = j0 + ty + 16 * a < p.Lk && keep(j0 + ty + 16 * a);
+  for (int a = 0; a < 4; ++a) see[a] = keep(j0 + ty + 16 * a);
   for (int e = e0; e < len && e < e0 + c.chunk; ++e) {
     const int h0 = hk * p.G + e / per_head * p.pack, i0 = (first + e % per_head) * nq;
     __syncthreads();
@@ -220,8 +274,9 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
         Ds[(ty + 16 * a) * kPPitch + tx + 16 * k] = ds;
       }
     __syncwarp();
-    sum_tile<DP>(Ps, Gs, ty, tx, dv);
-    sum_tile<DP>(Ds, Qs, ty, tx, dk);
+    // a tile's sum on its own: a key with the sinks' list sums thousands of rows, and one running sum of [1, 2720, 16 : 4, 128] was 1.4e-6 off, this is 6e-7
+    add_tile<DP>(Ps, Gs, ty, tx, dv);
+    add_tile<DP>(Ds, Qs, ty, tx, dk);
   }
   if (x < c.split_x) {
     float* out = part_of<kTile>(parts, c, p, (int64_t)bn * p.Hk + hk, x);
@@ -229,7 +284,7 @@ __device__ __forceinline__ void bwd_dkv(const WinP& p, const KeyPlan& c, float* 
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int e = 0; e < DP / 16; ++e) {
-        const int d = tx * (DP / 16) + e, row = ty + 16 * a;
+        const int d = column<DP>(tx, e), row = ty + 16 * a;
         if (d < p.D) { out[row * p.D + d] = dk[a][e]; out[(kTile + row) * p.D + d] = dv[a][e]; }
       }
     return;
@@ -248,7 +303,7 @@ __device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h
   const int64_t gs[5] = {(int64_t)p.N * p.Lq * p.H * p.D, (int64_t)p.Lq * p.H * p.D, (int64_t)p.H * p.D, p.D, 1};
   load_queries<T, DP>(Gs, p.d_o, gs, p.g_vec, p, b, n, i0, h0);
   const KeyRange range = key_range(p, i0, i1);
-  const auto keep = [&](int j) { return in_range(range, j) && kept(p, b, n, j); };
+  const auto keep = [&](int j) { return in_range(range, j) & there(p, b, n, j); };
   float dq[4][DP / 16] = {}, lse[4], dl[4];
   int at[4];
 #pragma unroll
@@ -262,11 +317,11 @@ __device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h
   for (int t = 0; t < tiles.count(); ++t) {
     const int j0 = tiles.at(t) * kTile;
     __syncthreads();
-    load_tile_where<T, DP>(Ks, p.k, p.ks, p.k_vec, b, n, hk, j0, p.Lk, p.D, keep);
-    load_tile_where<T, DP>(Vs, p.v, p.vs, p.v_vec, b, n, hk, j0, p.Lk, p.D, keep);
+    load_keys<T, DP>(Ks, p.k, p.ks, p.k_vec, p, b, n, hk, j0, keep);
+    load_keys<T, DP>(Vs, p.v, p.vs, p.v_vec, p, b, n, hk, j0, keep);
     bool see[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) see[c] = j0 + tx + 16 * c < p.Lk && keep(j0 + tx + 16 * c);
+    for (int c = 0; c < 4; ++c) see[c] = keep(j0 + tx + 16 * c);
     __syncthreads();
     float s[4][4] = {}, dp[4][4] = {};
     dot_tile<DP>(Qs, Ks, ty, tx, s);
@@ -280,15 +335,16 @@ __device__ __forceinline__ void bwd_dq(const WinP& p, float* smem, int bn, int h
         Ds[(ty + 16 * a) * kPPitch + tx + 16 * c] = ds;
       }
     __syncwarp();
-    sum_tile<DP>(Ds, Ks, ty, tx, dq);
+    sum_tile<DP, true>(Ds, Ks, ty, tx, dq);
   }
   const float sc[4] = {p.scale, p.scale, p.scale, p.scale};
   store_queries<T, DP>(p.dq, p, bn, i0, h0, ty, tx, dq, sc);
 }
 
 // blocks [0, n_dkv) work on dK and dV (the longest first: tiles with sinks lead), the others on dQ
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) window_bwd_simt_kernel(const __grid_constant__ WinP p, const KeyPlan c, float* parts, int64_t n_dkv) {
+// R: blocks of an SM
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(kThreads, R) window_bwd_simt_kernel(const __grid_constant__ WinP p, const KeyPlan c, float* parts, int64_t n_dkv) {
   extern __shared__ __align__(16) float smem[];
   const int64_t u = blockIdx.x;
   const int64_t heads = (int64_t)p.B * p.N * p.Hk;
@@ -378,7 +434,7 @@ template <typename T>
 int run_fwd(const WinP& p, const Split& sp, cudaStream_t st) {
   const auto go = [&](auto dp) -> int {
     constexpr int DP = decltype(dp)::value;
-    constexpr size_t smem = sizeof(float) * (3 * kTile * (DP + 4) + kTile * kPPitch);
+    constexpr size_t smem = sizeof(float) * ((one_buffer(DP) ? 2 : 3) * kTile * (DP + 4) + kTile * kPPitch);
     constexpr auto kern = window_fwd_simt_kernel<T, DP>;
     if (int e = opt_in_smem<kern>(smem)) return e;
     const int q = queries_of<kTile>(p);
@@ -396,14 +452,22 @@ int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
   const auto go = [&](auto dp) -> int {
     constexpr int DP = decltype(dp)::value;
     constexpr size_t smem = sizeof(float) * (4 * kTile * (DP + 4) + 2 * kTile * kPPitch);
-    constexpr auto kern = window_bwd_simt_kernel<T, DP>;
-    if (int e = opt_in_smem<kern>(smem)) return e;
     const int64_t n_dkv = (int64_t)c.x_total * p.B * p.N * p.Hk, q = queries_of<kTile>(p);
     const int64_t blocks = n_dkv + (int64_t)((p.Lq + q - 1) / q) * p.B * p.N * head_groups(p);
     MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%lld blocks of 64 rows are more than one launch takes", (long long)blocks);
-    kern<<<(unsigned)blocks, kThreads, smem, st>>>(p, c, parts, n_dkv);
-    MF_LAUNCHED("window_bwd_simt_kernel");
-    return MF_OK;
+    const auto launch = [&](auto resident) -> int {
+      constexpr auto kern = window_bwd_simt_kernel<T, DP, decltype(resident)::value>;
+      if (int e = opt_in_smem<kern>(smem)) return e;
+      kern<<<(unsigned)blocks, kThreads, smem, st>>>(p, c, parts, n_dkv);
+      MF_LAUNCHED("window_bwd_simt_kernel");
+      return MF_OK;
+    };
+    // Two blocks an SM have 128 registers a thread, too few for a block alone: [2, 517, 8 : 2, 24], window 100, 61 us instead of 50, but with 8 times as many tiles
+    // ([1, 2000, 8 : 1, 32], window 300) 137 instead of 172 and [1, 2000, 8, 64] 382 instead of 435.
+    if constexpr (DP <= 64) {
+      if (blocks > 3 * (int64_t)tcx::sm_count()) return launch(std::integral_constant<int, 2>{});
+    }
+    return launch(std::integral_constant<int, 1>{});
   };
   int r = p.D <= 32 ? go(std::integral_constant<int, 32>{}) : p.D <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
   return r ? r : window_join<T, kTile, kTile>(p, c, parts, st);
