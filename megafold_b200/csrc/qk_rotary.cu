@@ -305,7 +305,9 @@ __global__ void __launch_bounds__(kThreads, resident(V, sizeof(T), BWD)) qk_rota
       to = out + arr;
     }
     fetch(at, dp, live, xr, dr);
-    const float rstd = rsqrtf(fmaf(row_sum(ss2.x + ss2.y, lpr), inv_d, p.eps));
+    const float ss = row_sum(ss2.x + ss2.y, lpr);              // of every lane, whether its row exists or not
+    float rstd = rsqrtf(fmaf(ss, inv_d, p.eps));
+    if (BWD && !now) rstd = 0.f;                               // adds nothing to the weights' gradients, also without an eps: 0 * inf would
     const float2 rstd2 = make_float2(rstd, rstd);
     float2 dot2 = make_float2(0.f, 0.f);
 #pragma unroll
