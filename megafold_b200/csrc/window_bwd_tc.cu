@@ -23,7 +23,10 @@
 //
 // Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they, and those that no query of the tile sees, are overwritten
 // with zeros in shared memory.
-// P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  Waits are bounded as in the forward.
+// P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  The factor D^-1/2 of dQ and dK
+// comes last in bf16, which has the range of fp32, but goes into dS before it is rounded in fp16: with the gradients of a scaled loss, dS without
+// it overflowed up to sqrt(D) before dQ and dK did.  (In bf16, too, it cost 1 % at 16384 tokens, 16 heads of 64, window 1024: 553 -> 559 us forward
+// and backward.)  Waits are bounded as in the forward.
 #include <type_traits>
 
 #include "window_tc_common.cuh"
@@ -38,6 +41,8 @@ constexpr int kQB = 64;             // ... and rows of queries of a block
 constexpr int kRows = 128;          // dQ kernel: rows of queries of a CTA
 constexpr int kKB = 64;             // ... and keys of a block
 constexpr int kXB = kQB * 32;       // bytes of a block's term tile
+
+template <typename T> constexpr bool kScaledDs = std::is_same<T, __half>::value;
 
 struct BwdP {
   WinP w;
@@ -265,7 +270,9 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
       for (int e = 0; e < 32; e += 2) {
         float2 pr = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(f.c1, f.c1));
         pr = make_float2(ex2f(pr.x), ex2f(pr.y));
-        float2 ds = mul2(pr, make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])));
+        float2 dp = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
+        if constexpr (kScaledDs<T>) dp = mul2(dp, make_float2(p.scale, p.scale));
+        float2 ds = mul2(pr, dp);
         if (!whole) {
           if (!(bits >> e & 1)) pr.x = ds.x = 0.f;
           if (!(bits >> (e + 1) & 1)) pr.y = ds.y = 0.f;
@@ -303,7 +310,7 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
         if (T_ > 0) {
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c)
-            if (c * 32 < p.D) store_rows<T>(acc + c * 32, half ? 1.f : p.scale, out + c * 32, (int64_t)p.Hk * p.D, j, p.Lk, p.D - c * 32);
+            if (c * 32 < p.D) store_rows<T>(acc + c * 32, half || kScaledDs<T> ? 1.f : p.scale, out + c * 32, (int64_t)p.Hk * p.D, j, p.Lk, p.D - c * 32);
         } else if (j < p.Lk) {
           for (int e = 0; e < p.D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -436,11 +443,12 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
     const int half = warp >> 2, r = (warp & 3) * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const bool live = l_ < nq && i < p.Lq;
-    float lse = -INFINITY, delta = 0.f;
+    float lse = -INFINITY, minus = 0.f;           // minus: -delta, with dS's factor
+    const float factor = kScaledDs<T> ? p.scale : 1.f;
     const int64_t stat = ((int64_t)bn * p.H + h) * p.Lq + i;
     if (live) {
       lse = p.lse[stat];
-      if (!f.two_walks) delta = p.delta[stat];
+      if (!f.two_walks) minus = -p.delta[stat] * factor;
     }
     float sum = 0.f;                              // of P dP over this thread's columns
     const float off = lse == -INFINITY ? -INFINITY : -lse * kLog2e;       // a row that sees nothing: probability 0
@@ -463,8 +471,9 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
         mbar_arrive(&bar.summed);
         wait_or_flag(&bar.summed, 0, abort_flag);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
-        delta = sum + sums[half ^ 1][r];
+        const float delta = sum + sums[half ^ 1][r];
         if (half == 0 && live) f.delta[stat] = delta;
+        minus = -delta * factor;
       }
       wait_or_flag(&bar.s_ready, t & 1, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag)) break;
@@ -478,7 +487,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       mbar_arrive(&bar.s_read);
       const bool whole = all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + 32) && keep == ~0u;
       const uint32_t bits = whole ? ~0u : seen32(p, at, j0) & keep;
-      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off), d2 = make_float2(delta, delta);
+      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off), f2 = make_float2(factor, factor), d2 = make_float2(minus, minus);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
@@ -509,7 +518,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       uint32_t w[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
-        float2 ds = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sub2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), d2));
+        float2 ds = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fma2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), f2, d2));
         if (!whole) {
           if (!(bits >> e & 1)) ds.x = 0.f;
           if (!(bits >> (e + 1) & 1)) ds.y = 0.f;
@@ -545,7 +554,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)            // the two warps of a set of lanes take alternate columns
           if (c % 2 == half % (DP / 32 > 1 ? 2 : 1) && (DP > 32 || half == 0) && c * 32 < p.D)
-            store_rows_at<T>(tQ + lanes + c * 32, p.scale, live ? out + c * 32 : nullptr, p.D - c * 32);
+            store_rows_at<T>(tQ + lanes + c * 32, kScaledDs<T> ? 1.f : p.scale, live ? out + c * 32 : nullptr, p.D - c * 32);
       } else if (live && half == 0) {
         for (int e = 0; e < p.D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0u, 0u, 0u, 0u);
         if (f.two_walks) f.delta[stat] = 0.f;
@@ -628,7 +637,7 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   }
   dkv<<<(unsigned)grid_kv, kThreads, KvCfg<DP>::SMEM, st>>>(mk, mv, mq64, mg64, f);
   MF_LAUNCHED("window_dkv_tc_kernel");
-  return window_join<T, kKeys, kQB>(p, f.plan, f.parts, st);
+  return window_join<T, kKeys, kQB>(p, f.plan, f.parts, kScaledDs<T> ? 1.f : p.scale, st);
 }
 template <typename T>
 int by_size(const mf_window_args& a, cudaStream_t st) {
