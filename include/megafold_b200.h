@@ -281,7 +281,7 @@ MF_API int mf_bias_layout(void* rows, void* planes, int32_t L, int32_t np, int32
  * bias, d_bias: contiguous [B,1,H,Lq,Lk] in `dtype`.  d_weight [rows, H] in dw_dtype, fully overwritten, summed in a fixed
  * order (bit-reproducible).  workspace (backward): mf_relpos_bwd_workspace_bytes() bytes, 256-byte aligned.
  * ------------------------------------------------------------------------------------------ */
-#define MF_RELPOS_MAX_EDGES 512
+#define MF_RELPOS_MAX_EDGES 1023
 #define MF_RELPOS_MAX_ROWS 1024
 #define MF_RELPOS_MAX_DISTANCE 16384
 typedef struct mf_relpos_args {

@@ -23,8 +23,9 @@ struct RelP {
   bool pos64, seg64;
   int log_tpr;                       // threads of a block that share a row of the bias
   int strips;                        // blocks along the queries of a batch element
-  int edges[MF_RELPOS_MAX_EDGES];
+  uint16_t edges[MF_RELPOS_MAX_EDGES];
 };
+static_assert(MF_RELPOS_MAX_EDGES == MF_RELPOS_MAX_ROWS - 1 && MF_RELPOS_MAX_DISTANCE <= 65535, "one direction has a border between any two rows");
 
 __device__ __forceinline__ int64_t load_int(const void* p, int64_t i, bool wide) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
@@ -45,7 +46,7 @@ __device__ __forceinline__ int near_to(int64_t x, int64_t from, bool& near) {
 
 // Rows of the distances -reach .. reach.  The edges go through shared memory (`tmp`): read at an index that differs by lane from the
 // kernel's parameters, 1600 distances took each block some 5 us.
-__device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, int32_t* tmp, int tid, int nt) {
+__device__ __forceinline__ void fill_rows(const RelP& p, uint16_t* lut, uint16_t* tmp, int tid, int nt) {
   for (int x = tid; x < p.n_edges; x += nt) tmp[x] = p.edges[x];
   __syncthreads();
   // a thread fills adjacent distances of both signs, with one search among the edges
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 4) relpos_fwd_kernel(const __grid_co
   using C = Cols<T, VEC>;
   constexpr int kC = C::kC;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  __shared__ uint16_t tmp[MF_RELPOS_MAX_EDGES];
   uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
   T* table = reinterpret_cast<T*>(smem + ((2 * (2 * p.reach + 1) + 15) & ~15));       // [head of the group][row]
   const int tpr = 1 << p.log_tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x >> p.log_tpr, slots = kThreads >> p.log_tpr;
@@ -148,7 +149,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, kBwdResident / kThreads) relpos_bwd_kernel(const __grid_constant__ RelP p, const T* __restrict__ d_bias, float* __restrict__ parts) {
   constexpr int kC = kBwdCols;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int32_t tmp[MF_RELPOS_MAX_EDGES];
+  __shared__ uint16_t tmp[MF_RELPOS_MAX_EDGES];
   const int nt = blockDim.x, tid = threadIdx.x;
   const int tpr = 1 << p.log_tpr, lane = tid & (tpr - 1), slot = tid >> p.log_tpr, slots = nt >> p.log_tpr, width_max = tpr * kC;
   int32_t* kpos = reinterpret_cast<int32_t*>(smem);                                            // positions of the tile's keys
@@ -300,7 +301,7 @@ RelP relpos_params(const mf_relpos_args& a) {
   RelP p{};
   p.B = a.B; p.H = a.H; p.Lq = a.Lq; p.Lk = a.Lk; p.rows = a.rows; p.w_dtype = a.w_dtype;
   p.n_edges = a.n_edges; p.base_pos = a.base_pos; p.step_pos = a.step_pos; p.base_neg = a.base_neg; p.step_neg = a.step_neg;
-  for (int i = 0; i < a.n_edges; ++i) p.edges[i] = a.edges[i];
+  for (int i = 0; i < a.n_edges; ++i) p.edges[i] = (uint16_t)a.edges[i];
   p.reach = a.n_edges ? a.edges[a.n_edges - 1] : 0;
   if (p.reach < 1) p.reach = 1;
   p.q_pos = a.q_pos; p.k_pos = a.k_pos; p.q_seg = a.q_seg; p.k_seg = a.k_seg;

@@ -59,6 +59,11 @@ def _buckets(count: int, max_distance: int, scheme: str, bidirectional: bool):
     return tuple(edges), ((side, 1, 0, 1) if bidirectional else (0, 0, 0, 1))
 
 
+def _check_rows(rows: int):
+    if rows > MAX_ROWS:
+        raise ValueError(f"a table of at most {MAX_ROWS} rows is supported, got {rows}")
+
+
 def relative_position_bias(weight, q_positions, k_positions, *, max_distance: int, scheme: str = "log", bidirectional: bool = True, q_segments=None,
                            k_segments=None, dtype=None):
     """``[B, 1, H, Lq, Lk]``: ``weight[bucket(k_positions[b, j] - q_positions[b, i]), h]``.
@@ -69,8 +74,7 @@ def relative_position_bias(weight, q_positions, k_positions, *, max_distance: in
     (``bidirectional=False``): keys ahead of the query share the bucket of distance 0."""
     if weight.dim() != 2:
         raise ValueError(f"weight must be [rows, heads], got {tuple(weight.shape)}")
-    if weight.shape[0] > MAX_ROWS:
-        raise ValueError(f"a table of at most {MAX_ROWS} rows is supported, got {weight.shape[0]}")
+    _check_rows(weight.shape[0])
     if isinstance(q_positions, int) != isinstance(k_positions, int):
         raise TypeError("positions are two tensors or two lengths")
     edges, rows = _buckets(weight.shape[0] - (q_segments is not None), int(max_distance), scheme, bool(bidirectional))
@@ -84,6 +88,7 @@ class RelativePositionBias(nn.Module):
 
     def __init__(self, num_heads, num_buckets=32, max_distance=128, scheme="log", bidirectional=True, segments=False, device=None, dtype=None):
         super().__init__()
+        _check_rows(num_buckets + bool(segments))
         _buckets(num_buckets, max_distance, scheme, bool(bidirectional))
         self.max_distance, self.scheme, self.bidirectional, self.segments = max_distance, scheme, bool(bidirectional), segments
         self.weight = nn.Parameter(torch.empty(num_buckets + bool(segments), num_heads, device=device, dtype=dtype))
