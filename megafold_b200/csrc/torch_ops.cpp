@@ -757,6 +757,9 @@ Tensor pair_bias(const Tensor& x, const Tensor& lw, const Tensor& lb, const Tens
   return PairBiasFn::apply(x, lw, lb, w, H);
 }
 
+// Sizes for the library, which refuses those beyond its limits: what 32 bits do not hold must not come out as what is left of it.
+int32_t size_arg(int64_t x) { return (int32_t)std::min<int64_t>(x, INT32_MAX); }
+
 // ---- relative position bias ---------------------------------------------------------------------------------------------
 // The pairs' buckets in whole numbers: see mf_relpos_args.  q_pos and k_pos undefined: the queries are the last of the keys.
 struct Relpos {
@@ -799,7 +802,7 @@ Relpos relpos_plan(const Tensor& weight, const OptTensor& q_pos, const OptTensor
 }
 mf_relpos_args relpos_args(const Relpos& r, int64_t rows, int64_t H, at::ScalarType dtype) {
   mf_relpos_args a{};
-  a.B = (int32_t)r.B; a.H = (int32_t)H; a.Lq = (int32_t)r.Lq; a.Lk = (int32_t)r.Lk; a.rows = (int32_t)rows;
+  a.B = size_arg(r.B); a.H = size_arg(H); a.Lq = size_arg(r.Lq); a.Lk = size_arg(r.Lk); a.rows = size_arg(rows);
   a.dtype = dtype_code(dtype);
   a.n_edges = (int32_t)r.edges.size(); a.edges = r.edges.data();
   a.base_pos = (int32_t)r.base_pos; a.step_pos = (int32_t)r.step_pos; a.base_neg = (int32_t)r.base_neg; a.step_neg = (int32_t)r.step_neg;
@@ -868,6 +871,9 @@ struct Rotary { Tensor q, k, qw, kw, freq, pos; double eps; bool interleaved; };
 void check_rotary(const Rotary& t) {
   TORCH_CHECK_VALUE(t.q.dim() == 5 && t.k.dim() == 5, "q and k must be [B, N_seq, N_res, Head, Dim], got ", shape(t.q), " and ", shape(t.k));
   const auto &q = t.q.sizes(), &k = t.k.sizes();
+  // (the largest number of 32 bits would be a number of tokens that the library takes)
+  TORCH_CHECK(q[0] <= INT32_MAX && q[1] <= INT32_MAX && q[0] * q[1] <= INT32_MAX && q[2] <= INT32_MAX && q[0] * q[1] * q[2] <= INT32_MAX,
+              "megafold_b200: more than 2^31 - 1 tokens are not supported, got ", shape(t.q));
   TORCH_CHECK_VALUE(q[0] == k[0] && q[1] == k[1] && q[2] == k[2] && q[4] == k[4], "q and k differ in more than their heads: ", shape(t.q), " ", shape(t.k));
   TORCH_CHECK_TYPE(t.q.scalar_type() == t.k.scalar_type(), "q and k must share a dtype");
   TORCH_CHECK_VALUE(t.qw.defined() == t.kw.defined(), "queries and keys both have a weight, or neither has");
@@ -891,8 +897,8 @@ void check_rotary(const Rotary& t) {
 }
 mf_qk_rotary_args rotary_args(const Rotary& t) {
   mf_qk_rotary_args a{};
-  a.B = (int32_t)t.q.size(0); a.N = (int32_t)t.q.size(1); a.L = (int32_t)t.q.size(2); a.H = (int32_t)t.q.size(3); a.Hk = (int32_t)t.k.size(3);
-  a.D = (int32_t)t.q.size(4); a.R = (int32_t)(2 * t.freq.size(0));
+  a.B = size_arg(t.q.size(0)); a.N = size_arg(t.q.size(1)); a.L = size_arg(t.q.size(2)); a.H = size_arg(t.q.size(3)); a.Hk = size_arg(t.k.size(3));
+  a.D = size_arg(t.q.size(4)); a.R = size_arg(2 * t.freq.size(0));
   a.dtype = dtype_code(t.q.scalar_type()); a.w_dtype = t.qw.defined() ? dtype_code(t.qw.scalar_type()) : MF_F32;
   a.per_head = t.qw.defined() && t.qw.dim() == 2; a.interleaved = t.interleaved; a.eps = (float)t.eps;
   a.q = t.q.data_ptr(); a.k = t.k.data_ptr();
@@ -987,9 +993,9 @@ void check_window(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 }
 mf_window_args window_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, const Span& s, int64_t flags) {
   mf_window_args a{};
-  auto i32 = [](int64_t x) { return (int32_t)std::min<int64_t>(x, INT32_MAX); };
-  a.B = i32(q.size(0)); a.N = i32(q.size(1)); a.Lq = i32(q.size(2)); a.Lk = i32(k.size(2)); a.H = i32(q.size(3)); a.Hk = i32(k.size(3)); a.D = i32(q.size(4));
-  a.left = i32(s.left); a.right = i32(s.right); a.sinks = i32(s.sinks);
+  a.B = size_arg(q.size(0)); a.N = size_arg(q.size(1)); a.Lq = size_arg(q.size(2)); a.Lk = size_arg(k.size(2)); a.H = size_arg(q.size(3)); a.Hk = size_arg(k.size(3));
+  a.D = size_arg(q.size(4));
+  a.left = size_arg(s.left); a.right = size_arg(s.right); a.sinks = size_arg(s.sinks);
   a.dtype = dtype_code(q.scalar_type()); a.flags = (uint32_t)flags;
   a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
   for (int i = 0; i < 5; ++i) { a.q_strides[i] = q.stride(i); a.k_strides[i] = k.stride(i); a.v_strides[i] = v.stride(i); }
