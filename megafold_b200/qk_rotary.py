@@ -32,18 +32,32 @@ class QKNormRotary(nn.Module):
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim:
             raise ValueError(f"{rotary_dim} of {head_dim} elements cannot be rotated in pairs")
-        self.interleaved, self.eps = interleaved, eps
+        self.rotary_dim, self.base, self.interleaved, self.eps = rotary_dim, base, interleaved, eps
         num_key_heads = num_heads if num_key_heads is None else num_key_heads
-        self.q_weight = nn.Parameter(torch.ones(*(() if num_heads is None else (num_heads,)), head_dim, device=device, dtype=dtype))
-        self.k_weight = nn.Parameter(torch.ones(*(() if num_heads is None else (num_key_heads,)), head_dim, device=device, dtype=dtype))
-        freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(rotary_dim, 1))
-        self.register_buffer("inv_freq", freq.to(device=device, dtype=torch.float32), persistent=False)
+        self.q_weight = nn.Parameter(torch.empty(*(() if num_heads is None else (num_heads,)), head_dim, device=device, dtype=dtype))
+        self.k_weight = nn.Parameter(torch.empty(*(() if num_heads is None else (num_key_heads,)), head_dim, device=device, dtype=dtype))
+        self.register_buffer("inv_freq", self._frequencies(device), persistent=False)
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        nn.init.ones_(self.q_weight)
+        nn.init.ones_(self.k_weight)
+
+    def _frequencies(self, device):
+        # on the host, whatever device is the default at the time of a call with one
+        steps = torch.arange(0, self.rotary_dim, 2, dtype=torch.float64, device=None if device is None else "cpu")
+        freq = self.base ** (-steps / max(self.rotary_dim, 1))
+        return freq.to(device=device, dtype=torch.float32)
 
     def _apply(self, fn, recurse=True):
-        # frequencies stay float32 when the module is moved to another type
+        # Frequencies stay float32 when the module is moved to another type.  They are in no state dict: those of a module built without memory
+        # (the meta device) are computed when it gets some, by this call or by weights that load_state_dict assigned.
+        if self.inv_freq.is_meta and not self.q_weight.is_meta:
+            self.inv_freq = self._frequencies(self.q_weight.device)
         freq = self.inv_freq
         super()._apply(fn, recurse)
-        self.inv_freq = freq.to(self.inv_freq.device)
+        device = self.inv_freq.device
+        self.inv_freq = self._frequencies(device) if freq.is_meta and device.type != "meta" else freq.to(device)
         return self
 
     def forward(self, q, k, positions=None):
