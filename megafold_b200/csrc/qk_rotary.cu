@@ -155,7 +155,8 @@ __device__ __forceinline__ float row_sum(float v, int lpr) {
 // UPL: units of a thread.  Every thread of a warp takes part in each sum over a row: rows that do not exist are zeros.
 constexpr int units_per(int V) { return V >= 4 ? 1 : V == 2 ? 2 : 4; }
 // blocks of an SM ([1, 32768, 16 + 4, 128] bf16 in pieces of 16 bytes: forward 2 blocks 113 us, 3 99, 4 110; backward 1 186, 2 133, 3 233.
-// [1, 147456, 4 + 4, 32] fp32: forward 3 blocks 68, 4 60; backward 2 91, 3 93)
+// [1, 147456, 4 + 4, 32] fp32: forward 3 blocks 68, 4 60; backward 2 91, 3 93).  The registers that this leaves spill a little: 16-byte pieces of 16-bit
+// elements 24 bytes of stack forward and 24 to 32 backward, 8-byte ones 40 to 48 backward, fp32 32 forward, single elements 88 to 120 backward.
 constexpr int resident(int V, int es, bool bwd) { return units_per(V) > 1 ? 2 : V * es < 16 ? (bwd ? 3 : 4) : bwd ? 2 : es == 4 ? 4 : 3; }
 template <typename T, int V, int UPL, bool IL, bool BWD>
 __global__ void __launch_bounds__(kThreads, resident(V, sizeof(T), BWD)) qk_rotary_kernel(const __grid_constant__ RotP p) {

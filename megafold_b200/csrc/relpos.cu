@@ -7,7 +7,7 @@
 // all distances up to the last edge out in shared memory once; a pair then costs a subtraction, a clamp and a look-up,
 // shared by the heads of the block, and a second look-up a head.
 //
-// Bound: HBM writes (forward) and reads (backward).
+// Bound: HBM writes (forward with aligned rows), four- or two-byte stores (other rows), issue slots for the look-ups (backward).
 #include "common.cuh"
 
 namespace mf {

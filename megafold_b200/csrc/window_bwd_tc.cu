@@ -21,6 +21,8 @@
 // the next S is formed while the compute warps exponentiate (184 -> 168 us at 16384 tokens, 16 heads of 64, window 1024);
 // in the other one, where each barrier stands between two products, that cost more than it gave (199 -> 233).
 //
+// Two CTAs an SM leave a thread 96 registers: dK and dV at DP = 64 spill 4 (fp16) or 12 bytes of stores, dQ at DP = 128 spills 8.
+//
 // Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they, and those that no query of the tile sees, are overwritten
 // with zeros in shared memory.
 // P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  The factor D^-1/2 of dQ and dK
@@ -590,8 +592,9 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   float* delta = static_cast<float*>(a.workspace);
   uint8_t* terms = static_cast<uint8_t*>(a.workspace) + delta_bytes(p);
   // delta of a row is the sum of o d_o, o rounded to 16 bits, and dS = P (dP - delta) gets P times its error: with few keys a row, where P
-  // is large, that is as much as dS's own rounding (3 keys: dQ off by 3.2e-3 of its norm in bf16, instead of 2.4e-3; 129 keys: 2.6e-3).
-  // Up to 512 keys the dQ kernel forms it as the sum of P dP instead, in a walk of its own, which is short there.
+  // is large, that is as much as dS's own rounding.  Up to 512 keys the dQ kernel forms it as the sum of P dP instead, in a walk of its
+  // own, which is short there.  [1, 1, 3000, 2, 64] bf16, causal: dQ off by 2.4e-3 of its norm at 3, 5 and 129 keys a row; from o d_o 3.2e-3, 2.9e-3 and 2.4e-3
+  // (2.40e-3 and 2.46e-3 at 129 keys and heads of 32), dK alike.
   f.two_walks = (int64_t)p.left + p.right + 1 + p.sinks <= 512 || p.Lk <= 512;
   p.delta = f.delta = delta; f.terms = terms;
   f.parts = reinterpret_cast<float*>(terms + term_bytes(p));

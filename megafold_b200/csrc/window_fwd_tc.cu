@@ -10,9 +10,12 @@
 // in the order S(0) S(1) PV(0) S(2) PV(1) ..., so that a buffer's P has been read when the next scores go over it, and the next scores are
 // there while this block's are exponentiated.  O stays in TMEM and is brought to a new maximum only when that grew by more than
 // 2^8 in the exponent.  A window makes short walks (5 blocks at 64 + 64 keys), so nothing is pipelined across items: two CTAs share
-// an SM instead.  Tried at [1, 1, 16384, 16 on 4 heads, 64], window 1024 / [2, 1, 2048 of 6001, 16 on 4, 128], window 2047 / one token of 64
-// sequences, 32 on 8 heads of 128: this 160 / 88 / 68 us; one thread a row, one score buffer, four CTAs (two at 128 columns) 145 / 103 / 96;
-// one score buffer, two threads a row 159 / 127 / 87; blocks of 128 keys 168 / 102 / 77.
+// an SM instead.  Tried at [1, 1, 16384, 16 on 4 heads, 64], window 1024 / [2, 1, 2048 of 6001, 16 on 4, 128], window 2048 / one token of 64
+// sequences, 32 on 8 heads of 128, window 1024 / [1, 1, 4603, 4, 32], window 65: twenty calls in a row 158 / 88 / 56 / 8.7 us a call,
+// one call with its operands out of L2 168 / 97 / 72 / 14.  One thread a row, one score buffer, four CTAs (two at 128 columns): 131 / 89 / 81 / 9.8 and
+// 140 / 108 / 96 / 16, so ahead by a fifth where many tiles of up to 64 columns fill the processors four times over, and behind elsewhere: one form
+// serves all sizes, and long sequences of such heads pay for it.  One score buffer with two threads a row, and blocks of 128 keys, were no
+// better at the first size and behind at the next two (159 / 127 / 87 and 168 / 102 / 77, measured beside 160 / 88 / 68 for this).
 // Bound: the exponentials, half of the time at 64 columns (16 a clock and SM), and the waits between a block's steps.
 //
 // Blocks that a row does not see whole go through a 64-bit mask a row (window, sinks, end of the keys, key mask); rows of V whose

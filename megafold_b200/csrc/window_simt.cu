@@ -462,7 +462,7 @@ int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
       MF_LAUNCHED("window_bwd_simt_kernel");
       return MF_OK;
     };
-    // Two blocks an SM have 128 registers a thread, too few for a block alone: [2, 517, 8 : 2, 24], window 100, 61 us instead of 50, but with 8 times as many tiles
+    // Two blocks an SM have 128 registers a thread and spill (332 bytes of stores and 440 of loads at DP = 64, 184 and 240 at DP = 32), too few for a block alone: [2, 517, 8 : 2, 24], window 100, 61 us instead of 50, but with 8 times as many tiles
     // ([1, 2000, 8 : 1, 32], window 300) 137 instead of 172 and [1, 2000, 8, 64] 382 instead of 435.
     if constexpr (DP <= 64) {
       if (blocks > 3 * (int64_t)tcx::sm_count()) return launch(std::integral_constant<int, 2>{});

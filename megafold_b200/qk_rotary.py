@@ -20,7 +20,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, positions=None, eps: floa
 
     q: ``[B, N, L, H, D]``, k: ``[B, N, L, Hk, D]``; D at most 256.  q_weight, k_weight: ``[D]``, or ``[H, D]`` and ``[Hk, D]`` for a weight
     of each head, or None both.  inv_freq: float32 ``[R / 2]``, no gradient.  positions: int32 or int64 ``[L]``, ``[N, L]`` or ``[B, N, L]``;
-    None: 0, 1, ... along L.  interleaved: pairs are neighbours (2i, 2i + 1) instead of (i, i + R / 2)."""
+    None: 0, 1, ... along L.  eps: taken in 32 bits; 0 is fine for heads that are not all zeros.  interleaved: pairs are neighbours
+    (2i, 2i + 1) instead of (i, i + R / 2)."""
     return _lib.native().qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
 
 

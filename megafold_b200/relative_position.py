@@ -3,8 +3,10 @@
 ``relative_position_bias`` gives the ``[B, 1, H, Lq, Lk]`` tensor that ``TritonEvoformer`` takes as ``pair_bias``; its gradient comes
 back as the table's.  Two ways to put distances into buckets:
 
-* ``"clip"``: a bucket for each distance from ``-max_distance`` to ``max_distance``, farther ones in the outermost, as in the relative
-  position encoding of the pair representation (megafold/model/megafold.py, ``RelativePositionEncoding``);
+* ``"clip"``: a bucket for each distance from ``-max_distance`` to ``max_distance``, farther ones in the outermost.  The relative position
+  encoding of the pair representation (megafold/model/megafold.py, ``RelativePositionEncoding``) has the same buckets in the other order: it
+  clips query minus key, this key minus query.  A table that was learned there arrives mirrored: ``table[:2 * max_distance + 1].flip(0)``
+  brings its buckets into this order (a last row for other chains stays where it is);
 * ``"log"``: one bucket for each small distance, then buckets that grow by a constant ratio up to ``max_distance``; with
   ``bidirectional`` half of them for keys behind the query, half for keys before it.
 
@@ -70,7 +72,7 @@ def relative_position_bias(weight, q_positions, k_positions, *, max_distance: in
 
     weight: ``[buckets, H]``, with segments ``[buckets + 1, H]``, whose last row is that of pairs from different segments (chains).
     q_positions, k_positions: int32 or int64, ``[Lq]`` / ``[Lk]`` or ``[B, Lq]`` / ``[B, Lk]``; or two numbers, the lengths of rows whose
-    queries are the last of the keys.  dtype: of the result, ``weight.dtype`` by default.  One direction
+    queries are the last of the keys; differences of positions have to fit 64 bits.  dtype: of the result, ``weight.dtype`` by default.  One direction
     (``bidirectional=False``): keys ahead of the query share the bucket of distance 0."""
     if weight.dim() != 2:
         raise ValueError(f"weight must be [rows, heads], got {tuple(weight.shape)}")
