@@ -21,14 +21,18 @@
 // the next S is formed while the compute warps exponentiate (184 -> 168 us at 16384 tokens, 16 heads of 64, window 1024);
 // in the other one, where each barrier stands between two products, that cost more than it gave (199 -> 233).
 //
-// Two CTAs an SM leave a thread 96 registers: dK and dV at DP = 64 spill 4 (fp16) or 12 bytes of stores, dQ at DP = 128 spills 8.
+// Two CTAs an SM leave a thread 96 registers: dK and dV at DP = 64 spill 12 bytes of stores, dQ at DP = 128 spills 8 (bf16) or 16.
 //
 // Rows of masked keys: their lanes give zeros (dK, dV); as B operand of dQ they, and those that no query of the tile sees, are overwritten
 // with zeros in shared memory.
-// P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  The factor D^-1/2 of dQ and dK
-// comes last in bf16, which has the range of fp32, but goes into dS before it is rounded in fp16: with the gradients of a scaled loss, dS without
-// it overflowed up to sqrt(D) before dQ and dK did.  (In bf16, too, it cost 1 % at 16384 tokens, 16 heads of 64, window 1024: 553 -> 559 us forward
-// and backward.)  Waits are bounded as in the forward.
+// P and dS are rounded to the operands' type, the matrix instruction's; all sums are fp32.  Waits are bounded as in the forward.
+//
+// fp16 has five bits of exponent: with the gradients of a scaled loss dS overflowed up to sqrt(D) before dQ and dK did, and at small gradients and wide windows it
+// lost bits below 2^-14.  There dS is rounded with a power of two that the accumulator's write-out takes back, so that nothing else changes: in dQ one
+// a row, from the row's largest |dO|; in dK and dV's kernel one a CTA, from the largest |dS| of the rows that it walks, which the dQ kernel leaves in
+// `tops` (it runs before).  [1, 1, 3000, 2, 128] fp16, window 2048, error of dQ's norm at gradients of 1e-4 8.5e-3 -> 2.5e-3 (that of rounding the result), of 1e-3
+// 8.9e-4 -> 4e-4, of 1 3.1e-4 as before; [1, 1, 8192, 16 on 4 heads, 128], window 1024, forward and backward 551 -> 557 us.  Giving dS its factor D^-1/2 before it
+// is rounded, instead, left the small gradients ten times as far off.
 #include <type_traits>
 
 #include "window_tc_common.cuh"
@@ -44,7 +48,9 @@ constexpr int kRows = 128;          // dQ kernel: rows of queries of a CTA
 constexpr int kKB = 64;             // ... and keys of a block
 constexpr int kXB = kQB * 32;       // bytes of a block's term tile
 
-template <typename T> constexpr bool kScaledDs = std::is_same<T, __half>::value;
+template <typename T> constexpr bool kNarrow = std::is_same<T, __half>::value;          // dS needs a power of two
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ float back(float up) { return __int_as_float((254 << 23) - __float_as_int(up)); }      // 1 / up, a power of two
 
 struct BwdP {
   WinP w;
@@ -58,6 +64,7 @@ struct BwdP {
   int two_walks;            // dQ: a walk for delta first
   float* delta;             // ... which it writes here
   const uint8_t* terms;     // [packs of heads][n_blocks][kXB]
+  int* tops;                // fp16: the largest |dS| of each CTA of the dQ kernel, as bits of a float
   float* parts;
   int* status;
 };
@@ -249,6 +256,15 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
     // queries [a, z] see key j
     const int a = j - p.right - p.off, z = j < p.sinks ? p.Lq : j + p.left - p.off;
     const int a_all = j0 + kKeys - 1 - p.right - p.off, z_all = j0 + kKeys <= p.sinks ? p.Lq : j0 + p.left - p.off;       // every key of the tile
+    float up = 1.f;                               // dS's power of two: the largest |dS| comes to 2^13 .. 2^14
+    if constexpr (kNarrow<T>) {
+      const int nr = queries_of<kRows>(p), q0 = lo / nr, nt = hi > lo ? (hi + nr - 1) / nr - q0 : 0, packs = p.G / p.pack;
+      int top = 0;
+      for (int e = lane; e < nt * packs; e += 32)
+        top = max(top, __ldg(f.tops + (int64_t)(f.n_qt - 1 - q0 - e % nt) * f.groups + bn * head_groups(p) + hk * packs + e / nt));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (top > 0 && top < 0x7f800000) up = pow2(13 - clamp_i((top >> 23) - 127, -40, 40));
+    }
     int blk = first + e0 % per_pack;
     for (int t = 0; t < T_; ++t) {
       const int i0 = blk * nq;
@@ -273,7 +289,7 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
         float2 pr = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(f.c1, f.c1));
         pr = make_float2(ex2f(pr.x), ex2f(pr.y));
         float2 dp = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
-        if constexpr (kScaledDs<T>) dp = mul2(dp, make_float2(p.scale, p.scale));
+        if constexpr (kNarrow<T>) dp = mul2(dp, make_float2(up, up));
         float2 ds = mul2(pr, dp);
         if (!whole) {
           if (!(bits >> e & 1)) pr.x = ds.x = 0.f;
@@ -295,6 +311,7 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
       const uint32_t acc = (half ? tV : tK) + lanes;
       if (x < f.plan.split_x) {
         float* out = part_of<kKeys>(f.parts, f.plan, p, head, x) + (half * kKeys + r) * p.D;
+        const float f1 = half ? 1.f : back(up);
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           if (c * 32 >= p.D) break;
@@ -303,8 +320,8 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (c * 32 + e < p.D)
-              *reinterpret_cast<float4*>(out + c * 32 + e) = T_ > 0 ? make_float4(__uint_as_float(o32[e]), __uint_as_float(o32[e + 1]), __uint_as_float(o32[e + 2]),
-                                                                                  __uint_as_float(o32[e + 3]))
+              *reinterpret_cast<float4*>(out + c * 32 + e) = T_ > 0 ? make_float4(__uint_as_float(o32[e]) * f1, __uint_as_float(o32[e + 1]) * f1,
+                                                                                  __uint_as_float(o32[e + 2]) * f1, __uint_as_float(o32[e + 3]) * f1)
                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       } else {
@@ -312,7 +329,7 @@ window_dkv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_consta
         if (T_ > 0) {
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c)
-            if (c * 32 < p.D) store_rows<T>(acc + c * 32, half || kScaledDs<T> ? 1.f : p.scale, out + c * 32, (int64_t)p.Hk * p.D, j, p.Lk, p.D - c * 32);
+            if (c * 32 < p.D) store_rows<T>(acc + c * 32, half ? 1.f : p.scale * back(up), out + c * 32, (int64_t)p.Hk * p.D, j, p.Lk, p.D - c * 32);
         } else if (j < p.Lk) {
           for (int e = 0; e < p.D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -350,11 +367,11 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
   __shared__ QBars<NS> bar;
   __shared__ float sums[2][kRows];
   __shared__ uint32_t tmem_base_s;
-  __shared__ int abort_s;
+  __shared__ int abort_s, top_s;
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   if (tid == 0) {
-    abort_s = 0;
+    abort_s = top_s = 0;
     mbar_init(&bar.q_full, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&bar.kv_full[i], 1); mbar_init(&bar.kv_empty[i], 1); }
     mbar_init(&bar.s_ready, 1); mbar_init(&bar.d_ready, 1); mbar_init(&bar.s_read, kCompute); mbar_init(&bar.ds_written, kCompute); mbar_init(&bar.summed, kCompute); mbar_init(&bar.done, 1);
@@ -445,12 +462,30 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
     const int half = warp >> 2, r = (warp & 3) * 32 + lane, l_ = r / p.pack, i = i0 + l_, h = h0 + r - l_ * p.pack, at = i + p.off;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const bool live = l_ < nq && i < p.Lq;
-    float lse = -INFINITY, minus = 0.f;           // minus: -delta, with dS's factor
-    const float factor = kScaledDs<T> ? p.scale : 1.f;
+    float up = 1.f, top = 0.f;                    // dS's power of two; the largest |dS| so far, with it
+    if constexpr (kNarrow<T>) {
+      if (T_ > 0) {
+        // the row's largest |dO| comes to 4 .. 8, so that V may be some hundreds before dS overflows; bytes of a row stay in it when they are swizzled
+        wait_or_flag(&bar.q_full, 0, abort_flag);
+        uint32_t most = 0;
+#pragma unroll
+        for (int pn = 0; pn < G::PANELS; ++pn)
+#pragma unroll
+          for (int e = 0; e < G::ROWB / 16; ++e) {
+            // (each lane of eight begins at another piece: other banks)
+            const int piece = (e + (G::ROWB == 128 ? lane : lane >> 1)) % (G::ROWB / 16);
+            const uint4 g = *reinterpret_cast<const uint4*>(sG + pn * kRows * G::ROWB + r * G::ROWB + piece * 16);
+            most = __vmaxu2(__vmaxu2(most, __vmaxu2(g.x & 0x7fff7fffu, g.y & 0x7fff7fffu)), __vmaxu2(g.z & 0x7fff7fffu, g.w & 0x7fff7fffu));
+          }
+        const int m = max((int)(most & 0xffffu), (int)(most >> 16));
+        if (m > 0 && m < 0x7c00) up = pow2(2 - (m >= 0x400 ? (m >> 10) - 15 : 7 - __clz(m)));
+      }
+    }
+    float lse = -INFINITY, minus = 0.f;           // minus: -delta, with dS's power of two
     const int64_t stat = ((int64_t)bn * p.H + h) * p.Lq + i;
     if (live) {
       lse = p.lse[stat];
-      if (!f.two_walks) minus = -p.delta[stat] * factor;
+      if (!f.two_walks) minus = -p.delta[stat] * up;
     }
     float sum = 0.f;                              // of P dP over this thread's columns
     const float off = lse == -INFINITY ? -INFINITY : -lse * kLog2e;       // a row that sees nothing: probability 0
@@ -475,7 +510,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
         if (__any_sync(0xffffffffu, *abort_flag)) break;
         const float delta = sum + sums[half ^ 1][r];
         if (half == 0 && live) f.delta[stat] = delta;
-        minus = -delta * factor;
+        minus = -delta * up;
       }
       wait_or_flag(&bar.s_ready, t & 1, abort_flag);
       if (__any_sync(0xffffffffu, *abort_flag)) break;
@@ -489,7 +524,7 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       mbar_arrive(&bar.s_read);
       const bool whole = all_seen(p, i0 + p.off, i1 - 1 + p.off, j0, j0 + 32) && keep == ~0u;
       const uint32_t bits = whole ? ~0u : seen32(p, at, j0) & keep;
-      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off), f2 = make_float2(factor, factor), d2 = make_float2(minus, minus);
+      const float2 c2 = make_float2(f.c1, f.c1), o2 = make_float2(off, off), u2 = make_float2(up, up), d2 = make_float2(minus, minus);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, o2);
@@ -520,11 +555,12 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
       uint32_t w[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
-        float2 ds = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fma2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), f2, d2));
+        float2 ds = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), fma2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), u2, d2));
         if (!whole) {
           if (!(bits >> e & 1)) ds.x = 0.f;
           if (!(bits >> (e + 1) & 1)) ds.y = 0.f;
         }
+        if constexpr (kNarrow<T>) top = max3f(top, fabsf(ds.x), fabsf(ds.y));
         w[e / 2] = Pack2<T>::pack(ds.x, ds.y);
       }
       tmem_st16(tD, w);
@@ -556,16 +592,21 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c)            // the two warps of a set of lanes take alternate columns
           if (c % 2 == half % (DP / 32 > 1 ? 2 : 1) && (DP > 32 || half == 0) && c * 32 < p.D)
-            store_rows_at<T>(tQ + lanes + c * 32, kScaledDs<T> ? 1.f : p.scale, live ? out + c * 32 : nullptr, p.D - c * 32);
+            store_rows_at<T>(tQ + lanes + c * 32, p.scale * back(up), live ? out + c * 32 : nullptr, p.D - c * 32);
       } else if (live && half == 0) {
         for (int e = 0; e < p.D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0u, 0u, 0u, 0u);
         if (f.two_walks) f.delta[stat] = 0.f;
       }
     }
+    if constexpr (kNarrow<T>) {
+      const int most = __reduce_max_sync(0xffffffffu, live ? __float_as_int(top * back(up)) : 0);
+      if (lane == 0) atomicMax(&top_s, most);
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && abort_s) *reinterpret_cast<volatile int*>(f.status) = 1;
+  if (kNarrow<T> && tid == 0) f.tops[blockIdx.x] = top_s;
   if (warp == 0) tmem_dealloc(t0, C::COLS);
 }
 
@@ -574,6 +615,11 @@ window_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constan
 KeyPlan tc_plan(const WinP& p) { return key_plan<kKeys, kQB>(p, 2 * sm_count()); }
 int block_count(const WinP& p) { const int q = queries_of<kQB>(p); return (p.Lq + q - 1) / q; }
 size_t delta_bytes(const WinP& p) { return align_up(sizeof(float) * (size_t)p.B * p.N * p.H * p.Lq, 256); }
+// dQ: tiles of queries of a pack of heads
+int query_tiles(const WinP& p) { const int q = queries_of<kRows>(p); return (p.Lq + q - 1) / q; }
+size_t top_bytes(const WinP& p, int dtype) {
+  return dtype == MF_F16 ? align_up(sizeof(int) * (size_t)query_tiles(p) * p.B * p.N * head_groups(p), 256) : 0;
+}
 size_t term_bytes(const WinP& p) { return (size_t)p.B * p.N * head_groups(p) * block_count(p) * kXB; }
 
 template <int DP, typename T>
@@ -585,7 +631,7 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   f.plan = tc_plan(p);
   f.n_blocks = block_count(p);
   const int nq = queries_of<kRows>(p), nb = queries_of<kQB>(p);
-  f.n_qt = (a.Lq + nq - 1) / nq; f.groups = a.B * a.N * head_groups(p);
+  f.n_qt = query_tiles(p); f.groups = a.B * a.N * head_groups(p);
   f.q_bytes = nb * p.pack * DP * 2; f.qt_bytes = nq * p.pack * DP * 2;
   f.c1 = kLog2e / sqrtf((float)a.D);
   f.fmt = a.dtype == MF_BF16 ? 1u : 0u;
@@ -597,7 +643,8 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   // (2.40e-3 and 2.46e-3 at 129 keys and heads of 32), dK alike.
   f.two_walks = (int64_t)p.left + p.right + 1 + p.sinks <= 512 || p.Lk <= 512;
   p.delta = f.delta = delta; f.terms = terms;
-  f.parts = reinterpret_cast<float*>(terms + term_bytes(p));
+  f.tops = reinterpret_cast<int*>(terms + term_bytes(p));
+  f.parts = reinterpret_cast<float*>(terms + term_bytes(p) + top_bytes(p, a.dtype));
   f.status = status_word();
   MF_REQUIRE(f.status, MF_ERR_CUDA, "could not allocate the device status word");
   MF_REQUIRE(tc_async_status() == 0, MF_ERR_CUDA, "an earlier tensor-core kernel gave up on a bounded wait; results are invalid");
@@ -640,7 +687,7 @@ int launch(const mf_window_args& a, cudaStream_t st) {
   }
   dkv<<<(unsigned)grid_kv, kThreads, KvCfg<DP>::SMEM, st>>>(mk, mv, mq64, mg64, f);
   MF_LAUNCHED("window_dkv_tc_kernel");
-  return window_join<T, kKeys, kQB>(p, f.plan, f.parts, kScaledDs<T> ? 1.f : p.scale, st);
+  return window_join<T, kKeys, kQB>(p, f.plan, f.parts, st);
 }
 template <typename T>
 int by_size(const mf_window_args& a, cudaStream_t st) {
@@ -655,7 +702,7 @@ bool window_bwd_tc_supported(const mf_window_args& a) {
 }
 size_t window_bwd_tc_workspace(const mf_window_args& a) {
   const win::WinP p = win::window_params(a);
-  return win::delta_bytes(p) + win::term_bytes(p) + sizeof(float) * win::part_floats<win::kKeys>(win::tc_plan(p), p);
+  return win::delta_bytes(p) + win::term_bytes(p) + win::top_bytes(p, a.dtype) + sizeof(float) * win::part_floats<win::kKeys>(win::tc_plan(p), p);
 }
 int window_bwd_tc(const mf_window_args& a, cudaStream_t st) {
   return a.dtype == MF_BF16 ? win::by_size<__nv_bfloat16>(a, st) : win::by_size<__half>(a, st);

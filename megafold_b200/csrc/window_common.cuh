@@ -134,10 +134,9 @@ __device__ __forceinline__ float* part_of(float* parts, const KeyPlan& c, const 
 }
 
 // Adds the parts of the tiles that were split, a thread an element; blockIdx.x enumerates (head of all sequences, tile, piece of 256 elements).
-// (With a block a tile a long sequence's tile of sinks, 28 parts of it, took 163 us.)  dk_scale: what the parts of dK still lack.
+// (With a block a tile a long sequence's tile of sinks, 28 parts of it, took 163 us.)
 template <typename T, int KT, int QB>
-__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinP p, const KeyPlan c, const float* __restrict__ parts, int tiles, int pieces,
-                                                          float dk_scale) {
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WinP p, const KeyPlan c, const float* __restrict__ parts, int tiles, int pieces) {
   const int unit = blockIdx.x / pieces, tile = unit % tiles, nc = tile < c.n_sink ? c.nc_sink : c.nc_rest;
   const int x0 = tile < c.n_sink ? tile * c.nc_sink : c.n_sink * c.nc_sink + (tile - c.n_sink) * c.nc_rest;
   const int e = (blockIdx.x - unit * pieces) * 256 + threadIdx.x;
@@ -152,16 +151,16 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   float s = 0.f;
 #pragma unroll 8
   for (int k = 0; k < used; ++k) s += src[k * step];
-  if (which == 0) s *= dk_scale;
+  if (which == 0) s *= p.scale;
   static_cast<T*>(which ? p.dv : p.dk)[((bn * p.Lk + j) * p.Hk + (head - bn * p.Hk)) * p.D + d] = from_f<T>(s);
 }
 template <typename T, int KT, int QB>
-int window_join(const WinP& p, const KeyPlan& c, const float* parts, float dk_scale, cudaStream_t st) {
+int window_join(const WinP& p, const KeyPlan& c, const float* parts, cudaStream_t st) {
   if (!c.split_x) return MF_OK;
   const int tiles = c.nc_rest > 1 ? c.n_tiles : c.n_sink, pieces = (2 * KT * p.D + 255) / 256;
   const int64_t blocks = (int64_t)p.B * p.N * p.Hk * tiles * pieces;
   MF_REQUIRE(blocks <= 0x7fffffff, MF_ERR_UNSUPPORTED, "%d tiles of keys in parts are more than one launch takes", tiles);
-  window_join_kernel<T, KT, QB><<<(unsigned)blocks, 256, 0, st>>>(p, c, parts, tiles, pieces, dk_scale);
+  window_join_kernel<T, KT, QB><<<(unsigned)blocks, 256, 0, st>>>(p, c, parts, tiles, pieces);
   MF_LAUNCHED("window_join_kernel");
   return MF_OK;
 }

@@ -470,7 +470,7 @@ int run_bwd(const WinP& p, const KeyPlan& c, float* parts, cudaStream_t st) {
     return launch(std::integral_constant<int, 1>{});
   };
   int r = p.D <= 32 ? go(std::integral_constant<int, 32>{}) : p.D <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
-  return r ? r : window_join<T, kTile, kTile>(p, c, parts, p.scale, st);
+  return r ? r : window_join<T, kTile, kTile>(p, c, parts, st);
 }
 
 bool rows_vec(const void* ptr, const int64_t* s, int D, size_t es) {
